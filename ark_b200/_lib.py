@@ -66,6 +66,30 @@ class OptStatus(ctypes.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_}
 
 
+class Act8(ctypes.Structure):
+    """ark_act8."""
+    _fields_ = [("data", c_p), ("scale", c_p), ("rows", c_u64), ("cols", c_u64), ("kind", c_i32),
+                ("reserved", c_u32)]
+
+
+ARK_ROPE_MAX_DIM = 256
+
+
+class RopePlan(ctypes.Structure):
+    """ark_rope_plan."""
+    _fields_ = [("rotary_dim", c_u32), ("interleaved", c_u32), ("gain", c_f), ("reserved", c_u32),
+                ("turns", c_u64 * (ARK_ROPE_MAX_DIM // 2))]
+
+
+class Heads(ctypes.Structure):
+    """ark_heads."""
+    _fields_ = [("data", c_p), ("heads", c_u64), ("token_stride", c_u64), ("head_stride", c_u64)]
+
+
+_p_act8, _p_plan, _p_heads = (ctypes.POINTER(Act8), ctypes.POINTER(RopePlan),
+                              ctypes.POINTER(Heads))
+
+
 # every symbol include/ark_opt.h declares, with its ctypes signature
 SIGNATURES = {
     "ark_asm_adam_step_f16": (None, [c_p, c_p, c_p, c_p, c_u64, c_f, c_f, c_f, c_f, c_f, c_u32]),
@@ -107,6 +131,27 @@ SIGNATURES = {
     "ark_cuda_nccl_unique_id": (c_i, [c_p]),
     "ark_cuda_nccl_comm_init": (c_i, [c_i, c_i, c_p, c_i, ctypes.POINTER(c_p)]),
     "ark_cuda_nccl_comm_destroy": (c_i, [c_p]),
+    "ark_cuda_act8_pitch": (c_u64, [c_u64]),
+    "ark_cuda_act8_pack": (c_i, [c_p, c_i32, c_u64, _p_act8, c_p]),
+    "ark_cuda_act8_unpack": (c_i, [_p_act8, c_p, c_i32, c_u64, c_p]),
+    "ark_cuda_weight_grad_workspace": (c_u64, [c_u64, c_p, c_u64, c_u64]),
+    "ark_cuda_weight_grad": (c_i, [_p_act8, c_p, c_i32, c_u64, c_u64, c_p, c_i32, c_u64, c_i32, c_p,
+                                   c_u64, c_p]),
+    "ark_cuda_swiglu": (c_i, [c_p, c_u64, c_p, c_u64, c_i32, c_u64, c_u64, c_p, c_u64, _p_act8,
+                              _p_act8, c_p]),
+    "ark_cuda_swiglu_backward": (c_i, [c_p, c_u64, c_i32, _p_act8, _p_act8, c_p, c_u64, c_p, c_u64,
+                                       _p_act8, c_p]),
+    "ark_cuda_rope_plan": (c_i, [_p_plan, c_u32, c_u32, c_d, c_u32, c_d, c_d, c_d, c_d]),
+    "ark_cuda_rope": (c_i, [_p_plan, _p_heads, _p_heads, _p_heads, _p_heads, c_i32, c_u64, c_u64,
+                            c_p, c_i32, c_u64, c_i32, c_p]),
+    "ark_cuda_qk_norm_rope": (c_i, [_p_plan, _p_heads, _p_heads, _p_heads, _p_heads, c_i32, c_u64,
+                                    c_u64, c_p, c_p, c_i32, c_f, c_p, c_i32, c_u64, _p_act8,
+                                    _p_act8, c_p]),
+    "ark_cuda_qk_norm_rope_workspace": (c_u64, [c_u64]),
+    "ark_cuda_qk_norm_rope_backward": (c_i, [_p_plan, _p_heads, _p_heads, _p_heads, _p_heads, c_i32,
+                                             c_u64, c_u64, _p_act8, _p_act8, _p_heads, _p_heads,
+                                             c_p, c_p, c_i32, c_f, c_p, c_i32, c_u64, c_p, c_p,
+                                             c_i32, c_i32, c_p, c_u64, c_p]),
     "ark_synth_f16": (c_i, [c_p, c_u64, c_u64, c_u64, c_u64, c_f, c_f, c_u32, c_f, c_p]),
     "ark_synth_f32": (c_i, [c_p, c_u64, c_u64, c_u64, c_u64, c_f, c_i, c_p]),
 }

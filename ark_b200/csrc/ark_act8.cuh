@@ -1,0 +1,246 @@
+// ark_act8.cuh -- building blocks of the activation kernels: 8-element loads
+// and stores of FP16 / BF16 / FP32 rows, and the 8-bit checkpoint format.
+//
+// Checkpoint of a [rows, cols] activation: one byte per element in rows of
+// `pitch` bytes (cols rounded up to 128, so that every row starts on a
+// 128-byte boundary and its scale bytes on a 4-byte one), and one scale byte
+// per 32 columns.  The scale is a power of two 2^k, k the smallest integer >=
+// -126 with max|x| <= top * 2^k (top: 448 for e4m3, 127 for int8); the scale
+// byte is k + 127.  A power of two makes x * 2^-k and q * 2^k exact in FP32,
+// so the only rounding of the format is the one to 8 bits (nearest even), the
+// bytes do not depend on who computes them, and the matrix kernel can turn a
+// byte back into an FP16 / BF16 operand without a second rounding.  Against a
+// scale max|x| / top it costs int8 half a bit on average and e4m3 nothing.
+// A block that holds an infinity or a NaN gets scale byte 255 and bytes 0 and
+// reads back as NaN: an overflowed forward still makes the step a skipped one.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "ark_device.cuh"
+#include "ark_internal.h"
+
+namespace ark {
+
+constexpr int kActBlock = 32;    // columns per scale
+constexpr int kActPitch = 128;   // row pitch granule in bytes
+constexpr uint32_t kActBad = 255;
+
+enum : int { kE4M3 = ARK_ACT8_E4M3, kInt8 = ARK_ACT8_INT8 };
+
+__host__ __device__ inline uint64_t act8_pitch(uint64_t cols) {
+    return (cols + kActPitch - 1) / kActPitch * kActPitch;
+}
+
+// ------------------------------------------------------------ element types
+template <class T>
+struct Elem;
+template <>
+struct Elem<__half> {
+    static constexpr float kMax = 65504.0f;
+    static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr float kMax = 3.38953138925153547590e38f;
+    static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
+};
+template <>
+struct Elem<float> {
+    static constexpr float kMax = 3.40282346638528859812e38f;
+    static __device__ __forceinline__ float to_f(float x) { return x; }
+    static __device__ __forceinline__ float from_f(float x) { return x; }
+};
+
+// finite values saturate at the type's largest, a NaN stays one
+template <class T>
+__device__ __forceinline__ float saturate(float x) {
+    x = x > Elem<T>::kMax ? Elem<T>::kMax : x;
+    return x < -Elem<T>::kMax ? -Elem<T>::kMax : x;
+}
+
+__device__ __forceinline__ void widen2(uint32_t w, float& a, float& b, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x;
+    b = f.y;
+}
+__device__ __forceinline__ void widen2(uint32_t w, float& a, float& b, __nv_bfloat16) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// N consecutive elements (N = 4 or 8) at an address aligned to their size
+template <int N>
+__device__ __forceinline__ void load_vec(const float* p, float* v) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(p + i);
+        v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+    }
+}
+template <int N, class T>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+    if constexpr (N == 8) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p);
+        widen2(q.x, v[0], v[1], T());
+        widen2(q.y, v[2], v[3], T());
+        widen2(q.z, v[4], v[5], T());
+        widen2(q.w, v[6], v[7], T());
+    } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(p);
+        widen2(q.x, v[0], v[1], T());
+        widen2(q.y, v[2], v[3], T());
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_vec(float* p, const float* v) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+        *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+}
+template <int N, class T>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+    if constexpr (N == 8)
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(narrow2(v[0], v[1], T()), narrow2(v[2], v[3], T()),
+                       narrow2(v[4], v[5], T()), narrow2(v[6], v[7], T()));
+    else
+        *reinterpret_cast<uint2*>(p) = make_uint2(narrow2(v[0], v[1], T()), narrow2(v[2], v[3], T()));
+}
+
+// 8 elements of a row of which the first n are there (the others read as 0)
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float* v) {
+    if (vec && n >= 8) {
+        load_vec<8>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? Elem<T>::to_f(p[i]) : 0.0f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float* v) {
+    if (vec && n >= 8) {
+        store_vec<8>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = Elem<T>::from_f(v[i]);
+    }
+}
+
+// ------------------------------------------------------------ the 8-bit format
+template <int N>
+__device__ __forceinline__ uint32_t abs_max(const float* v) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+}
+
+// The block's scale byte from the bits of its largest magnitude.  448 is
+// 1.75 * 2^8 and 127 is 1.984375 * 2^6: adding the mantissa's distance to the
+// next power of two carries into the exponent exactly when 2^k must be one larger.
+template <int KIND>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+    if (amax_bits >= 0x7F800000u) return kActBad;
+    const int b = KIND == kE4M3 ? (int)((amax_bits + 0x1FFFFFu) >> 23) - 8
+                                : (int)((amax_bits + 0x01FFFFu) >> 23) - 6;
+    return (uint32_t)max(b, 1);
+}
+// 2^-k for a scale byte of 1 to 253
+__device__ __forceinline__ float inv_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^k; NaN for the byte of a block that held an infinity or a NaN
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return byte == kActBad ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
+}
+
+// Four values to four bytes, nearest even.
+template <int KIND>
+__device__ __forceinline__ uint32_t quant4(const float* v, float inv) {
+    if constexpr (KIND == kE4M3) {
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+            : "=h"(lo)
+            : "f"(__fmul_rn(v[1], inv)), "f"(__fmul_rn(v[0], inv)));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+            : "=h"(hi)
+            : "f"(__fmul_rn(v[3], inv)), "f"(__fmul_rn(v[2], inv)));
+        return pack16(lo, hi);
+    } else {
+        // |v * inv| <= 127: adding 1.5 * 2^23 rounds to the nearest even
+        // integer, whose two's complement is then the low byte
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], inv), 12582912.0f));
+        return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+    }
+}
+
+// Eight values of a block with scale byte `byte`.
+template <int KIND>
+__device__ __forceinline__ uint2 quant8(const float* v, uint32_t byte) {
+    if (byte == kActBad) return make_uint2(0u, 0u);
+    const float inv = inv_scale(byte);
+    return make_uint2(quant4<KIND>(v, inv), quant4<KIND>(v + 4, inv));
+}
+
+// Four bytes back to the integers or e4m3 values that they hold (not scaled).
+template <int KIND>
+__device__ __forceinline__ void bytes4(uint32_t w, float* v) {
+    if constexpr (KIND == kE4M3) {
+        uint32_t lo, hi;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((uint16_t)(w & 0xFFFFu)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((uint16_t)(w >> 16)));
+        widen2(lo, v[0], v[1], __half());
+        widen2(hi, v[2], v[3], __half());
+    } else {
+        // byte ^ 0x80 is q + 128; as the low mantissa byte of 2^23 it is 2^23 + q + 128
+        const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)), 8388736.0f);
+    }
+}
+template <int KIND>
+__device__ __forceinline__ void dequant8(uint2 w, uint32_t byte, float* v) {
+    const float s = scale_of(byte);
+    bytes4<KIND>(w.x, v);
+    bytes4<KIND>(w.y, v + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], s);
+}
+
+// ------------------------------------------------------------ host checks
+inline uint64_t type_size(int32_t type) {
+    return type == ARK_TYPE_F32 ? 4u : (type == ARK_TYPE_F16 || type == ARK_TYPE_BF16) ? 2u : 0u;
+}
+inline bool aligned_to(const void* p, uint64_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+// f called with a value of the element type
+template <class F>
+int by_type(int32_t type, F f) {
+    if (type == ARK_TYPE_F16) return f(__half());
+    if (type == ARK_TYPE_BF16) return f(__nv_bfloat16());
+    if (type == ARK_TYPE_F32) return f(float());
+    return ARK_E_INVALID_ARG;
+}
+
+// null data is fine for an empty checkpoint
+int act8_check(const ark_act8* c);
+
+}  // namespace ark

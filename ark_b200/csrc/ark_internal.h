@@ -36,6 +36,9 @@ __host__ __device__ inline bool aligned16(const void* p) {
 // with as many resident blocks as the kernel's occupancy allows.
 int streaming_grid(const void* kernel, int threads, size_t dyn_smem, uint64_t work_items);
 
+// SMs of the current device.
+int sm_count();
+
 // What the checkpoint code needs of an optimizer state (ark_step.cu).
 struct OptView {
     int device, rank, world;

@@ -88,7 +88,7 @@ static uint64_t resident_capacity(const void* kernel, int threads, size_t dyn_sm
 }
 
 // SMs of the current device (looked up once per device).
-static int sm_count() {
+int sm_count() {
     static std::atomic<int> cache[64];
     int dev = 0;
     cudaGetDevice(&dev);

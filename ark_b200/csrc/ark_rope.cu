@@ -1,0 +1,790 @@
+// ark_rope.cu -- rotary positions of queries and keys, alone or in one pass
+// with the RMS norm of each head; the backward of both.
+//
+//   n = x * rsqrt(mean(x^2) + eps) * gain            (norm, over one head's dim)
+//   y1 = n1 cos - n2 sin, y2 = n2 cos + n1 sin       (each rotated pair)
+//
+// Backward: u = the inverse rotation of dy; h = x * r with r the rsqrt;
+//   dgain = sum over tokens and heads of u * h,  dx = r * (u gain - h * mean(u gain h)).
+//
+// Angles.  A plan holds each pair's turns per position as a 64-bit fraction of
+// a turn, so position * fraction wraps exactly at whole turns: the angle of a
+// position in the millions is as good as that of the first ones, with one
+// integer product and no table in memory.
+//
+// HBM bounds both passes.  One CTA takes a few tokens at a time: the cosines
+// and sines of their pairs are formed once into shared memory, then groups of
+// lanes each take whole heads.  A lane owns two chunks of VEC elements that
+// hold whole pairs (for the half layout one chunk of each half), so a pair is
+// rotated in one lane, and the same chunks of every head, so gains and the
+// gains' gradients stay with the lane.
+#include <math.h>
+#include <string.h>
+
+#include "ark_act8.cuh"
+
+namespace ark {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxDim = ARK_ROPE_MAX_DIM;
+
+struct Heads {
+    void* p;
+    uint64_t heads, ts, hs;   // element strides of tokens and heads
+};
+
+// How a head's elements are dealt to lanes.
+struct Deal {
+    uint32_t dim, rot, half;       // half: pairs per head
+    uint32_t group;                // lanes per head, a power of two
+    uint32_t units, rot_units;     // chunk pairs of a head, and those that are rotated
+    int interleaved;
+};
+
+struct Args {
+    ark_rope_plan plan;
+    Deal d;
+    const void* pos;
+    int pos64, inverse;
+    uint64_t tokens, seq;
+    uint32_t per_block;            // tokens of a CTA at a time
+    Heads q, k, oq, ok;            // inputs (x or dy) and outputs
+    const void *gq, *gk;
+    int gain_type;
+    float eps;
+    // checkpoints: written by the forward, read by the backward
+    uint8_t *q8, *sq, *k8, *sk;
+    uint64_t pq, pk;               // pitches in bytes
+    int kind;                      // ARK_ACT8_*, or -1: x comes from xq / xk
+    Heads xq, xk;
+    float* partial;                // backward: [q blocks + k blocks][dim]
+    uint32_t q_blocks;
+};
+
+__device__ __forceinline__ float gain_at(const void* g, int type, uint32_t i) {
+    if (type == ARK_TYPE_F32) return static_cast<const float*>(g)[i];
+    if (type == ARK_TYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]);
+    return __half2float(static_cast<const __half*>(g)[i]);
+}
+
+// position of a token; negative: padding
+__device__ __forceinline__ int64_t position(const Args& a, uint64_t t) {
+    if (!a.pos) return (int64_t)(t % a.seq);
+    return a.pos64 ? static_cast<const long long*>(a.pos)[t]
+                   : (int64_t) static_cast<const int*>(a.pos)[t];
+}
+
+// cos and sin (times the plan's gain) of the pairs of `count` tokens from t0
+__device__ __forceinline__ void angles(const Args& a, const uint64_t* turns, uint64_t t0,
+                                       uint32_t count, float2* cs) {
+    for (uint32_t i = threadIdx.x; i < count * a.d.half; i += kThreads) {
+        const uint32_t t = i / a.d.half, j = i - t * a.d.half;
+        const int64_t p = position(a, t0 + t);
+        // the top 32 bits of the turn, signed: [-1/2, 1/2) of a turn
+        const int32_t top = (int32_t)(((uint64_t)p * turns[j]) >> 32);
+        float s, c;
+        sincospif(__fmul_rn((float)top, 4.656612873077392578125e-10f), &s, &c);
+        if (a.inverse) s = -s;
+        cs[i] = make_float2(__fmul_rn(c, a.plan.gain), __fmul_rn(s, a.plan.gain));
+    }
+}
+
+// the two chunks of unit u: where they start and whether they are there
+template <int VEC>
+__device__ __forceinline__ void chunks(const Deal& d, uint32_t u, uint32_t& o1, uint32_t& o2,
+                                       bool& h1, bool& h2, bool& turned) {
+    turned = u < d.rot_units;
+    if (turned && !d.interleaved) {
+        o1 = u * VEC;
+        o2 = d.half + u * VEC;
+    } else {
+        o1 = turned ? u * 2 * VEC : d.rot + (u - d.rot_units) * 2 * VEC;
+        o2 = o1 + VEC;
+    }
+    h1 = u < d.units && o1 < d.dim;
+    h2 = u < d.units && o2 < d.dim;
+}
+
+template <int VEC, class T>
+__device__ __forceinline__ void load_chunk(const T* p, bool there, float* v) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
+    if (!there) return;
+    if constexpr (VEC == 1)
+        v[0] = Elem<T>::to_f(*p);
+    else
+        load_vec<VEC>(p, v);
+}
+template <int VEC, class T>
+__device__ __forceinline__ void store_chunk(T* p, bool there, const float* v) {
+    if (!there) return;
+    if constexpr (VEC == 1)
+        *p = Elem<T>::from_f(v[0]);
+    else
+        store_vec<VEC>(p, v);
+}
+
+// rotate the pairs of a unit in place: x holds chunk 1 then chunk 2
+template <int VEC>
+__device__ __forceinline__ void rotate(const Deal& d, const float2* cs, uint32_t u, float* x) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        const int p = d.interleaved ? 2 * i : i, q = d.interleaved ? 2 * i + 1 : i + VEC;
+        const float2 c = cs[u * VEC + i];
+        const float a = x[p], b = x[q];
+        x[p] = __fmaf_rn(a, c.x, -__fmul_rn(b, c.y));
+        x[q] = __fmaf_rn(b, c.x, __fmul_rn(a, c.y));
+    }
+}
+
+__device__ __forceinline__ float group_sum(float v, uint32_t group) {
+    for (uint32_t o = group >> 1; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+// Checkpoint the two chunks of 8 of a lane.  A scale block is 4 lanes' chunks
+// of one half (half layout), or both chunks of 2 lanes.
+template <int KIND>
+__device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col, uint32_t o1,
+                                     uint32_t o2, bool there, const float* x) {
+    uint32_t m1 = there ? abs_max<8>(x) : 0, m2 = there ? abs_max<8>(x + 8) : 0;
+    const bool next = o2 == o1 + 8;
+    if (next) m1 = m2 = max(m1, m2);
+    m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, 1));
+    m2 = max(m2, __shfl_xor_sync(0xFFFFFFFFu, m2, 1));
+    const uint32_t n1 = __shfl_xor_sync(0xFFFFFFFFu, m1, 2), n2 = __shfl_xor_sync(0xFFFFFFFFu, m2, 2);
+    if (!next) m1 = max(m1, n1), m2 = max(m2, n2);
+    if (!there) return;
+    const uint32_t b1 = scale_byte<KIND>(m1), b2 = scale_byte<KIND>(m2);
+    *reinterpret_cast<uint2*>(data + col + o1) = quant8<KIND>(x, b1);
+    *reinterpret_cast<uint2*>(data + col + o2) = quant8<KIND>(x + 8, b2);
+    if ((o1 & 31u) == 0) scale[(col + o1) >> 5] = (uint8_t)b1;
+    if ((o2 & 31u) == 0) scale[(col + o2) >> 5] = (uint8_t)b2;
+}
+
+// a row's columns behind the last head, up to the pitch
+__device__ __forceinline__ void hold_rest(uint8_t* data, uint8_t* scale, uint64_t cols,
+                                          uint64_t pitch) {
+    for (uint64_t c = cols + threadIdx.x * 32; c < pitch; c += kThreads * 32) {
+        *reinterpret_cast<uint4*>(data + c) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(data + c + 16) = make_uint4(0u, 0u, 0u, 0u);
+        scale[c >> 5] = 1;
+    }
+}
+
+// ------------------------------------------------------------ forward
+// HOLD: 0 no checkpoint, 1 e4m3, 2 int8.  A padding token's outputs are zero,
+// and so is its checkpoint.
+template <class T, int VEC, int NU, bool NORM, int HOLD>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args a) {
+    __shared__ uint64_t turns[kMaxDim / 2];
+    __shared__ float gains[NORM ? 2 * kMaxDim : 1];
+    extern __shared__ float2 cs[];   // [per_block][half]
+    const Deal& d = a.d;
+    for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
+    if (NORM)
+        for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) {
+            gains[i] = gain_at(a.gq, a.gain_type, i);
+            gains[kMaxDim + i] = a.k.heads ? gain_at(a.gk, a.gain_type, i) : 0.0f;
+        }
+    const uint32_t lane = threadIdx.x & (d.group - 1), mine = threadIdx.x / d.group;
+    const uint32_t groups = kThreads / d.group;
+    const uint32_t heads = (uint32_t)(a.q.heads + a.k.heads);
+    const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
+    uint32_t o1[NU], o2[NU];
+    bool h1[NU], h2[NU], turned[NU];
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+        chunks<VEC>(d, lane + n * d.group, o1[n], o2[n], h1[n], h2[n], turned[n]);
+
+    for (uint64_t t0 = (uint64_t)blockIdx.x * a.per_block; t0 < a.tokens;
+         t0 += (uint64_t)gridDim.x * a.per_block) {
+        const uint32_t count = (uint32_t)min((uint64_t)a.per_block, a.tokens - t0);
+        __syncthreads();
+        angles(a, turns, t0, count, cs);
+        __syncthreads();
+        const uint32_t items = count * heads;
+        // all lanes take every round: groups of one warp shuffle together
+        for (uint32_t base = 0; base < items; base += groups) {
+            const uint32_t item = base + mine;
+            const bool on = item < items;
+            const uint32_t tl = on ? item / heads : 0, h = on ? item - tl * heads : 0;
+            const uint64_t t = t0 + tl;
+            const bool is_q = h < a.q.heads;
+            const uint32_t hh = is_q ? h : h - (uint32_t)a.q.heads;
+            const Heads& in = is_q ? a.q : a.k;
+            const Heads& out = is_q ? a.oq : a.ok;
+            const bool live = on && position(a, t) >= 0;
+            const T* x = static_cast<const T*>(in.p) + t * in.ts + hh * in.hs;
+            float v[NU][2 * VEC];
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+                load_chunk<VEC>(x + o1[n], live && h1[n], v[n]);
+                load_chunk<VEC>(x + o2[n], live && h2[n], v[n] + VEC);
+            }
+            if constexpr (HOLD != 0 && VEC == 8) {
+                const uint64_t pitch = is_q ? a.pq : a.pk;
+                hold<HOLD - 1>((is_q ? a.q8 : a.k8) + t * pitch, (is_q ? a.sq : a.sk) + t * (pitch >> 5),
+                               (uint64_t)hh * d.dim, o1[0], o2[0], on && h1[0], v[0]);
+            }
+            if (NORM) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NU; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(v[n][i], v[n][i], ss);
+                ss = group_sum(ss, d.group);
+                const float r = rsqrtf(__fmaf_rn(ss, inv_dim, a.eps));
+                const float* g = gains + (is_q ? 0 : kMaxDim);
+#pragma unroll
+                for (int n = 0; n < NU; ++n)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        if (h1[n]) v[n][i] = __fmul_rn(__fmul_rn(v[n][i], r), g[o1[n] + i]);
+                        if (h2[n]) v[n][VEC + i] = __fmul_rn(__fmul_rn(v[n][VEC + i], r), g[o2[n] + i]);
+                    }
+            }
+            T* y = static_cast<T*>(out.p) + t * out.ts + hh * out.hs;
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+                if (turned[n] && h1[n]) rotate<VEC>(d, cs + tl * d.half, lane + n * d.group, v[n]);
+                store_chunk<VEC>(y + o1[n], on && h1[n], v[n]);
+                store_chunk<VEC>(y + o2[n], on && h2[n], v[n] + VEC);
+            }
+        }
+        if constexpr (HOLD != 0 && VEC == 8)
+            for (uint32_t tl = 0; tl < count; ++tl) {
+                hold_rest(a.q8 + (t0 + tl) * a.pq, a.sq + (t0 + tl) * (a.pq >> 5),
+                          a.q.heads * d.dim, a.pq);
+                if (a.k.heads)
+                    hold_rest(a.k8 + (t0 + tl) * a.pk, a.sk + (t0 + tl) * (a.pk >> 5),
+                              a.k.heads * d.dim, a.pk);
+            }
+    }
+}
+
+// ------------------------------------------------------------ backward
+template <int VEC, int KIND>
+__device__ __forceinline__ void held_chunk(const uint8_t* data, const uint8_t* scale, uint64_t col,
+                                           bool there, float* v) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
+    if (!there) return;
+    const uint32_t byte = scale[col >> 5];
+    if constexpr (VEC == 8) {
+        dequant8<KIND>(*reinterpret_cast<const uint2*>(data + col), byte, v);
+    } else if constexpr (VEC == 4) {
+        bytes4<KIND>(*reinterpret_cast<const uint32_t*>(data + col), v);
+        const float s = scale_of(byte);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], s);
+    } else {
+        float w[4];
+        bytes4<KIND>(data[col], w);
+        v[0] = __fmul_rn(w[0], scale_of(byte));
+    }
+}
+
+// The blocks below a.q_blocks take the queries, the others the keys, so that a
+// lane's running gradient belongs to one gain.  Each block leaves its sums in
+// a.partial; gains_kernel adds them in block order.
+// SRC: 0 x as T, 1 e4m3, 2 int8.
+template <class T, int VEC, int NU, int SRC>
+__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args a) {
+    __shared__ uint64_t turns[kMaxDim / 2];
+    extern __shared__ float2 cs[];   // [per_block][half]; at the end [groups][dim] floats
+    const Deal& d = a.d;
+    for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
+    const bool is_q = blockIdx.x < a.q_blocks;
+    const uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
+    const uint32_t blocks = is_q ? a.q_blocks : gridDim.x - a.q_blocks;
+    const Heads in = is_q ? a.q : a.k, out = is_q ? a.oq : a.ok, src = is_q ? a.xq : a.xk;
+    const uint32_t heads = (uint32_t)in.heads;
+    const void* gain = is_q ? a.gq : a.gk;
+    const uint8_t* data = is_q ? a.q8 : a.k8;
+    const uint8_t* scale = is_q ? a.sq : a.sk;
+    const uint64_t pitch = is_q ? a.pq : a.pk;
+
+    const uint32_t lane = threadIdx.x & (d.group - 1), mine = threadIdx.x / d.group;
+    const uint32_t groups = kThreads / d.group;
+    const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
+    uint32_t o1[NU], o2[NU];
+    bool h1[NU], h2[NU], turned[NU];
+    float g[NU][2 * VEC], dg[NU][2 * VEC];
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+        chunks<VEC>(d, lane + n * d.group, o1[n], o2[n], h1[n], h2[n], turned[n]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            g[n][i] = h1[n] ? gain_at(gain, a.gain_type, o1[n] + i) : 0.0f;
+            g[n][VEC + i] = h2[n] ? gain_at(gain, a.gain_type, o2[n] + i) : 0.0f;
+            dg[n][i] = dg[n][VEC + i] = 0.0f;
+        }
+    }
+    for (uint64_t t0 = (uint64_t)block * a.per_block; t0 < a.tokens;
+         t0 += (uint64_t)blocks * a.per_block) {
+        const uint32_t count = (uint32_t)min((uint64_t)a.per_block, a.tokens - t0);
+        __syncthreads();
+        angles(a, turns, t0, count, cs);
+        __syncthreads();
+        const uint32_t items = count * heads;
+        for (uint32_t base = 0; base < items; base += groups) {
+            const uint32_t item = base + mine;
+            const bool on = item < items;
+            const uint32_t tl = on ? item / heads : 0, h = on ? item - tl * heads : 0;
+            const uint64_t t = t0 + tl;
+            const bool live = on && position(a, t) >= 0;
+            const T* dy = static_cast<const T*>(in.p) + t * in.ts + h * in.hs;
+            float u[NU][2 * VEC], x[NU][2 * VEC];
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+                load_chunk<VEC>(dy + o1[n], live && h1[n], u[n]);
+                load_chunk<VEC>(dy + o2[n], live && h2[n], u[n] + VEC);
+                if constexpr (SRC == 0) {
+                    const T* xp = static_cast<const T*>(src.p) + t * src.ts + h * src.hs;
+                    load_chunk<VEC>(xp + o1[n], live && h1[n], x[n]);
+                    load_chunk<VEC>(xp + o2[n], live && h2[n], x[n] + VEC);
+                } else {
+                    const uint8_t* row = data + t * pitch;
+                    const uint8_t* srow = scale + t * (pitch >> 5);
+                    const uint64_t col = (uint64_t)h * d.dim;
+                    held_chunk<VEC, SRC - 1>(row, srow, col + o1[n], live && h1[n], x[n]);
+                    held_chunk<VEC, SRC - 1>(row, srow, col + o2[n], live && h2[n], x[n] + VEC);
+                }
+            }
+            float ss = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NU; ++n)
+#pragma unroll
+                for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(x[n][i], x[n][i], ss);
+            ss = group_sum(ss, d.group);
+            const float r = rsqrtf(__fmaf_rn(ss, inv_dim, a.eps));
+            float dot = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+                if (turned[n] && h1[n]) rotate<VEC>(d, cs + tl * d.half, lane + n * d.group, u[n]);
+#pragma unroll
+                for (int i = 0; i < 2 * VEC; ++i) {
+                    x[n][i] = __fmul_rn(x[n][i], r);
+                    dg[n][i] = __fmaf_rn(u[n][i], x[n][i], dg[n][i]);
+                    u[n][i] = __fmul_rn(u[n][i], g[n][i]);
+                    dot = __fmaf_rn(u[n][i], x[n][i], dot);
+                }
+            }
+            dot = __fmul_rn(group_sum(dot, d.group), inv_dim);
+            T* dx = static_cast<T*>(out.p) + t * out.ts + h * out.hs;
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+#pragma unroll
+                for (int i = 0; i < 2 * VEC; ++i)
+                    u[n][i] = __fmul_rn(__fmaf_rn(-x[n][i], dot, u[n][i]), r);
+                store_chunk<VEC>(dx + o1[n], on && h1[n], u[n]);
+                store_chunk<VEC>(dx + o2[n], on && h2[n], u[n] + VEC);
+            }
+        }
+    }
+    // the groups' sums, added in group order
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(cs);
+#pragma unroll
+    for (int n = 0; n < NU; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            if (h1[n]) sums[mine * d.dim + o1[n] + i] = dg[n][i];
+            if (h2[n]) sums[mine * d.dim + o2[n] + i] = dg[n][VEC + i];
+        }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) {
+        float s = 0.0f;
+        for (uint32_t m = 0; m < groups; ++m) s = __fadd_rn(s, sums[m * d.dim + i]);
+        a.partial[(uint64_t)blockIdx.x * d.dim + i] = s;
+    }
+}
+
+// blocks' sums to the gains' gradients: one warp per element, in a fixed order
+__global__ void __launch_bounds__(kThreads) gains_kernel(const float* __restrict__ partial,
+                                                         uint32_t q_blocks, uint32_t blocks,
+                                                         uint32_t dim, void* dgq, void* dgk,
+                                                         int type, int accumulate) {
+    const uint32_t at = (blockIdx.x * kThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+    const bool is_q = at < dim;
+    const uint32_t i = is_q ? at : at - dim;
+    if (i >= dim) return;
+    const uint32_t lo = is_q ? 0 : q_blocks, hi = is_q ? q_blocks : blocks;
+    if (lo == hi) return;
+    float s = 0.0f;
+    for (uint32_t b = lo + lane; b < hi; b += 32) s = __fadd_rn(s, partial[(uint64_t)b * dim + i]);
+    s = group_sum(s, 32);
+    if (lane) return;
+    void* out = is_q ? dgq : dgk;
+    if (accumulate) s = __fadd_rn(s, gain_at(out, type, i));
+    if (type == ARK_TYPE_F32)
+        static_cast<float*>(out)[i] = s;
+    else if (type == ARK_TYPE_BF16)
+        static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(s);
+    else
+        static_cast<__half*>(out)[i] = __float2half_rn(s);
+}
+
+// ------------------------------------------------------------ host
+Heads heads_of(const ark_heads* h) {
+    return h ? Heads{h->data, h->heads, h->token_stride, h->head_stride} : Heads{nullptr, 0, 0, 0};
+}
+
+bool heads_ok(const Heads& h, uint64_t tokens, uint64_t dim, uint64_t e, bool written, int* rc) {
+    if (h.heads == 0 || tokens == 0) return true;
+    if (!h.p || h.heads >= (1u << 16)) {
+        *rc = ARK_E_INVALID_ARG;
+        return false;
+    }
+    if (!aligned_to(h.p, e)) {
+        *rc = ARK_E_MISALIGNED;
+        return false;
+    }
+    // written heads may not overlap, in either order of tokens and heads
+    if (written) {
+        const bool inner = (h.heads == 1 || h.hs >= dim) &&
+                           (tokens == 1 || h.ts >= (h.heads - 1) * h.hs + dim);
+        const bool outer = (tokens == 1 || h.ts >= dim) &&
+                           (h.heads == 1 || h.hs >= (tokens - 1) * h.ts + dim);
+        if (!inner && !outer) {
+            *rc = ARK_E_INVALID_ARG;
+            return false;
+        }
+    }
+    return true;
+}
+
+// elements that every row of a set of heads starts at a multiple of
+bool multiple(const Heads& h, uint64_t e, uint64_t vec) {
+    if (h.heads == 0) return true;
+    const uint64_t bytes = vec * e > 16 ? 16 : vec * e;
+    return aligned_to(h.p, bytes) && h.ts * e % bytes == 0 && h.hs * e % bytes == 0;
+}
+
+// The widest chunk that divides the head, its rotated part and every row's start.
+int chunk_of(const ark_rope_plan* p, uint64_t dim, uint64_t e, const Heads* h, int n) {
+    for (int vec = 8; vec > 1; vec /= 2) {
+        if (vec == 2) continue;
+        const uint64_t rot = p->rotary_dim;
+        bool ok = dim % vec == 0 && (p->interleaved ? rot % (2 * vec) == 0 : rot / 2 % vec == 0);
+        for (int i = 0; ok && i < n; ++i) ok = multiple(h[i], e, (uint64_t)vec);
+        if (ok) return vec;
+    }
+    return 1;
+}
+
+Deal deal_of(const ark_rope_plan* p, uint64_t dim, int vec) {
+    Deal d;
+    d.dim = (uint32_t)dim;
+    d.rot = p->rotary_dim;
+    d.half = d.rot / 2;
+    d.interleaved = p->interleaved != 0;
+    d.rot_units = d.half / vec;
+    d.units = d.rot_units + (d.dim - d.rot + 2 * vec - 1) / (2 * vec);
+    d.group = 1;
+    while (d.group < 32 && d.group < d.units) d.group *= 2;
+    return d;
+}
+
+int plan_ok(const ark_rope_plan* p, uint64_t dim) {
+    if (!p || p->rotary_dim < 2 || p->rotary_dim % 2 || p->interleaved > 1) return ARK_E_INVALID_ARG;
+    if (dim > kMaxDim) return ARK_E_UNSUPPORTED;
+    return p->rotary_dim <= dim ? ARK_OK : ARK_E_INVALID_ARG;
+}
+
+int common_ok(const Args& a, uint64_t e, uint64_t dim, int pos_type) {
+    if (!a.pos && a.seq == 0) return ARK_E_INVALID_ARG;
+    if (a.pos && pos_type != ARK_TYPE_I32 && pos_type != ARK_TYPE_I64) return ARK_E_INVALID_ARG;
+    if (a.pos && !aligned_to(a.pos, a.pos64 ? 8 : 4)) return ARK_E_MISALIGNED;
+    if (a.tokens >= (1ull << 40)) return ARK_E_INVALID_ARG;
+    if (a.oq.heads != a.q.heads || a.ok.heads != a.k.heads) return ARK_E_INVALID_ARG;
+    int rc = ARK_OK;
+    heads_ok(a.q, a.tokens, dim, e, false, &rc) && heads_ok(a.k, a.tokens, dim, e, false, &rc) &&
+        heads_ok(a.oq, a.tokens, dim, e, true, &rc) && heads_ok(a.ok, a.tokens, dim, e, true, &rc);
+    return rc;
+}
+
+// Tokens of a CTA at a time: enough pairs for every thread to form one angle,
+// but never so many that SMs stay without a token.
+uint32_t tokens_per_block(uint64_t tokens, uint32_t half) {
+    uint32_t n = kThreads / (half < kThreads ? half : kThreads);
+    if (n > 8) n = 8;
+    while (n > 1 && (tokens + n - 1) / n < (uint64_t)sm_count()) --n;
+    return n ? n : 1;
+}
+
+template <class T, int VEC, int NU, bool NORM, int HOLD>
+int forward_t(Args& a, cudaStream_t s) {
+    auto k = forward_kernel<T, VEC, NU, NORM, HOLD>;
+    a.per_block = tokens_per_block(a.tokens, a.d.half);
+    const size_t smem = (size_t)a.per_block * a.d.half * sizeof(float2);
+    const uint64_t work = (a.tokens + a.per_block - 1) / a.per_block;
+    const int grid = streaming_grid(reinterpret_cast<const void*>(k), kThreads, smem, work * kThreads);
+    k<<<grid, kThreads, smem, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+}
+
+template <class T, bool NORM, int HOLD>
+int forward_v(Args& a, int vec, cudaStream_t s) {
+    if (vec == 8) return forward_t<T, 8, 1, NORM, HOLD>(a, s);
+    if constexpr (HOLD != 0)
+        return ARK_E_UNSUPPORTED;   // not reached: the checkpoint is then a launch of its own
+    else
+        return vec == 4 ? forward_t<T, 4, 1, NORM, 0>(a, s) : forward_t<T, 1, 4, NORM, 0>(a, s);
+}
+
+template <class T, int VEC, int NU>
+int backward_t(Args& a, uint32_t blocks, cudaStream_t s) {
+    const size_t angles = (size_t)a.per_block * a.d.half * sizeof(float2);
+    const size_t sums = (size_t)(kThreads / a.d.group) * a.d.dim * sizeof(float);
+    const size_t smem = angles > sums ? angles : sums;
+    if (a.kind < 0)
+        backward_kernel<T, VEC, NU, 0><<<blocks, kThreads, smem, s>>>(a);
+    else if (a.kind == kE4M3)
+        backward_kernel<T, VEC, NU, 1 + kE4M3><<<blocks, kThreads, smem, s>>>(a);
+    else
+        backward_kernel<T, VEC, NU, 1 + kInt8><<<blocks, kThreads, smem, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+}
+
+// Blocks of the backward: 4 to an SM, shared between queries and keys by their
+// heads, and none without a token.
+uint32_t back_blocks(uint64_t tokens, uint64_t hq, uint64_t hk, uint32_t per_block, uint32_t* q) {
+    const uint64_t need = (tokens + per_block - 1) / per_block;
+    const uint64_t most = (uint64_t)sm_count() * 4;
+    uint64_t bq = hq ? most * hq / (hq + hk) : 0, bk = hk ? most - bq : 0;
+    if (hq && !bq) bq = 1;
+    if (hk && !bk) bk = 1;
+    if (bq > need) bq = need;
+    if (bk > need) bk = need;
+    *q = (uint32_t)bq;
+    return (uint32_t)(bq + bk);
+}
+
+void fill_positions(Args& a, const void* positions, int32_t type, uint64_t seq) {
+    a.pos = positions;
+    a.pos64 = type == ARK_TYPE_I64;
+    a.seq = seq;
+}
+
+int held_ok(const ark_act8* c, const Heads& h, uint64_t tokens, uint64_t dim) {
+    const int rc = act8_check(c);
+    if (rc) return rc;
+    return c->rows == tokens && c->cols == h.heads * dim ? ARK_OK : ARK_E_INVALID_ARG;
+}
+
+}  // namespace
+}  // namespace ark
+
+using namespace ark;
+
+extern "C" {
+
+int ark_cuda_rope_plan(ark_rope_plan* out, uint32_t rotary_dim, uint32_t interleaved, double base,
+                       uint32_t scaling, double factor, double original, double fast, double slow) {
+    if (!out || rotary_dim < 2 || rotary_dim % 2 || rotary_dim > kMaxDim || interleaved > 1 ||
+        !(base > 1.0) || !isfinite(base) || scaling > ARK_ROPE_WAVE)
+        return ARK_E_INVALID_ARG;
+    const double pi2 = 6.283185307179586476925;
+    if (scaling != ARK_ROPE_NONE && (!(factor >= 1.0) || !isfinite(factor))) return ARK_E_INVALID_ARG;
+    if (scaling == ARK_ROPE_BASE) {
+        if (rotary_dim == 2) return ARK_E_INVALID_ARG;
+        base *= pow(factor, (double)rotary_dim / (rotary_dim - 2));
+    }
+    double lo = 0.0, hi = 0.0;
+    if (scaling == ARK_ROPE_PARTS || scaling == ARK_ROPE_WAVE) {
+        if (!(original > 0.0) || !isfinite(original) || !(slow > 0.0) || !(fast > slow) || !isfinite(fast))
+            return ARK_E_INVALID_ARG;
+        if (scaling == ARK_ROPE_PARTS) {
+            // pairs that make `fast` and `slow` turns over the original length
+            lo = floor(rotary_dim * log(original / (fast * pi2)) / (2.0 * log(base)));
+            hi = ceil(rotary_dim * log(original / (slow * pi2)) / (2.0 * log(base)));
+            if (lo < 0.0) lo = 0.0;
+            if (hi > rotary_dim - 1.0) hi = rotary_dim - 1.0;
+        }
+    }
+    memset(out, 0, sizeof(*out));
+    out->rotary_dim = rotary_dim;
+    out->interleaved = interleaved;
+    out->gain = scaling == ARK_ROPE_PARTS ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+    for (uint32_t i = 0; i < rotary_dim / 2; ++i) {
+        double w = pow(base, -2.0 * i / rotary_dim);   // radians per position
+        if (scaling == ARK_ROPE_LINEAR) {
+            w /= factor;
+        } else if (scaling == ARK_ROPE_PARTS) {
+            const double span = hi - lo > 0.001 ? hi - lo : 0.001;
+            double ramp = (i - lo) / span;
+            ramp = ramp < 0.0 ? 0.0 : ramp > 1.0 ? 1.0 : ramp;
+            w = w / factor * ramp + w * (1.0 - ramp);
+        } else if (scaling == ARK_ROPE_WAVE) {
+            double keep = (original * w / pi2 - slow) / (fast - slow);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            w = w * keep + w / factor * (1.0 - keep);
+        }
+        out->turns[i] = (uint64_t)ldexp(w / pi2, 64);   // w <= 1: below a sixth of a turn
+    }
+    return ARK_OK;
+}
+
+int ark_cuda_rope(const ark_rope_plan* plan, const ark_heads* q, const ark_heads* k,
+                  const ark_heads* out_q, const ark_heads* out_k, int32_t type, uint64_t tokens,
+                  uint64_t dim, const void* positions, int32_t pos_type, uint64_t seq_len,
+                  int32_t inverse, void* cuda_stream) {
+    int rc = plan_ok(plan, dim);
+    if (rc) return rc;
+    const uint64_t e = type_size(type);
+    if (!e || !q || !out_q || (!k != !out_k)) return ARK_E_INVALID_ARG;
+    Args a;
+    memset(&a, 0, sizeof(a));
+    a.plan = *plan;
+    fill_positions(a, positions, pos_type, seq_len);
+    a.inverse = inverse != 0;
+    a.tokens = tokens;
+    a.q = heads_of(q), a.k = heads_of(k), a.oq = heads_of(out_q), a.ok = heads_of(out_k);
+    a.kind = -1;
+    rc = common_ok(a, e, dim, pos_type);
+    if (rc) return rc;
+    if (tokens == 0 || a.q.heads + a.k.heads == 0) return ARK_OK;
+    const Heads all[4] = {a.q, a.k, a.oq, a.ok};
+    const int vec = chunk_of(plan, dim, e, all, 4);
+    a.d = deal_of(plan, dim, vec);
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    return by_type(type, [&](auto t) { return forward_v<decltype(t), false, 0>(a, vec, s); });
+}
+
+int ark_cuda_qk_norm_rope(const ark_rope_plan* plan, const ark_heads* q, const ark_heads* k,
+                          const ark_heads* out_q, const ark_heads* out_k, int32_t type,
+                          uint64_t tokens, uint64_t dim, const void* gain_q, const void* gain_k,
+                          int32_t gain_type, float eps, const void* positions, int32_t pos_type,
+                          uint64_t seq_len, const ark_act8* q8, const ark_act8* k8,
+                          void* cuda_stream) {
+    int rc = plan_ok(plan, dim);
+    if (rc) return rc;
+    const uint64_t e = type_size(type);
+    if (!e || !type_size(gain_type) || !q || !out_q || (!k != !out_k) || !(eps >= 0.0f))
+        return ARK_E_INVALID_ARG;
+    Args a;
+    memset(&a, 0, sizeof(a));
+    a.plan = *plan;
+    fill_positions(a, positions, pos_type, seq_len);
+    a.tokens = tokens;
+    a.q = heads_of(q), a.k = heads_of(k), a.oq = heads_of(out_q), a.ok = heads_of(out_k);
+    a.gq = gain_q, a.gk = gain_k, a.gain_type = gain_type, a.eps = eps;
+    a.kind = -1;
+    rc = common_ok(a, e, dim, pos_type);
+    if (rc) return rc;
+    if ((a.q.heads && !gain_q) || (a.k.heads && !gain_k)) return ARK_E_INVALID_ARG;
+    if (!aligned_to(gain_q, type_size(gain_type)) || !aligned_to(gain_k, type_size(gain_type)))
+        return ARK_E_MISALIGNED;
+    if (q8) {
+        if (k && !k8) return ARK_E_INVALID_ARG;
+        rc = held_ok(q8, a.q, tokens, dim);
+        if (!rc && k) rc = held_ok(k8, a.k, tokens, dim);
+        if (rc) return rc;
+        if (k && k8->kind != q8->kind) return ARK_E_INVALID_ARG;
+    } else if (k8) {
+        return ARK_E_INVALID_ARG;
+    }
+    if (tokens == 0 || a.q.heads + a.k.heads == 0) return ARK_OK;
+    const Heads all[4] = {a.q, a.k, a.oq, a.ok};
+    const int vec = chunk_of(plan, dim, e, all, 4);
+    a.d = deal_of(plan, dim, vec);
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    if (q8) {
+        a.q8 = q8->data, a.sq = q8->scale, a.pq = act8_pitch(q8->cols);
+        if (k) a.k8 = k8->data, a.sk = k8->scale, a.pk = act8_pitch(k8->cols);
+        // a scale block lies in one head and in the chunks of lanes side by side
+        const uint32_t rot = plan->rotary_dim;
+        if (vec == 8 && dim % 32 == 0 && rot % (plan->interleaved ? 32 : 64) == 0)
+            return by_type(type, [&](auto t) {
+                using T = decltype(t);
+                return q8->kind == kE4M3 ? forward_v<T, true, 1 + kE4M3>(a, vec, s)
+                                         : forward_v<T, true, 1 + kInt8>(a, vec, s);
+            });
+        // else a launch of its own before x may be overwritten; heads side by side
+        if ((a.q.heads > 1 && a.q.hs != dim) || (a.k.heads > 1 && a.k.hs != dim))
+            return ARK_E_UNSUPPORTED;
+        rc = ark_cuda_act8_pack(a.q.p, type, a.q.ts, q8, cuda_stream);
+        if (!rc && k) rc = ark_cuda_act8_pack(a.k.p, type, a.k.ts, k8, cuda_stream);
+        if (rc) return rc;
+    }
+    return by_type(type, [&](auto t) { return forward_v<decltype(t), true, 0>(a, vec, s); });
+}
+
+uint64_t ark_cuda_qk_norm_rope_workspace(uint64_t dim) {
+    return (uint64_t)sm_count() * 4 * dim * sizeof(float) + 2 * dim * sizeof(float);
+}
+
+int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* dq,
+                                   const ark_heads* dk, const ark_heads* out_dq,
+                                   const ark_heads* out_dk, int32_t type, uint64_t tokens,
+                                   uint64_t dim, const ark_act8* q8, const ark_act8* k8,
+                                   const ark_heads* q, const ark_heads* k, const void* gain_q,
+                                   const void* gain_k, int32_t gain_type, float eps,
+                                   const void* positions, int32_t pos_type, uint64_t seq_len,
+                                   void* dgain_q, void* dgain_k, int32_t dgain_type,
+                                   int32_t accumulate, void* workspace, uint64_t workspace_bytes,
+                                   void* cuda_stream) {
+    int rc = plan_ok(plan, dim);
+    if (rc) return rc;
+    const uint64_t e = type_size(type);
+    if (!e || !type_size(gain_type) || !type_size(dgain_type) || !dq || !out_dq ||
+        (!dk != !out_dk) || !(eps >= 0.0f) || (!q8 == !q) || (dk && (!k8 == !k)) ||
+        (dk && !q8 != !k8))
+        return ARK_E_INVALID_ARG;
+    Args a;
+    memset(&a, 0, sizeof(a));
+    a.plan = *plan;
+    fill_positions(a, positions, pos_type, seq_len);
+    a.inverse = 1;
+    a.tokens = tokens;
+    a.q = heads_of(dq), a.k = heads_of(dk), a.oq = heads_of(out_dq), a.ok = heads_of(out_dk);
+    a.xq = heads_of(q), a.xk = heads_of(dk ? k : nullptr);
+    a.gq = gain_q, a.gk = gain_k, a.gain_type = gain_type, a.eps = eps;
+    a.kind = -1;
+    rc = common_ok(a, e, dim, pos_type);
+    if (rc) return rc;
+    if (q8) {
+        rc = held_ok(q8, a.q, tokens, dim);
+        if (!rc && dk) rc = held_ok(k8, a.k, tokens, dim);
+        if (rc) return rc;
+        if (dk && k8->kind != q8->kind) return ARK_E_INVALID_ARG;
+        a.kind = q8->kind;
+        a.q8 = q8->data, a.sq = q8->scale, a.pq = act8_pitch(q8->cols);
+        if (dk) a.k8 = k8->data, a.sk = k8->scale, a.pk = act8_pitch(k8->cols);
+    } else {
+        if (a.xq.heads != a.q.heads || a.xk.heads != a.k.heads) return ARK_E_INVALID_ARG;
+        if (!heads_ok(a.xq, tokens, dim, e, false, &rc) || !heads_ok(a.xk, tokens, dim, e, false, &rc))
+            return rc;
+    }
+    if ((a.q.heads && (!gain_q || !dgain_q)) || (a.k.heads && (!gain_k || !dgain_k)))
+        return ARK_E_INVALID_ARG;
+    if (!aligned_to(gain_q, type_size(gain_type)) || !aligned_to(gain_k, type_size(gain_type)) ||
+        !aligned_to(dgain_q, type_size(dgain_type)) || !aligned_to(dgain_k, type_size(dgain_type)))
+        return ARK_E_MISALIGNED;
+    if (a.q.heads + a.k.heads == 0) return ARK_OK;
+    if (!workspace || workspace_bytes < ark_cuda_qk_norm_rope_workspace(dim)) return ARK_E_INVALID_ARG;
+    if (!aligned_to(workspace, 4)) return ARK_E_MISALIGNED;
+    a.partial = static_cast<float*>(workspace);
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    const Heads all[6] = {a.q, a.k, a.oq, a.ok, a.xq, a.xk};
+    const int vec = chunk_of(plan, dim, e, all, 6);
+    a.d = deal_of(plan, dim, vec);
+    // no tokens: one block without work leaves zero sums
+    a.per_block = tokens_per_block(tokens, a.d.half);
+    const uint32_t blocks = back_blocks(tokens ? tokens : 1, a.q.heads, a.k.heads, a.per_block, &a.q_blocks);
+    rc = by_type(type, [&](auto t) {
+        using T = decltype(t);
+        return vec == 8   ? backward_t<T, 8, 1>(a, blocks, s)
+               : vec == 4 ? backward_t<T, 4, 1>(a, blocks, s)
+                          : backward_t<T, 1, 4>(a, blocks, s);
+    });
+    if (rc) return rc;
+    gains_kernel<<<(2 * (unsigned)dim * 32 + kThreads - 1) / kThreads, kThreads, 0, s>>>(
+        a.partial, a.q_blocks, blocks, (uint32_t)dim, dgain_q, dgain_k, dgain_type, accumulate != 0);
+    return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+}
+
+}  // extern "C"

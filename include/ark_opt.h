@@ -382,6 +382,162 @@ ARK_API int ark_synth_f16(uint16_t* out, uint64_t n, uint64_t offset, uint64_t s
 ARK_API int ark_synth_f32(float* out, uint64_t n, uint64_t offset, uint64_t seed, uint64_t stream,
                   float sigma, int square, void* cuda_stream);
 
+/* ======================================================================
+ * 4. Activations: what the backward that fills the gradient buffer keeps
+ *    and reads.  No counterpart in the reference's native library (its
+ *    forward and backward are MPSGraph, objc/bridge.m:229-411).
+ *
+ * Every call is enqueued on cuda_stream (NULL: the default stream) of the
+ * current device, which the buffers belong to; nothing is waited for,
+ * nothing is allocated, and every call may be captured into a graph.  Calls
+ * share no state: they may overlap freely on different streams as long as
+ * their buffers and workspaces do.  Rows are contiguous, `ld` elements
+ * apart; a stride of 0 repeats a row of an input.  Misaligned or ragged
+ * rows are served by slower loads.  Inputs and outputs may not overlap
+ * unless a call says so.
+ * ====================================================================== */
+#define ARK_TYPE_F16  0
+#define ARK_TYPE_BF16 1
+#define ARK_TYPE_F32  2
+#define ARK_TYPE_I32  3   /* positions only */
+#define ARK_TYPE_I64  4   /* positions only */
+
+/* An 8-bit checkpoint of a [rows, cols] activation.
+ *   data:  rows of ark_cuda_act8_pitch(cols) bytes (cols rounded up to 128;
+ *          the padding holds zeros), one byte per element, 16-byte aligned;
+ *   scale: rows of pitch/32 bytes, one per 32 columns, 4-byte aligned.
+ * The scale of a block is the power of two 2^k with the smallest k >= -126
+ * such that max|x| <= top * 2^k (top 448 for e4m3, 127 for int8); its byte
+ * is k + 127 and the element is x * 2^-k rounded to nearest even.  A block
+ * that holds an infinity or a NaN has scale byte 255 and reads back as NaN,
+ * so that an overflowed forward still makes the step a skipped one. */
+#define ARK_ACT8_E4M3 0
+#define ARK_ACT8_INT8 1
+typedef struct ark_act8 {
+    uint8_t* data;
+    uint8_t* scale;
+    uint64_t rows, cols;
+    int32_t  kind;      /* ARK_ACT8_* */
+    uint32_t reserved;
+} ark_act8;
+
+ARK_API uint64_t ark_cuda_act8_pitch(uint64_t cols);
+
+/* x (F16, BF16 or F32) into a checkpoint, and back.  A finite value that
+ * the type of y cannot hold saturates at its largest. */
+ARK_API int ark_cuda_act8_pack(const void* x, int32_t type, uint64_t ldx, const ark_act8* out,
+                               void* cuda_stream);
+ARK_API int ark_cuda_act8_unpack(const ark_act8* in, void* y, int32_t type, uint64_t ldy,
+                                 void* cuda_stream);
+
+/* Weight gradient of y = x W for W [in, out] (the reference's weight
+ * layout, objc/bridge.m:229-411) from the checkpoint of x [tokens, in]:
+ *   dw[i, o] = (accumulate ? dw[i, o] : 0) + sum over t of x[t, i] dy[t, o],
+ * products and sums in FP32, rounded once to dw's type.  dy: F16 or BF16
+ * [tokens, n_out]; dw: F16, BF16 or F32 [x->cols, n_out], for example a
+ * tensor's range of ark_cuda_opt_grad_buffer with dy carrying the loss
+ * scale; a sum that F16 cannot hold becomes an infinity, which the step
+ * takes for an overflow.  The result is the same bits on every call.
+ * workspace: 16-byte aligned, ark_cuda_weight_grad_workspace bytes (0, and
+ * then it may be NULL, when dy's rows are 16-byte aligned). */
+ARK_API uint64_t ark_cuda_weight_grad_workspace(uint64_t tokens, const void* dy, uint64_t lddy,
+                                                uint64_t n_out);
+ARK_API int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
+                                 uint64_t n_out, void* dw, int32_t dw_type, uint64_t lddw,
+                                 int32_t accumulate, void* workspace, uint64_t workspace_bytes,
+                                 void* cuda_stream);
+
+/* y = silu(a) * b, [rows, cols].  With a8 and b8 (both or neither), a and b
+ * are checkpointed in the same pass.  y may be a or b. */
+ARK_API int ark_cuda_swiglu(const void* a, uint64_t lda, const void* b, uint64_t ldb, int32_t type,
+                            uint64_t rows, uint64_t cols, void* y, uint64_t ldy,
+                            const ark_act8* a8, const ark_act8* b8, void* cuda_stream);
+/* Its backward from the checkpoints: da = dy b silu'(a), db = dy silu(a).
+ * With y8, silu(a) * b is remade from the checkpoints, rounded to `type` and
+ * checkpointed, for the weight gradient of the projection that reads it: the
+ * forward then keeps no y.  da or db may be dy. */
+ARK_API int ark_cuda_swiglu_backward(const void* dy, uint64_t lddy, int32_t type,
+                                     const ark_act8* a8, const ark_act8* b8, void* da,
+                                     uint64_t ldda, void* db, uint64_t lddb, const ark_act8* y8,
+                                     void* cuda_stream);
+
+/* Rotary positions.  The first rotary_dim elements of each head are rotated
+ * in pairs (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved; the
+ * others pass.  turns[i]: turns of pair i per position, in 2^-64 of a turn;
+ * gain: factor on the rotated elements.  A plain host struct: it may be
+ * copied, and is read during the call that gets it. */
+#define ARK_ROPE_MAX_DIM 256
+typedef struct ark_rope_plan {
+    uint32_t rotary_dim;
+    uint32_t interleaved;
+    float    gain;
+    uint32_t reserved;
+    uint64_t turns[ARK_ROPE_MAX_DIM / 2];
+} ark_rope_plan;
+
+/* Pair i turns base^(-2i/rotary_dim) radians per position, scaled for
+ * contexts longer than the trained one by
+ *   LINEAR: every frequency divided by factor;
+ *   BASE:   base * factor^(rotary_dim / (rotary_dim - 2));
+ *   PARTS:  pairs that make more than `fast` turns over the `original`
+ *           length keep their frequency, those below `slow` turns are divided
+ *           by factor, a linear ramp over the pairs between; gain
+ *           0.1 ln(factor) + 1;
+ *   WAVE:   the same ends, a ramp linear in the number of turns, gain 1.
+ * factor >= 1; the arguments that a scaling does not use are ignored. */
+#define ARK_ROPE_NONE   0
+#define ARK_ROPE_LINEAR 1
+#define ARK_ROPE_BASE   2
+#define ARK_ROPE_PARTS  3
+#define ARK_ROPE_WAVE   4
+ARK_API int ark_cuda_rope_plan(ark_rope_plan* out, uint32_t rotary_dim, uint32_t interleaved,
+                               double base, uint32_t scaling, double factor, double original,
+                               double fast, double slow);
+
+/* [tokens, heads, dim] with element strides; dim is contiguous. */
+typedef struct ark_heads {
+    void*    data;
+    uint64_t heads;
+    uint64_t token_stride, head_stride;
+} ark_heads;
+
+/* The rotation (inverse: its backward) of q and k (k, out_k: NULL for q
+ * alone).  positions: I32 or I64 [tokens], or NULL for token index modulo
+ * seq_len.  A negative position marks a padding token: its inputs are not
+ * read and its outputs are zero.  out_q / out_k may be q / k.  dim up to
+ * ARK_ROPE_MAX_DIM. */
+ARK_API int ark_cuda_rope(const ark_rope_plan* plan, const ark_heads* q, const ark_heads* k,
+                          const ark_heads* out_q, const ark_heads* out_k, int32_t type,
+                          uint64_t tokens, uint64_t dim, const void* positions, int32_t pos_type,
+                          uint64_t seq_len, int32_t inverse, void* cuda_stream);
+
+/* RMS norm of each head, x * rsqrt(mean(x^2) + eps) * gain[dim], then the
+ * rotation, in one pass; nothing is rounded between.  With q8 (and k8), q and
+ * k as they come in are checkpointed too, as [tokens, heads * dim] (padding
+ * tokens' rows are unspecified); where dim or the rotated part is not made of
+ * whole scale blocks that needs head_stride == dim (else ARK_E_UNSUPPORTED). */
+ARK_API int ark_cuda_qk_norm_rope(const ark_rope_plan* plan, const ark_heads* q,
+                                  const ark_heads* k, const ark_heads* out_q,
+                                  const ark_heads* out_k, int32_t type, uint64_t tokens,
+                                  uint64_t dim, const void* gain_q, const void* gain_k,
+                                  int32_t gain_type, float eps, const void* positions,
+                                  int32_t pos_type, uint64_t seq_len, const ark_act8* q8,
+                                  const ark_act8* k8, void* cuda_stream);
+/* Its backward.  dq, dk: gradients of the outputs; x from the checkpoints q8 /
+ * k8, or else from q / k themselves (exactly one of the two).  out_dq / out_dk
+ * may be dq / dk.  dgain_q, dgain_k [dim]: the gains' gradients, summed in
+ * FP32 over tokens and heads in a fixed order and rounded once, or added to
+ * what is there.  workspace: ark_cuda_qk_norm_rope_workspace(dim) bytes of
+ * the current device, 4-byte aligned. */
+ARK_API uint64_t ark_cuda_qk_norm_rope_workspace(uint64_t dim);
+ARK_API int ark_cuda_qk_norm_rope_backward(
+    const ark_rope_plan* plan, const ark_heads* dq, const ark_heads* dk, const ark_heads* out_dq,
+    const ark_heads* out_dk, int32_t type, uint64_t tokens, uint64_t dim, const ark_act8* q8,
+    const ark_act8* k8, const ark_heads* q, const ark_heads* k, const void* gain_q,
+    const void* gain_k, int32_t gain_type, float eps, const void* positions, int32_t pos_type,
+    uint64_t seq_len, void* dgain_q, void* dgain_k, int32_t dgain_type, int32_t accumulate,
+    void* workspace, uint64_t workspace_bytes, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
