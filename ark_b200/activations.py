@@ -28,7 +28,10 @@ PITCH, BLOCK = 128, 32
 
 
 # ----------------------------------------------------------------- arguments
-def _float(t, what, types=(torch.float16, torch.bfloat16, torch.float32)):
+FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _float(t, what, types=FLOATS):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a CUDA torch.Tensor")
     if t.dtype not in types:
@@ -56,7 +59,7 @@ def _rows(t, what, rows=None, cols=None, written=False, like=None):
     return t.data_ptr(), ld
 
 
-def _heads(t, what, like=None, shape=None, written=False):
+def _heads(t, what, like=None, shape=None):
     """ark_heads of a [tokens, heads, dim] tensor."""
     _float(t, what)
     if t.dim() != 3:
@@ -82,7 +85,9 @@ def _device(first, *others):
 
 
 class _on:
-    """Makes a device the current one for a call, and gives the stream."""
+    """Makes a device the current one for a call, and gives the handle of
+    torch's current stream there (without making a Stream object: 3 us)."""
+    __slots__ = ("index", "before")
 
     def __init__(self, device):
         self.index = device.index
@@ -91,7 +96,7 @@ class _on:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
@@ -113,7 +118,7 @@ class Act8:
     kind:  "e4m3" (4 significant bits at every size) or "int8" (a fixed step
            of 1/127 to 1/64 of the block's largest).
     """
-    __slots__ = ("data", "scale", "rows", "cols", "kind", "c")
+    __slots__ = ("_data", "_scale", "_whole", "device", "rows", "cols", "kind", "c")
 
     def __init__(self, data, scale, cols, kind="e4m3"):
         cols = int(cols)
@@ -129,23 +134,47 @@ class Act8:
                 raise ValueError(f"{n}: expected contiguous [rows, {w}], got {tuple(t.shape)}")
         if data.device != scale.device:
             raise ValueError("data and scale on different devices")
-        self.data, self.scale, self.rows, self.cols, self.kind = data, scale, data.shape[0], cols, kind
+        self._data, self._scale, self._whole, self.device = data, scale, None, data.device
+        self.rows, self.cols, self.kind = data.shape[0], cols, kind
         self.c = _lib.Act8(data.data_ptr(), scale.data_ptr(), self.rows, cols, KINDS[kind], 0)
 
     @classmethod
     def empty(cls, rows, cols, kind="e4m3", device="cuda"):
-        """Room for a checkpoint (its contents are whatever was there)."""
+        """Room for a checkpoint (its contents are whatever was there), in one
+        allocation; `data` and `scale` are views of it."""
+        if kind not in KINDS:
+            raise ValueError(f"kind: expected one of {sorted(KINDS)}, got {kind!r}")
         pitch = -(-cols // PITCH) * PITCH
-        return cls(torch.empty((rows, pitch), dtype=torch.uint8, device=device),
-                   torch.empty((rows, pitch // BLOCK), dtype=torch.uint8, device=device), cols, kind)
+        self = cls.__new__(cls)
+        self._whole = torch.empty(rows * (pitch + pitch // BLOCK), dtype=torch.uint8, device=device)
+        if not self._whole.is_cuda:
+            raise ValueError("buffers must be CUDA tensors (device memory)")
+        self._data = self._scale = None
+        self.device = self._whole.device
+        self.rows, self.cols, self.kind = rows, cols, kind
+        p = self._whole.data_ptr()
+        self.c = _lib.Act8(p, p + rows * pitch, rows, cols, KINDS[kind], 0)
+        return self
 
     @property
-    def device(self):
-        return self.data.device
+    def pitch(self):
+        return -(-self.cols // PITCH) * PITCH
+
+    @property
+    def data(self):
+        if self._data is None:
+            self._data = self._whole[: self.rows * self.pitch].view(self.rows, self.pitch)
+        return self._data
+
+    @property
+    def scale(self):
+        if self._scale is None:
+            self._scale = self._whole[self.rows * self.pitch:].view(self.rows, self.pitch // BLOCK)
+        return self._scale
 
     @property
     def nbytes(self):
-        return self.data.numel() + self.scale.numel()
+        return self.rows * (self.pitch + self.pitch // BLOCK)
 
 
 def _held(c, what, rows=None, cols=None):
@@ -163,8 +192,10 @@ def act8_pack(x, kind="e4m3", out=None) -> Act8:
     with _on(x.device) as s:
         if out is None:
             out = Act8.empty(x.shape[0], x.shape[1], kind, x.device)
-        _device(x, out)
-        _call("ark_cuda_act8_pack", p, TYPES[x.dtype], ld, _held(out, "out", *x.shape), s)
+        else:
+            _held(out, "out", *x.shape)
+            _device(x, out)
+        _call("ark_cuda_act8_pack", p, TYPES[x.dtype], ld, ctypes.byref(out.c), s)
     return out
 
 
@@ -174,9 +205,13 @@ def act8_unpack(c, dtype=torch.float16, out=None):
     h = _held(c, "checkpoint")
     with _on(c.device) as s:
         if out is None:
+            if dtype not in FLOATS:
+                raise TypeError(f"unsupported type {dtype}")
             out = torch.empty((c.rows, c.cols), dtype=dtype, device=c.device)
-        p, ld = _rows(out, "out", c.rows, c.cols, written=True)
-        _device(c, out)
+            p, ld = out.data_ptr(), c.cols
+        else:
+            p, ld = _rows(out, "out", c.rows, c.cols, written=True)
+            _device(c, out)
         _call("ark_cuda_act8_unpack", h, p, TYPES[out.dtype], ld, s)
     return out
 
@@ -198,10 +233,14 @@ def weight_grad(x, dy, out=None, accumulate=False, dtype=None):
     n = dy.shape[1]
     with _on(_device(x, dy, out)) as s:
         if out is None:
+            if dtype is not None and dtype not in FLOATS:
+                raise TypeError(f"unsupported type {dtype}")
             out = torch.empty((x.cols, n), dtype=dtype or dy.dtype, device=dy.device)
-        elif dtype is not None and out.dtype != dtype:
-            raise ValueError(f"out: expected {dtype}, got {out.dtype}")
-        po, ldo = _rows(out, "out", x.cols, n, written=True)
+            po, ldo = out.data_ptr(), n
+        else:
+            if dtype is not None and out.dtype != dtype:
+                raise ValueError(f"out: expected {dtype}, got {out.dtype}")
+            po, ldo = _rows(out, "out", x.cols, n, written=True)
         need = _lib.lib().ark_cuda_weight_grad_workspace(x.rows, p, ld, n)
         ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
         _call("ark_cuda_weight_grad", hx, p, TYPES[dy.dtype], ld, n, po, TYPES[out.dtype], ldo,
@@ -219,7 +258,9 @@ def swiglu(a, b, checkpoint=None, out=None):
     with _on(a.device) as s:
         if out is None:
             out = torch.empty(a.shape, dtype=a.dtype, device=a.device)
-        py, ly = _rows(out, "out", a.shape[0], a.shape[1], written=True, like=a)
+            py, ly = out.data_ptr(), a.shape[1]
+        else:
+            py, ly = _rows(out, "out", a.shape[0], a.shape[1], written=True, like=a)
         ca = cb = ha = hb = None
         if checkpoint is not None:
             ca, cb = (Act8.empty(a.shape[0], a.shape[1], checkpoint, a.device) for _ in range(2))
@@ -240,11 +281,14 @@ def swiglu_backward(dy, ca, cb, checkpoint=None, out=None):
     pg, lg = _rows(dy, "dy", ca.rows, ca.cols)
     with _on(_device(dy, ca, cb)) as s:
         if out is None:
-            out = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device), \
-                torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-        da, db = out
-        pa, la = _rows(da, "da", ca.rows, ca.cols, written=True, like=dy)
-        pb, lb = _rows(db, "db", ca.rows, ca.cols, written=True, like=dy)
+            da = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+            db = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+            pa, pb, la = da.data_ptr(), db.data_ptr(), ca.cols
+            lb = la
+        else:
+            da, db = out
+            pa, la = _rows(da, "da", ca.rows, ca.cols, written=True, like=dy)
+            pb, lb = _rows(db, "db", ca.rows, ca.cols, written=True, like=dy)
         cy = Act8.empty(ca.rows, ca.cols, ca.kind, dy.device) if checkpoint is not None else None
         _call("ark_cuda_swiglu_backward", pg, lg, TYPES[dy.dtype], ha, hb, pa, la, pb, lb,
               ctypes.byref(cy.c) if cy is not None else None, s)
@@ -314,23 +358,32 @@ def _qk(q, k, plan, out, names=("q", "k")):
     if not isinstance(plan, RopePlan):
         raise TypeError("plan: expected a RopePlan")
     hq = _heads(q, names[0])
-    if q.shape[2] < plan.rotary_dim:
-        raise ValueError(f"{names[0]}: heads of {q.shape[2]} are shorter than the rotated "
-                         f"{plan.rotary_dim}")
-    hk = None
+    t, h, d = q.shape
+    if d < plan.rotary_dim:
+        raise ValueError(f"{names[0]}: heads of {d} are shorter than the rotated {plan.rotary_dim}")
+    if d > _lib.ARK_ROPE_MAX_DIM:
+        raise ValueError(f"{names[0]}: heads of {d}: at most {_lib.ARK_ROPE_MAX_DIM} are supported")
+    hk = hp = ok = None
     if k is not None:
         hk = _heads(k, names[1], like=q)
-        if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-            raise ValueError(f"{names[1]}: expected [{q.shape[0]}, heads, {q.shape[2]}], got "
-                             f"{tuple(k.shape)}")
+        if k.shape[0] != t or k.shape[2] != d:
+            raise ValueError(f"{names[1]}: expected [{t}, heads, {d}], got {tuple(k.shape)}")
     if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None)
-    oq, ok = out
-    ho = _heads(oq, "out " + names[0], like=q, shape=q.shape, written=True)
-    hp = _heads(ok, "out " + names[1], like=q, shape=k.shape, written=True) if k is not None else None
-    ref = [ctypes.byref(h) if h is not None else None for h in (hq, hk, ho, hp)]
-    return ref, oq, ok
+        oq = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
+        ho = _lib.Heads(oq.data_ptr(), h, h * d, d)
+        if k is not None:
+            h = k.shape[1]
+            ok = torch.empty((t, h, d), dtype=q.dtype, device=q.device)
+            hp = _lib.Heads(ok.data_ptr(), h, h * d, d)
+    else:
+        oq, ok = out
+        ho = _heads(oq, "out " + names[0], like=q, shape=q.shape)
+        if k is not None:
+            hp = _heads(ok, "out " + names[1], like=q, shape=k.shape)
+        elif ok is not None:
+            raise ValueError(f"out {names[1]}: there is no {names[1]}")
+    byref = ctypes.byref
+    return (byref(hq), hk and byref(hk), byref(ho), hp and byref(hp)), oq, ok
 
 
 def rope(q, k, plan, positions=None, seq_len=None, inverse=False, out=None):

@@ -199,16 +199,17 @@ bool shape_ok(uint64_t rows, uint64_t cols, uint64_t ld) {
     return cols < (1ull << 31) && rows < (1ull << 40) && (rows <= 1 || ld >= cols || ld == 0);
 }
 
-template <class K>
-int grid_of(K kernel, uint64_t work) {
-    return streaming_grid(reinterpret_cast<const void*>(kernel), kThreads, 0, work);
+// at most the 8 blocks of 256 threads that an SM holds
+unsigned grid_of(uint64_t work) {
+    const uint64_t need = (work + kThreads - 1) / kThreads, most = (uint64_t)sm_count() * 8;
+    return (unsigned)(need < most ? need : most);
 }
 
 template <class T, int KIND>
 int pack_t(const T* x, uint64_t ldx, const ark_act8* o, cudaStream_t s) {
     const uint32_t per = (uint32_t)(act8_pitch(o->cols) / 8);
     auto k = pack_kernel<T, KIND>;
-    k<<<grid_of(k, o->rows * per), kThreads, 0, s>>>(x, ldx, o->rows, (uint32_t)o->cols, per,
+    k<<<grid_of(o->rows * per), kThreads, 0, s>>>(x, ldx, o->rows, (uint32_t)o->cols, per,
                                                      rows_vec(x, ldx), o->data, o->scale);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
@@ -217,7 +218,7 @@ template <class T, int KIND>
 int unpack_t(const ark_act8* c, T* y, uint64_t ldy, cudaStream_t s) {
     const uint32_t per = (uint32_t)(act8_pitch(c->cols) / 8);
     auto k = unpack_kernel<T, KIND>;
-    k<<<grid_of(k, c->rows * per), kThreads, 0, s>>>(c->data, c->scale, c->rows, (uint32_t)c->cols,
+    k<<<grid_of(c->rows * per), kThreads, 0, s>>>(c->data, c->scale, c->rows, (uint32_t)c->cols,
                                                      per, rows_vec(y, ldy), y, ldy);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
@@ -228,7 +229,7 @@ int swiglu_t(const T* a, uint64_t lda, const T* b, uint64_t ldb, uint64_t rows, 
     const uint32_t per = (uint32_t)(act8_pitch(cols) / 8);
     const bool vec = rows_vec(a, lda) && rows_vec(b, ldb) && rows_vec(y, ldy);
     auto k = swiglu_kernel<T, KIND, HOLD>;
-    k<<<grid_of(k, rows * per), kThreads, 0, s>>>(
+    k<<<grid_of(rows * per), kThreads, 0, s>>>(
         a, lda, b, ldb, rows, (uint32_t)cols, per, vec, y, ldy, HOLD ? a8->data : nullptr,
         HOLD ? a8->scale : nullptr, HOLD ? b8->data : nullptr, HOLD ? b8->scale : nullptr);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
@@ -240,7 +241,7 @@ int swiglu_back_t(const T* dy, uint64_t lddy, const ark_act8* a8, const ark_act8
     const uint32_t per = (uint32_t)(act8_pitch(a8->cols) / 8);
     const bool vec = rows_vec(dy, lddy) && rows_vec(da, ldda) && rows_vec(db, lddb);
     auto k = swiglu_back_kernel<T, KIND, REMAKE>;
-    k<<<grid_of(k, a8->rows * per), kThreads, 0, s>>>(
+    k<<<grid_of(a8->rows * per), kThreads, 0, s>>>(
         dy, lddy, a8->data, a8->scale, b8->data, b8->scale, a8->rows, (uint32_t)a8->cols, per, vec,
         da, ldda, db, lddb, REMAKE ? y8->data : nullptr, REMAKE ? y8->scale : nullptr);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;

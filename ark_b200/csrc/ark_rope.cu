@@ -12,12 +12,13 @@
 // position in the millions is as good as that of the first ones, with one
 // integer product and no table in memory.
 //
-// HBM bounds both passes.  One CTA takes a few tokens at a time: the cosines
-// and sines of their pairs are formed once into shared memory, then groups of
-// lanes each take whole heads.  A lane owns two chunks of VEC elements that
-// hold whole pairs (for the half layout one chunk of each half), so a pair is
-// rotated in one lane, and the same chunks of every head, so gains and the
-// gains' gradients stay with the lane.
+// HBM bounds both passes.  A group of lanes (8 for a head of 128 in 16-bit
+// chunks) takes one token and walks over its heads: the token's cosines and
+// sines are formed once, in registers, and nothing is shared between groups,
+// so no barrier holds loads back.  A lane owns two chunks of VEC elements that
+// hold whole pairs (for the half layout one chunk of each half), the same ones
+// of every head, so a pair is rotated in one lane and the gains' gradients
+// stay with it.  With few tokens the heads of a token are split over groups.
 #include <math.h>
 #include <string.h>
 
@@ -26,7 +27,7 @@
 namespace ark {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxDim = ARK_ROPE_MAX_DIM;
 
 struct Heads {
@@ -48,7 +49,7 @@ struct Args {
     const void* pos;
     int pos64, inverse;
     uint64_t tokens, seq;
-    uint32_t per_block;            // tokens of a CTA at a time
+    uint32_t splits;               // groups that share a token's heads
     Heads q, k, oq, ok;            // inputs (x or dy) and outputs
     const void *gq, *gk;
     int gain_type;
@@ -59,7 +60,7 @@ struct Args {
     int kind;                      // ARK_ACT8_*, or -1: x comes from xq / xk
     Heads xq, xk;
     float* partial;                // backward: [q blocks + k blocks][dim]
-    uint32_t q_blocks;
+    uint32_t q_blocks, q_splits, k_splits;
 };
 
 __device__ __forceinline__ float gain_at(const void* g, int type, uint32_t i) {
@@ -75,14 +76,13 @@ __device__ __forceinline__ int64_t position(const Args& a, uint64_t t) {
                    : (int64_t) static_cast<const int*>(a.pos)[t];
 }
 
-// cos and sin (times the plan's gain) of the pairs of `count` tokens from t0
-__device__ __forceinline__ void angles(const Args& a, const uint64_t* turns, uint64_t t0,
-                                       uint32_t count, float2* cs) {
-    for (uint32_t i = threadIdx.x; i < count * a.d.half; i += kThreads) {
-        const uint32_t t = i / a.d.half, j = i - t * a.d.half;
-        const int64_t p = position(a, t0 + t);
+// cos and sin (times the plan's gain) of `pairs` from the first on, at position p
+template <int N>
+__device__ __forceinline__ void angles(const Args& a, const uint64_t* turns, int64_t p, float2* cs) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
         // the top 32 bits of the turn, signed: [-1/2, 1/2) of a turn
-        const int32_t top = (int32_t)(((uint64_t)p * turns[j]) >> 32);
+        const int32_t top = (int32_t)(((uint64_t)p * turns[i]) >> 32);
         float s, c;
         sincospif(__fmul_rn((float)top, 4.656612873077392578125e-10f), &s, &c);
         if (a.inverse) s = -s;
@@ -127,14 +127,18 @@ __device__ __forceinline__ void store_chunk(T* p, bool there, const float* v) {
 
 // rotate the pairs of a unit in place: x holds chunk 1 then chunk 2
 template <int VEC>
-__device__ __forceinline__ void rotate(const Deal& d, const float2* cs, uint32_t u, float* x) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        const int p = d.interleaved ? 2 * i : i, q = d.interleaved ? 2 * i + 1 : i + VEC;
-        const float2 c = cs[u * VEC + i];
+__device__ __forceinline__ void rotate(const Deal& d, const float2* cs, float* x) {
+    auto turn = [&](int p, int q, float2 c) {
         const float a = x[p], b = x[q];
         x[p] = __fmaf_rn(a, c.x, -__fmul_rn(b, c.y));
         x[q] = __fmaf_rn(b, c.x, __fmul_rn(a, c.y));
+    };
+    if (d.interleaved) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) turn(2 * i, 2 * i + 1, cs[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) turn(i, i + VEC, cs[i]);
     }
 }
 
@@ -165,8 +169,8 @@ __device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col
 
 // a row's columns behind the last head, up to the pitch
 __device__ __forceinline__ void hold_rest(uint8_t* data, uint8_t* scale, uint64_t cols,
-                                          uint64_t pitch) {
-    for (uint64_t c = cols + threadIdx.x * 32; c < pitch; c += kThreads * 32) {
+                                          uint64_t pitch, uint32_t lane, uint32_t lanes) {
+    for (uint64_t c = cols + lane * 32; c < pitch; c += lanes * 32) {
         *reinterpret_cast<uint4*>(data + c) = make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(data + c + 16) = make_uint4(0u, 0u, 0u, 0u);
         scale[c >> 5] = 1;
@@ -178,9 +182,10 @@ __device__ __forceinline__ void hold_rest(uint8_t* data, uint8_t* scale, uint64_
 // and so is its checkpoint.
 template <class T, int VEC, int NU, bool NORM, int HOLD>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args a) {
+    // two heads in flight per lane, where a head is few registers
+    constexpr int kHeads = NU == 1 ? 2 : 1;
     __shared__ uint64_t turns[kMaxDim / 2];
     __shared__ float gains[NORM ? 2 * kMaxDim : 1];
-    extern __shared__ float2 cs[];   // [per_block][half]
     const Deal& d = a.d;
     for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
     if (NORM)
@@ -188,9 +193,10 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
             gains[i] = gain_at(a.gq, a.gain_type, i);
             gains[kMaxDim + i] = a.k.heads ? gain_at(a.gk, a.gain_type, i) : 0.0f;
         }
-    const uint32_t lane = threadIdx.x & (d.group - 1), mine = threadIdx.x / d.group;
-    const uint32_t groups = kThreads / d.group;
-    const uint32_t heads = (uint32_t)(a.q.heads + a.k.heads);
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & (d.group - 1), in_warp = 32 / d.group;
+    const uint32_t hq = (uint32_t)a.q.heads, heads = hq + (uint32_t)a.k.heads;
+    const uint32_t per_split = (heads + a.splits - 1) / a.splits;
     const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
     uint32_t o1[NU], o2[NU];
     bool h1[NU], h2[NU], turned[NU];
@@ -198,69 +204,89 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     for (int n = 0; n < NU; ++n)
         chunks<VEC>(d, lane + n * d.group, o1[n], o2[n], h1[n], h2[n], turned[n]);
 
-    for (uint64_t t0 = (uint64_t)blockIdx.x * a.per_block; t0 < a.tokens;
-         t0 += (uint64_t)gridDim.x * a.per_block) {
-        const uint32_t count = (uint32_t)min((uint64_t)a.per_block, a.tokens - t0);
-        __syncthreads();
-        angles(a, turns, t0, count, cs);
-        __syncthreads();
-        const uint32_t items = count * heads;
-        // all lanes take every round: groups of one warp shuffle together
-        for (uint32_t base = 0; base < items; base += groups) {
-            const uint32_t item = base + mine;
-            const bool on = item < items;
-            const uint32_t tl = on ? item / heads : 0, h = on ? item - tl * heads : 0;
-            const uint64_t t = t0 + tl;
-            const bool is_q = h < a.q.heads;
-            const uint32_t hh = is_q ? h : h - (uint32_t)a.q.heads;
-            const Heads& in = is_q ? a.q : a.k;
-            const Heads& out = is_q ? a.oq : a.ok;
-            const bool live = on && position(a, t) >= 0;
-            const T* x = static_cast<const T*>(in.p) + t * in.ts + hh * in.hs;
-            float v[NU][2 * VEC];
+    // A warp takes as many tasks (a token, a split of its heads) as it has
+    // groups; all its lanes take every round, since groups shuffle together.
+    const uint64_t tasks = a.tokens * a.splits;
+    const uint64_t stride = (uint64_t)gridDim.x * (kThreads / 32) * in_warp;
+    uint64_t first = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * in_warp;
+    for (; first < tasks; first += stride) {
+        const uint64_t task = first + (threadIdx.x & 31) / d.group;
+        const bool on = task < tasks;
+        const uint64_t t = on ? task / a.splits : 0;
+        const uint32_t lo = on ? (uint32_t)(task - t * a.splits) * per_split : 0;
+        const uint32_t hi = on ? min(lo + per_split, heads) : 0;
+        const int64_t p = on ? position(a, t) : -1;
+        const bool live = p >= 0;
+        float2 cs[NU][VEC];
 #pragma unroll
-            for (int n = 0; n < NU; ++n) {
-                load_chunk<VEC>(x + o1[n], live && h1[n], v[n]);
-                load_chunk<VEC>(x + o2[n], live && h2[n], v[n] + VEC);
+        for (int n = 0; n < NU; ++n)
+            if (turned[n] && h1[n]) angles<VEC>(a, turns + (lane + n * d.group) * VEC, p, cs[n]);
+        for (uint32_t step = 0; step < per_split; step += kHeads) {
+            float v[kHeads][NU][2 * VEC];
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) {
+                const uint32_t h = lo + step + j;
+                const bool here = h < hi && live;
+                const Heads& in = h < hq ? a.q : a.k;
+                const T* x = static_cast<const T*>(in.p) + t * in.ts + (h < hq ? h : h - hq) * in.hs;
+#pragma unroll
+                for (int n = 0; n < NU; ++n) {
+                    load_chunk<VEC>(x + o1[n], here && h1[n], v[j][n]);
+                    load_chunk<VEC>(x + o2[n], here && h2[n], v[j][n] + VEC);
+                }
             }
-            if constexpr (HOLD != 0 && VEC == 8) {
-                const uint64_t pitch = is_q ? a.pq : a.pk;
-                hold<HOLD - 1>((is_q ? a.q8 : a.k8) + t * pitch, (is_q ? a.sq : a.sk) + t * (pitch >> 5),
-                               (uint64_t)hh * d.dim, o1[0], o2[0], on && h1[0], v[0]);
-            }
-            if (NORM) {
-                float ss = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NU; ++n)
+            for (int j = 0; j < kHeads; ++j) {
+                const uint32_t h = lo + step + j;
+                const bool here = h < hi, is_q = h < hq;
+                const uint32_t hh = is_q ? h : h - hq;
+                if constexpr (HOLD != 0 && VEC == 8) {
+                    const uint64_t pitch = is_q ? a.pq : a.pk;
+                    hold<HOLD - 1>((is_q ? a.q8 : a.k8) + t * pitch,
+                                   (is_q ? a.sq : a.sk) + t * (pitch >> 5), (uint64_t)hh * d.dim,
+                                   o1[0], o2[0], here && h1[0], v[j][0]);
+                }
+                if (NORM) {
+                    float ss = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(v[n][i], v[n][i], ss);
-                ss = group_sum(ss, d.group);
-                const float r = rsqrtf(__fmaf_rn(ss, inv_dim, a.eps));
-                const float* g = gains + (is_q ? 0 : kMaxDim);
+                    for (int n = 0; n < NU; ++n)
 #pragma unroll
-                for (int n = 0; n < NU; ++n)
+                        for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(v[j][n][i], v[j][n][i], ss);
+                    ss = group_sum(ss, d.group);
+                    const float r = rsqrtf(__fmaf_rn(ss, inv_dim, a.eps));
+                    const float* g = gains + (is_q ? 0 : kMaxDim);
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        if (h1[n]) v[n][i] = __fmul_rn(__fmul_rn(v[n][i], r), g[o1[n] + i]);
-                        if (h2[n]) v[n][VEC + i] = __fmul_rn(__fmul_rn(v[n][VEC + i], r), g[o2[n] + i]);
+                    for (int n = 0; n < NU; ++n)
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) {
+                            if (h1[n])
+                                v[j][n][i] = __fmul_rn(__fmul_rn(v[j][n][i], r), g[o1[n] + i]);
+                            if (h2[n])
+                                v[j][n][VEC + i] =
+                                    __fmul_rn(__fmul_rn(v[j][n][VEC + i], r), g[o2[n] + i]);
+                        }
+                }
+                const Heads& out = is_q ? a.oq : a.ok;
+                T* y = static_cast<T*>(out.p) + t * out.ts + hh * out.hs;
+#pragma unroll
+                for (int n = 0; n < NU; ++n) {
+                    if (turned[n]) rotate<VEC>(d, cs[n], v[j][n]);
+                    if (!live) {
+#pragma unroll
+                        for (int i = 0; i < 2 * VEC; ++i) v[j][n][i] = 0.0f;
                     }
-            }
-            T* y = static_cast<T*>(out.p) + t * out.ts + hh * out.hs;
-#pragma unroll
-            for (int n = 0; n < NU; ++n) {
-                if (turned[n] && h1[n]) rotate<VEC>(d, cs + tl * d.half, lane + n * d.group, v[n]);
-                store_chunk<VEC>(y + o1[n], on && h1[n], v[n]);
-                store_chunk<VEC>(y + o2[n], on && h2[n], v[n] + VEC);
+                    store_chunk<VEC>(y + o1[n], here && h1[n], v[j][n]);
+                    store_chunk<VEC>(y + o2[n], here && h2[n], v[j][n] + VEC);
+                }
             }
         }
-        if constexpr (HOLD != 0 && VEC == 8)
-            for (uint32_t tl = 0; tl < count; ++tl) {
-                hold_rest(a.q8 + (t0 + tl) * a.pq, a.sq + (t0 + tl) * (a.pq >> 5),
-                          a.q.heads * d.dim, a.pq);
+        if constexpr (HOLD != 0 && VEC == 8) {
+            if (on && lo == 0) {
+                hold_rest(a.q8 + t * a.pq, a.sq + t * (a.pq >> 5), a.q.heads * d.dim, a.pq, lane, d.group);
                 if (a.k.heads)
-                    hold_rest(a.k8 + (t0 + tl) * a.pk, a.sk + (t0 + tl) * (a.pk >> 5),
-                              a.k.heads * d.dim, a.pk);
+                    hold_rest(a.k8 + t * a.pk, a.sk + t * (a.pk >> 5), a.k.heads * d.dim, a.pk, lane, d.group);
             }
+        }
     }
 }
 
@@ -293,9 +319,10 @@ __device__ __forceinline__ void held_chunk(const uint8_t* data, const uint8_t* s
 template <class T, int VEC, int NU, int SRC>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args a) {
     __shared__ uint64_t turns[kMaxDim / 2];
-    extern __shared__ float2 cs[];   // [per_block][half]; at the end [groups][dim] floats
+    extern __shared__ float sums[];   // at the end [groups][dim]
     const Deal& d = a.d;
     for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
+    __syncthreads();
     const bool is_q = blockIdx.x < a.q_blocks;
     const uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
     const uint32_t blocks = is_q ? a.q_blocks : gridDim.x - a.q_blocks;
@@ -305,9 +332,9 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
     const uint8_t* data = is_q ? a.q8 : a.k8;
     const uint8_t* scale = is_q ? a.sq : a.sk;
     const uint64_t pitch = is_q ? a.pq : a.pk;
+    const uint32_t splits = is_q ? a.q_splits : a.k_splits, per_split = (heads + splits - 1) / splits;
 
-    const uint32_t lane = threadIdx.x & (d.group - 1), mine = threadIdx.x / d.group;
-    const uint32_t groups = kThreads / d.group;
+    const uint32_t lane = threadIdx.x & (d.group - 1), in_warp = 32 / d.group;
     const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
     uint32_t o1[NU], o2[NU];
     bool h1[NU], h2[NU], turned[NU];
@@ -322,35 +349,40 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
             dg[n][i] = dg[n][VEC + i] = 0.0f;
         }
     }
-    for (uint64_t t0 = (uint64_t)block * a.per_block; t0 < a.tokens;
-         t0 += (uint64_t)blocks * a.per_block) {
-        const uint32_t count = (uint32_t)min((uint64_t)a.per_block, a.tokens - t0);
-        __syncthreads();
-        angles(a, turns, t0, count, cs);
-        __syncthreads();
-        const uint32_t items = count * heads;
-        for (uint32_t base = 0; base < items; base += groups) {
-            const uint32_t item = base + mine;
-            const bool on = item < items;
-            const uint32_t tl = on ? item / heads : 0, h = on ? item - tl * heads : 0;
-            const uint64_t t = t0 + tl;
-            const bool live = on && position(a, t) >= 0;
+    const uint64_t tasks = a.tokens * splits;
+    const uint64_t stride = (uint64_t)blocks * (kThreads / 32) * in_warp;
+    uint64_t first = ((uint64_t)block * (kThreads / 32) + (threadIdx.x >> 5)) * in_warp;
+    for (; first < tasks; first += stride) {
+        const uint64_t task = first + (threadIdx.x & 31) / d.group;
+        const bool on = task < tasks;
+        const uint64_t t = on ? task / splits : 0;
+        const uint32_t lo = on ? (uint32_t)(task - t * splits) * per_split : 0;
+        const uint32_t hi = on ? min(lo + per_split, heads) : 0;
+        const int64_t p = on ? position(a, t) : -1;
+        const bool live = p >= 0;
+        float2 cs[NU][VEC];
+#pragma unroll
+        for (int n = 0; n < NU; ++n)
+            if (turned[n] && h1[n]) angles<VEC>(a, turns + (lane + n * d.group) * VEC, p, cs[n]);
+        for (uint32_t step = 0; step < per_split; ++step) {
+            const uint32_t h = lo + step;
+            const bool here = h < hi, read = here && live;
             const T* dy = static_cast<const T*>(in.p) + t * in.ts + h * in.hs;
             float u[NU][2 * VEC], x[NU][2 * VEC];
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
-                load_chunk<VEC>(dy + o1[n], live && h1[n], u[n]);
-                load_chunk<VEC>(dy + o2[n], live && h2[n], u[n] + VEC);
+                load_chunk<VEC>(dy + o1[n], read && h1[n], u[n]);
+                load_chunk<VEC>(dy + o2[n], read && h2[n], u[n] + VEC);
                 if constexpr (SRC == 0) {
                     const T* xp = static_cast<const T*>(src.p) + t * src.ts + h * src.hs;
-                    load_chunk<VEC>(xp + o1[n], live && h1[n], x[n]);
-                    load_chunk<VEC>(xp + o2[n], live && h2[n], x[n] + VEC);
+                    load_chunk<VEC>(xp + o1[n], read && h1[n], x[n]);
+                    load_chunk<VEC>(xp + o2[n], read && h2[n], x[n] + VEC);
                 } else {
                     const uint8_t* row = data + t * pitch;
                     const uint8_t* srow = scale + t * (pitch >> 5);
                     const uint64_t col = (uint64_t)h * d.dim;
-                    held_chunk<VEC, SRC - 1>(row, srow, col + o1[n], live && h1[n], x[n]);
-                    held_chunk<VEC, SRC - 1>(row, srow, col + o2[n], live && h2[n], x[n] + VEC);
+                    held_chunk<VEC, SRC - 1>(row, srow, col + o1[n], read && h1[n], x[n]);
+                    held_chunk<VEC, SRC - 1>(row, srow, col + o2[n], read && h2[n], x[n] + VEC);
                 }
             }
             float ss = 0.0f;
@@ -359,11 +391,12 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 #pragma unroll
                 for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(x[n][i], x[n][i], ss);
             ss = group_sum(ss, d.group);
-            const float r = rsqrtf(__fmaf_rn(ss, inv_dim, a.eps));
+            // nothing of a padding token may reach the sums, not even 0 * rsqrt(0)
+            const float r = read ? rsqrtf(__fmaf_rn(ss, inv_dim, a.eps)) : 0.0f;
             float dot = 0.0f;
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
-                if (turned[n] && h1[n]) rotate<VEC>(d, cs + tl * d.half, lane + n * d.group, u[n]);
+                if (turned[n] && read) rotate<VEC>(d, cs[n], u[n]);
 #pragma unroll
                 for (int i = 0; i < 2 * VEC; ++i) {
                     x[n][i] = __fmul_rn(x[n][i], r);
@@ -379,14 +412,13 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 #pragma unroll
                 for (int i = 0; i < 2 * VEC; ++i)
                     u[n][i] = __fmul_rn(__fmaf_rn(-x[n][i], dot, u[n][i]), r);
-                store_chunk<VEC>(dx + o1[n], on && h1[n], u[n]);
-                store_chunk<VEC>(dx + o2[n], on && h2[n], u[n] + VEC);
+                store_chunk<VEC>(dx + o1[n], here && h1[n], u[n]);
+                store_chunk<VEC>(dx + o2[n], here && h2[n], u[n] + VEC);
             }
         }
     }
     // the groups' sums, added in group order
-    __syncthreads();
-    float* sums = reinterpret_cast<float*>(cs);
+    const uint32_t mine = threadIdx.x / d.group, groups = kThreads / d.group;
 #pragma unroll
     for (int n = 0; n < NU; ++n)
 #pragma unroll
@@ -506,23 +538,26 @@ int common_ok(const Args& a, uint64_t e, uint64_t dim, int pos_type) {
     return rc;
 }
 
-// Tokens of a CTA at a time: enough pairs for every thread to form one angle,
-// but never so many that SMs stay without a token.
-uint32_t tokens_per_block(uint64_t tokens, uint32_t half) {
-    uint32_t n = kThreads / (half < kThreads ? half : kThreads);
-    if (n > 8) n = 8;
-    while (n > 1 && (tokens + n - 1) / n < (uint64_t)sm_count()) --n;
-    return n ? n : 1;
+// Groups that share a token's heads: one, unless that leaves an SM with fewer
+// than 16 warps; then up to one per head.
+uint32_t splits_of(uint64_t tokens, uint64_t heads, uint32_t group) {
+    const uint64_t want = (uint64_t)sm_count() * 16 * (32 / group);
+    if (heads < 2 || tokens >= want) return 1;
+    const uint64_t n = (want + tokens - 1) / tokens;
+    return (uint32_t)(n < heads ? n : heads);
+}
+
+// blocks that `tasks` groups of lanes fill, at most `most`
+uint32_t blocks_of(uint64_t tasks, uint32_t group, uint64_t most) {
+    const uint64_t per = kThreads / group, need = (tasks + per - 1) / per;
+    return (uint32_t)(need < most ? need : most);
 }
 
 template <class T, int VEC, int NU, bool NORM, int HOLD>
 int forward_t(Args& a, cudaStream_t s) {
-    auto k = forward_kernel<T, VEC, NU, NORM, HOLD>;
-    a.per_block = tokens_per_block(a.tokens, a.d.half);
-    const size_t smem = (size_t)a.per_block * a.d.half * sizeof(float2);
-    const uint64_t work = (a.tokens + a.per_block - 1) / a.per_block;
-    const int grid = streaming_grid(reinterpret_cast<const void*>(k), kThreads, smem, work * kThreads);
-    k<<<grid, kThreads, smem, s>>>(a);
+    a.splits = splits_of(a.tokens, a.q.heads + a.k.heads, a.d.group);
+    const uint32_t grid = blocks_of(a.tokens * a.splits, a.d.group, (uint64_t)sm_count() * 16);
+    forward_kernel<T, VEC, NU, NORM, HOLD><<<grid, kThreads, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
@@ -537,9 +572,7 @@ int forward_v(Args& a, int vec, cudaStream_t s) {
 
 template <class T, int VEC, int NU>
 int backward_t(Args& a, uint32_t blocks, cudaStream_t s) {
-    const size_t angles = (size_t)a.per_block * a.d.half * sizeof(float2);
-    const size_t sums = (size_t)(kThreads / a.d.group) * a.d.dim * sizeof(float);
-    const size_t smem = angles > sums ? angles : sums;
+    const size_t smem = (size_t)(kThreads / a.d.group) * a.d.dim * sizeof(float);
     if (a.kind < 0)
         backward_kernel<T, VEC, NU, 0><<<blocks, kThreads, smem, s>>>(a);
     else if (a.kind == kE4M3)
@@ -549,18 +582,19 @@ int backward_t(Args& a, uint32_t blocks, cudaStream_t s) {
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
-// Blocks of the backward: 4 to an SM, shared between queries and keys by their
-// heads, and none without a token.
-uint32_t back_blocks(uint64_t tokens, uint64_t hq, uint64_t hk, uint32_t per_block, uint32_t* q) {
-    const uint64_t need = (tokens + per_block - 1) / per_block;
-    const uint64_t most = (uint64_t)sm_count() * 4;
+// Blocks of the backward: kBackPerSm to an SM, shared between queries and keys
+// by their heads, and none without a task.
+constexpr uint64_t kBackPerSm = 5;
+uint32_t back_blocks(Args& a) {
+    const uint64_t hq = a.q.heads, hk = a.k.heads, most = (uint64_t)sm_count() * kBackPerSm;
+    const uint64_t tokens = a.tokens ? a.tokens : 1;   // no tokens: a block without work leaves zero sums
+    a.q_splits = splits_of(tokens, hq, a.d.group);
+    a.k_splits = splits_of(tokens, hk, a.d.group);
     uint64_t bq = hq ? most * hq / (hq + hk) : 0, bk = hk ? most - bq : 0;
     if (hq && !bq) bq = 1;
     if (hk && !bk) bk = 1;
-    if (bq > need) bq = need;
-    if (bk > need) bk = need;
-    *q = (uint32_t)bq;
-    return (uint32_t)(bq + bk);
+    a.q_blocks = hq ? blocks_of(tokens * a.q_splits, a.d.group, bq) : 0;
+    return a.q_blocks + (hk ? blocks_of(tokens * a.k_splits, a.d.group, bk) : 0);
 }
 
 void fill_positions(Args& a, const void* positions, int32_t type, uint64_t seq) {
@@ -714,7 +748,7 @@ int ark_cuda_qk_norm_rope(const ark_rope_plan* plan, const ark_heads* q, const a
 }
 
 uint64_t ark_cuda_qk_norm_rope_workspace(uint64_t dim) {
-    return (uint64_t)sm_count() * 4 * dim * sizeof(float) + 2 * dim * sizeof(float);
+    return ((uint64_t)sm_count() * kBackPerSm + 2) * dim * sizeof(float);
 }
 
 int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* dq,
@@ -772,9 +806,7 @@ int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* d
     const Heads all[6] = {a.q, a.k, a.oq, a.ok, a.xq, a.xk};
     const int vec = chunk_of(plan, dim, e, all, 6);
     a.d = deal_of(plan, dim, vec);
-    // no tokens: one block without work leaves zero sums
-    a.per_block = tokens_per_block(tokens, a.d.half);
-    const uint32_t blocks = back_blocks(tokens ? tokens : 1, a.q.heads, a.k.heads, a.per_block, &a.q_blocks);
+    const uint32_t blocks = back_blocks(a);
     rc = by_type(type, [&](auto t) {
         using T = decltype(t);
         return vec == 8   ? backward_t<T, 8, 1>(a, blocks, s)
