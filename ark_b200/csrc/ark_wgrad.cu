@@ -8,8 +8,8 @@
 // registers (exact: at most 8 significant bits times a power of two) and
 // stored to the same swizzled shape, so the 16-bit X never exists in HBM.
 //
-// Warp roles (14 warps): 0-3 epilogue, 4-11 turn bytes into operands, 12 TMA,
-// 13 MMA.  One CTA owns a 128 x BN tile; accumulators are FP32 in TMEM.
+// Warp roles (22 warps): 0-3 epilogue, 4-19 turn bytes into operands, 20 TMA,
+// 21 MMA.  One CTA owns a 128 x BN tile; accumulators are FP32 in TMEM.
 // With enough tiles the grid is persistent and two accumulators alternate, so
 // that the epilogue of a tile runs under the products of the next one.  With
 // few tiles the tokens are split over a cluster of up to 8 CTAs whose FP32
@@ -29,22 +29,23 @@ namespace ark {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpiWarps = 4, kCvtWarps = 8;
+constexpr int kEpiWarps = 4, kTeam = 4, kTeams = 4, kCvtWarps = kTeam * kTeams;
 constexpr int kThreads = (kEpiWarps + kCvtWarps + 2) * 32;
 constexpr int kTmaWarp = kEpiWarps + kCvtWarps, kMmaWarp = kTmaWarp + 1;
 constexpr int kAtom = kBK * 128;              // 64 tokens x 64 columns of 16 bits
 constexpr int kABytes = kBM / 64 * kAtom;
-constexpr int kAhead = 3;                     // byte tiles in flight per thread
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kAhead = 2;                     // steps of a team in flight
+constexpr long long kWaitClocks = 4000000000ll;   // 2 s
 
-template <int BN>
-struct Shape {
-    static constexpr int kBBytes = BN / 64 * kAtom;
-    static constexpr int kStage = kABytes + kBBytes;
-    static constexpr int kStages = BN == 256 ? 4 : 6;
-    static constexpr int kSmem = kStages * kStage + 1024;  // slack to align to 1024
-    static constexpr int kRow = BN + 4;                    // FP32 row of a partial tile
+struct Few {      // a CTA alone: 128 x 128
+    static constexpr int kBN = 128, kBBytes = kBN / 64 * kAtom, kStage = kABytes + kBBytes;
+    static constexpr int kStages = 6, kSmem = kStages * kStage + 1024;   // slack to align to 1024
+    static constexpr int kRow = kBN + 4;                                 // FP32 row of a partial tile
     static_assert(kBM * kRow * 4 <= kStages * kStage, "partial tile fits the stages");
+};
+struct Pair {     // two CTAs: 256 x 256, of which each brings 128 columns of dY
+    static constexpr int kBN = 256, kBBytes = kBN / 2 / 64 * kAtom, kStage = kABytes + kBBytes;
+    static constexpr int kStages = 6, kSmem = kStages * kStage + 1024;
 };
 
 struct Args {
@@ -53,7 +54,8 @@ struct Args {
     uint64_t pitch, spitch;   // bytes
     uint32_t tokens, m, n;
     uint32_t iters;           // 64-token steps in all
-    uint32_t tiles_n, tiles;
+    uint32_t tiles_m, tiles_n, tiles;
+    uint32_t chunks;          // runs of steps whose sums are added by the epilogue
     void* dw;
     uint64_t ldw;
     int dw_f32, dw_bf16, accumulate, vec;
@@ -62,11 +64,6 @@ struct Args {
 // ------------------------------------------------------------ PTX
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
 }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -78,11 +75,21 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
+// an mbarrier's address in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t bar_of(uint32_t bar, uint32_t rank) {
+    uint32_t p;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(bar), "r"(rank));
+    return p;
+}
+__device__ __forceinline__ void bar_arrive_at(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+                 : "memory");
+}
 __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -91,18 +98,29 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
 }
 // false once the wait has run out, or another warp's has
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    if (bar_test(bar, parity)) return true;
-    const uint64_t t0 = now_ns();
+    long long t0 = 0;   // the clock is not read by a wait that ends soon
     for (uint32_t i = 1;; ++i) {
         if (bar_test(bar, parity)) return true;
         if ((i & 63u) == 0) {
             if (*gave_up) return false;
-            if (now_ns() - t0 > kWaitNs) {
+            const long long now = clock64();
+            if (!t0) t0 = now;
+            if (now - t0 > kWaitClocks) {
                 *gave_up = 1;
                 return false;
             }
         }
     }
+}
+// the same, for what has to be over before a CTA leaves
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!bar_test(bar, parity))
+        if (clock64() - t0 > kWaitClocks) break;
+}
+// the first, for all lanes of a warp
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, gave_up));
 }
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y,
                                          uint32_t bar) {
@@ -124,6 +142,23 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+// a pair of CTAs: M = 256, each CTA holds its 128 rows of A and half of B
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+// arrives at the same barrier of both CTAs of the pair
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
@@ -183,12 +218,94 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) {
     asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
+
+// Scale bytes between which q * 2^k needs neither saturation nor a scale
+// outside of T; every block of ordinary activations lies between them.  The
+// others (and NaN blocks) go through FP32.
 template <class T, int KIND>
-__device__ __forceinline__ uint4 operand8(uint2 w, uint32_t byte) {
-    float v[8];
-    dequant8<KIND>(w, byte, v);
-    return make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
-                      pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+struct Fast;
+template <>
+struct Fast<__half, kE4M3> {
+    // 2^-24 is the smallest FP16; 448 * 2^7 is below 65504
+    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 7;
+    __half2 s;
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        s = __float2half2_rn(__uint_as_float(byte << 23));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {   // bytes at, at + 1
+        uint32_t h;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (8 * at))));
+        const __half2 r = __hmul2_rn(*reinterpret_cast<__half2*>(&h), s);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <>
+struct Fast<__half, kInt8> {
+    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 5;
+    __half2 s, t;   // 2^k and -1152 * 2^k
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        const float f = __uint_as_float(byte << 23);
+        s = __float2half2_rn(f);
+        t = __float2half2_rn(__fmul_rn(f, -1152.0f));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
+        // (q + 128) as the low byte of 1024 is 1152 + q: one fused operation
+        // takes the offset off and scales, exactly
+        const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, at ? 0x4342 : 0x4140);
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&h), s, t);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <>
+struct Fast<__nv_bfloat16, kE4M3> {
+    // exponent and mantissa of e4m3 moved to BF16's, whose bias is 120 larger:
+    // the value times 2^-120, subnormals included
+    static constexpr uint32_t kLo = 1, kHi = 127 + 7;
+    __nv_bfloat162 s;
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        s = __float2bfloat162_rn(__uint_as_float((byte + 120u) << 23));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
+        const uint32_t h = __byte_perm(w, 0u, at ? 0x3424 : 0x1404);   // bytes to the high halves
+        const uint32_t v = (h & 0x80008000u) | ((h >> 4) & 0x07F007F0u);
+        const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&v), s);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <>
+struct Fast<__nv_bfloat16, kInt8> {
+    static constexpr uint32_t kLo = 1, kHi = 127 + 120;
+    __nv_bfloat162 s;
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        s = __float2bfloat162_rn(__uint_as_float(byte << 23));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
+        // under the exponent of 128 the low 7 bits are 128 + (q mod 128), and the
+        // sign bit alone is 128 or 256: their difference is q
+        const uint32_t h = __byte_perm(w, 0x43434343u, at ? 0x4342 : 0x4140);
+        const uint32_t lo = h & 0xFF7FFF7Fu, hi = h & 0xFF80FF80u;
+        const __nv_bfloat162 r =
+            __hmul2_rn(__hsub2_rn(*reinterpret_cast<const __nv_bfloat162*>(&lo),
+                                  *reinterpret_cast<const __nv_bfloat162*>(&hi)),
+                       s);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <class T, int KIND>
+__device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uint4& hi) {
+    if (byte >= Fast<T, KIND>::kLo && byte <= Fast<T, KIND>::kHi) {
+        const Fast<T, KIND> f(byte);
+        lo = make_uint4(f.pair(w.x, 0), f.pair(w.x, 2), f.pair(w.y, 0), f.pair(w.y, 2));
+        hi = make_uint4(f.pair(w.z, 0), f.pair(w.z, 2), f.pair(w.w, 0), f.pair(w.w, 2));
+    } else {
+        float v[8];
+        dequant8<KIND>(make_uint2(w.x, w.y), byte, v);
+        lo = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
+                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+        dequant8<KIND>(make_uint2(w.z, w.w), byte, v);
+        hi = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
+                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+    }
 }
 
 // ------------------------------------------------------------ output
@@ -207,14 +324,15 @@ __device__ __forceinline__ void dw_put(const Args& a, uint64_t i, float v) {
 }
 // N (4 or 8) sums of one row, rounded once to the gradient's type
 template <int N>
-__device__ __forceinline__ void dw_row(const Args& a, uint32_t row, uint32_t col, float* v) {
+__device__ __forceinline__ void dw_row(const Args& a, uint32_t row, uint32_t col, float* v,
+                                       bool accumulate) {
     if (row >= a.m || col >= a.n) return;
     const uint64_t i = (uint64_t)row * a.ldw + col;
     if (a.vec && col + N <= a.n) {
         float old[N];
         if (a.dw_f32) {
             float* p = static_cast<float*>(a.dw) + i;
-            if (a.accumulate) {
+            if (accumulate) {
                 load_vec<N>(p, old);
 #pragma unroll
                 for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
@@ -222,7 +340,7 @@ __device__ __forceinline__ void dw_row(const Args& a, uint32_t row, uint32_t col
             store_vec<N>(p, v);
         } else if (a.dw_bf16) {
             __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.dw) + i;
-            if (a.accumulate) {
+            if (accumulate) {
                 load_vec<N>(p, old);
 #pragma unroll
                 for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
@@ -230,7 +348,7 @@ __device__ __forceinline__ void dw_row(const Args& a, uint32_t row, uint32_t col
             store_vec<N>(p, v);
         } else {
             __half* p = static_cast<__half*>(a.dw) + i;
-            if (a.accumulate) {
+            if (accumulate) {
                 load_vec<N>(p, old);
 #pragma unroll
                 for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
@@ -241,63 +359,195 @@ __device__ __forceinline__ void dw_row(const Args& a, uint32_t row, uint32_t col
 #pragma unroll
         for (int j = 0; j < N; ++j)
             if (col + j < a.n)
-                dw_put(a, i + j, a.accumulate ? __fadd_rn(v[j], dw_get(a, i + j)) : v[j]);
+                dw_put(a, i + j, accumulate ? __fadd_rn(v[j], dw_get(a, i + j)) : v[j]);
     }
 }
 
-// ------------------------------------------------------------ the kernel
-template <int BN, class T, int KIND, bool SPLIT>
+// ------------------------------------------------------------ bytes to a stage
+// Which steps of which tiles a CTA works through, in order.
+struct Work {
+    uint32_t first, step, tiles;      // tiles first, first + step, ... below tiles
+    uint32_t it0, it1, chunks;        // its steps of each, in `chunks` runs
+    __device__ __forceinline__ uint32_t chunk_at(uint32_t c) const {
+        return it0 + (uint32_t)((uint64_t)(it1 - it0) * c / chunks);
+    }
+    __device__ __forceinline__ uint32_t steps() const {
+        return first < tiles ? ((tiles - 1 - first) / step + 1) * (it1 - it0) : 0;
+    }
+};
+
+// Teams of 4 warps take steps in turn, so that one's waits, fences and
+// instruction latency run under the others' conversions.  A thread turns 16
+// bytes (half a scale block) of each of four token rows.
+//   column(t): first column of x of this CTA's part of tile t
+//   ready(s, phase): called by one lane once its warp has filled its part
+template <class T, int KIND, int STAGE, int STAGES, class Column, class Ready>
+__device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32_t stages,
+                                            const uint64_t* empty, volatile int* gave_up,
+                                            Column column, Ready ready) {
+    static_assert(STAGES >= kTeams, "a team has a stage of its own");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t = (threadIdx.x - kEpiWarps * 32) & (kTeam * 32 - 1);
+    const uint32_t team = (warp - kEpiWarps) / kTeam;
+    const uint32_t row = t >> 3, unit = t & 7;
+    const uint32_t atom = unit >> 2, chunk = (unit & 3) * 2;
+    uint4 q[kAhead][4];
+    uint32_t sc[kAhead][4];
+    // the step that is loaded next, and where this thread's first row of it is
+    uint32_t lt = w.first, lit = w.it0 + team, tok = 0;
+    const uint8_t *xp = nullptr, *sp = nullptr;
+    auto seek = [&] {
+        while (lit >= w.it1 && lt < w.tiles) lit -= w.it1 - w.it0, lt += w.step;
+        tok = a.tokens;
+        if (lt >= w.tiles) return;
+        const uint64_t col = column(lt);
+        if (col >= a.pitch) return;   // the second half of a pair behind the last column
+        tok = lit * kBK + row;
+        xp = a.x + tok * a.pitch + col + unit * 16;
+        sp = a.scale + tok * a.spitch + (col >> 5) + (unit >> 1);
+    };
+    const uint64_t next_x = kTeams * kBK * a.pitch, next_s = kTeams * kBK * a.spitch;
+    auto load = [&](int p) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            q[p][h] = make_uint4(0u, 0u, 0u, 0u);
+            sc[p][h] = 127;
+            if (tok + 16 * h < a.tokens) {
+                q[p][h] = __ldg(reinterpret_cast<const uint4*>(xp + h * 16 * a.pitch));
+                sc[p][h] = __ldg(sp + h * 16 * a.spitch);
+            }
+        }
+        lit += kTeams;
+        if (lit < w.it1) {
+            if (tok < a.tokens) {
+                tok += kTeams * kBK;
+                xp += next_x;
+                sp += next_s;
+            }
+        } else {
+            seek();
+        }
+    };
+    seek();
+#pragma unroll
+    for (int p = 0; p < kAhead; ++p) load(p);
+    uint32_t todo = (w.steps() + kTeams - 1 - team) / kTeams;
+    uint32_t s = team, phase = 0;
+    bool ok = true;
+    while (ok && todo) {
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p) {
+            if (!ok || !todo) break;
+            if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
+            const uint32_t at = stages + s * STAGE + atom * kAtom;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const uint32_t r = row + 16 * h;
+                uint4 lo, hi;
+                operand16<T, KIND>(q[p][h], sc[p][h], lo, hi);
+                // the two atoms' threads store their halves in opposite order: 8
+                // neighbouring lanes then cover all 32 banks
+                const uint4 one = atom ? hi : lo, two = atom ? lo : hi;
+                const uint32_t base = at + r * 128;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                 base + (((chunk + atom) ^ (r & 7u)) << 4)),
+                             "r"(one.x), "r"(one.y), "r"(one.z), "r"(one.w)
+                             : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                 base + (((chunk + 1 - atom) ^ (r & 7u)) << 4)),
+                             "r"(two.x), "r"(two.y), "r"(two.z), "r"(two.w)
+                             : "memory");
+            }
+            load(p);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) ok = ready(s, phase);
+            ok = __shfl_sync(0xFFFFFFFFu, (int)ok, 0) != 0;
+            s += kTeams;
+            if (s >= STAGES) s -= STAGES, phase ^= 1u;
+            --todo;
+        }
+    }
+}
+
+// ------------------------------------------------------------ the kernels
+// FP32 accumulator, FP16 or BF16 operands, both MN-major
+template <class T>
+__device__ __forceinline__ uint32_t mma_shape(uint32_t m, uint32_t n) {
+    const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return 1u << 4 | type << 7 | type << 10 | 1u << 15 | 1u << 16 | (n >> 3) << 17 | (m >> 4) << 24;
+}
+
+// One lane brings dY's part of every step: columns column(t) on.
+template <int BYTES, int STAGE, int STAGES, class Column>
+__device__ __forceinline__ void bring_steps(const CUtensorMap* map, const Work& w, uint32_t stages,
+                                            const uint64_t* empty, const uint64_t* full_b,
+                                            volatile int* gave_up, Column column) {
+    uint32_t s = 0, phase = 0, loads = 0;
+    bool ok = true;
+    for (uint32_t t = w.first; ok && t < w.tiles; t += w.step) {
+        const int n0 = (int)column(t);
+        for (uint32_t it = w.it0; it < w.it1; ++it) {
+            if (!(ok = bar_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
+            const uint32_t dst = stages + s * STAGE + kABytes, bar = smem_u32(full_b + s);
+            bar_expect(bar, BYTES);
+#pragma unroll
+            for (int j = 0; j < BYTES / kAtom; ++j)
+                tma_load(dst + j * kAtom, map, n0 + 64 * j, (int)(it * kBK), bar);
+            ++loads;
+            if (++s == STAGES) s = 0, phase ^= 1u;
+        }
+    }
+    // the copies in flight land before the CTA may leave
+    for (uint32_t i = 0; i < min(loads, (uint32_t)STAGES); ++i) {
+        const uint32_t l = loads - 1 - i;
+        bar_drain(smem_u32(full_b + l % STAGES), l / STAGES & 1u);
+    }
+}
+
+// Few tiles: one 128 x 128 tile per CTA, the tokens split over the CTAs of a
+// cluster, and each CTA's run of them over up to 4 accumulators, so that no
+// accumulator sums more than it must.  The partial tiles meet in shared memory.
+template <class T, int KIND>
 __global__ void __launch_bounds__(kThreads, 1)
-    wgrad_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
-    using S = Shape<BN>;
+    few_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
+    using S = Few;
     constexpr int kStages = S::kStages;
-    constexpr int kBufs = SPLIT ? 1 : 2;
-    constexpr int kCols = BN * kBufs;   // TMEM columns: 128, 256 or 512
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t bars[3 * kStages + 2 * kBufs + 1];
+    __shared__ uint64_t full[kStages], full_b[kStages], empty[kStages], acc_full, drain;
     __shared__ uint32_t tmem_at;
     __shared__ int gave_up_s;
     volatile int* gave_up = &gave_up_s;
 
     const uint32_t stages = (smem_u32(raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto full_a = [&](int s) { return smem_u32(bars + s); };
-    auto full_b = [&](int s) { return smem_u32(bars + kStages + s); };
-    auto empty = [&](int s) { return smem_u32(bars + 2 * kStages + s); };
-    auto acc_full = [&](int b) { return smem_u32(bars + 3 * kStages + b); };
-    auto acc_empty = [&](int b) { return smem_u32(bars + 3 * kStages + kBufs + b); };
-    const uint32_t drain = smem_u32(bars + 3 * kStages + 2 * kBufs);
-
-    // this CTA's tiles and its steps of each
-    uint32_t parts = 1, part = 0;
-    if (SPLIT) {
-        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
-        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
-    }
-    const uint32_t first = blockIdx.x / parts, step = SPLIT ? a.tiles : gridDim.x;
-    const uint32_t it0 = (uint32_t)((uint64_t)a.iters * part / parts);
-    const uint32_t it1 = (uint32_t)((uint64_t)a.iters * (part + 1) / parts);
-    const uint32_t per_tile = it1 - it0;
+    uint32_t parts, part;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
+    Work w;
+    w.first = blockIdx.x / parts;
+    w.step = w.tiles = a.tiles;
+    w.it0 = (uint32_t)((uint64_t)a.iters * part / parts);
+    w.it1 = (uint32_t)((uint64_t)a.iters * (part + 1) / parts);
+    w.chunks = a.chunks;
+    const uint32_t m0 = w.first / a.tiles_n * kBM, n0 = w.first % a.tiles_n * S::kBN;
 
     if (threadIdx.x == 0) {
         gave_up_s = 0;
         for (int s = 0; s < kStages; ++s) {
-            bar_init(full_a(s), kCvtWarps);
-            bar_init(full_b(s), 1);
-            bar_init(empty(s), 1);
+            bar_init(smem_u32(full + s), kTeam);
+            bar_init(smem_u32(full_b + s), 1);
+            bar_init(smem_u32(empty + s), 1);
         }
-        for (int b = 0; b < kBufs; ++b) {
-            bar_init(acc_full(b), 1);
-            bar_init(acc_empty(b), kEpiWarps);
-        }
-        bar_init(drain, 1);
+        bar_init(smem_u32(&acc_full), 1);
+        bar_init(smem_u32(&drain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&tmem_at)),
-                     "r"(kCols)
+                     "r"(4 * S::kBN)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -307,194 +557,253 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = tmem_at;
 
     if (warp == kTmaWarp) {
-        if (lane == 0) {
-            uint32_t s = 0, phase = 0, loads = 0;
-            bool ok = true;
-            for (uint32_t t = first; ok && t < a.tiles; t += step) {
-                const int n0 = (int)(t % a.tiles_n) * BN;
-                for (uint32_t it = it0; it < it1; ++it) {
-                    if (!(ok = bar_wait(empty(s), phase ^ 1u, gave_up))) break;
-                    const uint32_t dst = stages + s * S::kStage + kABytes;
-                    bar_expect(full_b(s), S::kBBytes);
-                    for (int j = 0; j < BN / 64; ++j)
-                        tma_load(dst + j * kAtom, &map, n0 + 64 * j, (int)(it * kBK), full_b(s));
-                    ++loads;
-                    if (++s == kStages) s = 0, phase ^= 1u;
-                }
-            }
-            // the copies in flight land before the CTA may leave
-            for (uint32_t i = 0; i < min(loads, (uint32_t)kStages); ++i) {
-                const uint32_t l = loads - 1 - i;
-                const uint64_t t0 = now_ns();
-                while (!bar_test(full_b((int)(l % kStages)), (l / kStages) & 1u))
-                    if (now_ns() - t0 > kWaitNs) break;
-            }
-        }
+        if (lane == 0)
+            bring_steps<S::kBBytes, S::kStage, kStages>(&map, w, stages, empty, full_b, gave_up,
+                                                        [&](uint32_t) { return n0; });
     } else if (warp == kMmaWarp) {
         if (lane == 0) {
-            const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-            // FP32 accumulator, both operands MN-major
-            const uint32_t idesc = 1u << 4 | type << 7 | type << 10 | 1u << 15 | 1u << 16 |
-                                   (uint32_t)(BN >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
-            uint32_t s = 0, phase = 0, buf = 0, bphase = 0;
+            const uint32_t shape = mma_shape<T>(kBM, S::kBN);
+            uint32_t s = 0, phase = 0;
             bool ok = true;
-            for (uint32_t t = first; ok && t < a.tiles; t += step) {
-                if (!(ok = bar_wait(acc_empty(buf), bphase ^ 1u, gave_up))) break;
-                fence_after();
-                for (uint32_t it = it0; it < it1; ++it) {
-                    ok = bar_wait(full_b(s), phase, gave_up) && bar_wait(full_a(s), phase, gave_up);
-                    if (!ok) break;
+            for (uint32_t c = 0; ok && c < w.chunks; ++c) {
+                const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
+                for (uint32_t it = from; it < to; ++it) {
+                    if (!(ok = bar_wait(smem_u32(full + s), phase, gave_up))) break;
                     fence_after();
                     const uint32_t at = stages + s * S::kStage;
 #pragma unroll
                     for (int k = 0; k < kBK / 16; ++k)   // 16 tokens: two groups of 8
-                        mma_f16(tmem + buf * BN, operand(at + k * 2048),
-                                operand(at + kABytes + k * 2048), idesc, it > it0 || k > 0);
-                    mma_commit(empty(s));
+                        mma_f16(tmem + c * S::kBN, operand(at + k * 2048),
+                                operand(at + kABytes + k * 2048), shape, it > from || k > 0);
+                    mma_commit(smem_u32(empty + s));
                     if (++s == kStages) s = 0, phase ^= 1u;
                 }
-                if (!ok) break;
-                mma_commit(acc_full(buf));
-                if (++buf == kBufs) buf = 0, bphase ^= 1u;
             }
+            if (ok) mma_commit(smem_u32(&acc_full));
             // no product is in flight when the accumulators are given back
-            mma_commit(drain);
-            const uint64_t t0 = now_ns();
-            while (!bar_test(drain, 0))
-                if (now_ns() - t0 > kWaitNs) break;
+            mma_commit(smem_u32(&drain));
+            bar_drain(smem_u32(&drain), 0);
         }
     } else if (warp >= kEpiWarps) {
-        // 16 bytes (half a scale block) of two token rows per thread and step
-        const int t = threadIdx.x - kEpiWarps * 32;
-        const uint32_t row = t >> 3, unit = t & 7;
-        const uint32_t atom = unit >> 2, chunk = (unit & 3) * 2;
-        uint4 q[kAhead][2];
-        uint32_t sc[kAhead][2];
-        uint32_t lt = first, lit = it0;   // what is loaded next
-        uint64_t lcol = 0;
-        auto load = [&](int p) {
-            const bool any = lt < a.tiles;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t tok = lit * kBK + row + 32 * h;
-                q[p][h] = make_uint4(0u, 0u, 0u, 0u);
-                sc[p][h] = 1;
-                if (any && tok < a.tokens) {
-                    q[p][h] = __ldg(reinterpret_cast<const uint4*>(a.x + tok * a.pitch + lcol + unit * 16));
-                    sc[p][h] = __ldg(a.scale + tok * a.spitch + (lcol >> 5) + (unit >> 1));
-                }
-            }
-            if (++lit == it1) {
-                lit = it0;
-                lt += step;
-                lcol = (uint64_t)(lt / a.tiles_n) * kBM;
-            }
-        };
-        lcol = (uint64_t)(lt / a.tiles_n) * kBM;
-#pragma unroll
-        for (int p = 0; p < kAhead; ++p) load(p);
-        uint32_t todo = 0;
-        for (uint32_t i = first; i < a.tiles; i += step) todo += per_tile;
-        uint32_t s = 0, phase = 0;
-        bool ok = true;
-        while (ok && todo) {
-#pragma unroll
-            for (int p = 0; p < kAhead; ++p) {
-                if (!ok || !todo) break;
-                if (!(ok = bar_wait(empty(s), phase ^ 1u, gave_up))) break;
-                const uint32_t at = stages + s * S::kStage + atom * kAtom;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t r = row + 32 * h;
-                    const uint4 lo = operand8<T, KIND>(make_uint2(q[p][h].x, q[p][h].y), sc[p][h]);
-                    const uint4 hi = operand8<T, KIND>(make_uint2(q[p][h].z, q[p][h].w), sc[p][h]);
-                    // the two atoms' threads store their halves in opposite order: 8
-                    // neighbouring lanes then cover all 32 banks
-                    const uint4 one = atom ? hi : lo, two = atom ? lo : hi;
-                    const uint32_t base = at + r * 128;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                     base + (((chunk + atom) ^ (r & 7u)) << 4)),
-                                 "r"(one.x), "r"(one.y), "r"(one.z), "r"(one.w)
-                                 : "memory");
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                     base + (((chunk + 1 - atom) ^ (r & 7u)) << 4)),
-                                 "r"(two.x), "r"(two.y), "r"(two.z), "r"(two.w)
-                                 : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bar_arrive(full_a(s));
-                if (++s == kStages) s = 0, phase ^= 1u;
-                --todo;
-                load(p);
-            }
-        }
+        fill_stages<T, KIND, S::kStage, kStages>(
+            a, w, stages, empty, gave_up, [&](uint32_t) { return (uint64_t)m0; },
+            [&](uint32_t s, uint32_t phase) {
+                // dY's part has landed too: the products wait on one barrier
+                if (warp % kTeam == 0 && !bar_wait(smem_u32(full_b + s), phase, gave_up)) return false;
+                bar_arrive(smem_u32(full + s));
+                return true;
+            });
     } else {
-        uint32_t buf = 0, bphase = 0;
-        for (uint32_t t = first; t < a.tiles; t += step) {
-            const bool ok = bar_wait(acc_full(buf), bphase, gave_up);
-            __syncwarp();
-            fence_after();
-            const uint32_t m0 = t / a.tiles_n * kBM, n0 = t % a.tiles_n * BN;
-            const uint32_t row = warp * 32 + lane;
+        const bool ok = warp_wait(smem_u32(&acc_full), 0, gave_up);
+        fence_after();
+        const uint32_t row = warp * 32 + lane;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(tmem + buf * BN + ((uint32_t)(warp * 32) << 16) + c, r);
-                float* v = reinterpret_cast<float*>(r);
-                if (!ok) {
+        for (int c = 0; c < S::kBN; c += 32) {
+            float v[32];
+            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + c;
+            tmem_ld32(from, reinterpret_cast<uint32_t*>(v));
+            for (uint32_t k = 1; k < w.chunks; ++k) {
+                float more[32];
+                tmem_ld32(from + k * S::kBN, reinterpret_cast<uint32_t*>(more));
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
-                }
-                if (SPLIT) {
-                    // the stages are idle: every product of this CTA is done
-                    const uint32_t at = stages + (row * S::kRow + c) * 4;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4),
-                                     "f"(v[j]), "f"(v[j + 1]), "f"(v[j + 2]), "f"(v[j + 3])
-                                     : "memory");
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8) dw_row<8>(a, m0 + row, n0 + c + j, v + j);
-                }
+                for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], more[j]);
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(acc_empty(buf));
-            if (++buf == kBufs) buf = 0, bphase ^= 1u;
+            if (!ok) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
+            }
+            // the stages are idle: every product of this CTA is done
+            const uint32_t at = stages + (row * S::kRow + c) * 4;
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4),
+                             "f"(v[j]), "f"(v[j + 1]), "f"(v[j + 2]), "f"(v[j + 3])
+                             : "memory");
         }
+        fence_before();
     }
-
-    if (SPLIT) {
-        __syncwarp();
-        cluster_sync();
-        // rows part, part + parts, ... of the tile: four columns per thread, the
-        // partial tiles added in rank order
-        const uint32_t m0 = first / a.tiles_n * kBM, n0 = first % a.tiles_n * BN;
-        const uint32_t rows = kBM / parts;
-        int lost = 0;   // a partial tile of a CTA that gave up is not to be trusted
-        for (uint32_t p = 0; p < parts; ++p) lost |= peer_flag(smem_u32(&gave_up_s), p);
-        for (uint32_t i = threadIdx.x; i < rows * (BN / 4); i += kThreads) {
-            const uint32_t row = part * rows + i / (BN / 4), col = i % (BN / 4) * 4;
-            const uint32_t at = stages + (row * S::kRow + col) * 4;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t p = 0; p < parts; ++p) {
-                const float4 q = peer_ld(at, p);
-                v[0] = __fadd_rn(v[0], q.x);
-                v[1] = __fadd_rn(v[1], q.y);
-                v[2] = __fadd_rn(v[2], q.z);
-                v[3] = __fadd_rn(v[3], q.w);
-            }
-            if (lost) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
-            dw_row<4>(a, m0 + row, n0 + col, v);
+    __syncwarp();
+    cluster_sync();
+    // this CTA's share of the tile's rows, four columns per thread, the partial
+    // tiles added in rank order
+    const uint32_t rows = kBM / parts;
+    int lost = 0;   // a partial tile of a CTA that gave up is not to be trusted
+    for (uint32_t p = 0; p < parts; ++p) lost |= peer_flag(smem_u32(&gave_up_s), p);
+    for (uint32_t i = threadIdx.x; i < rows * (S::kBN / 4); i += kThreads) {
+        const uint32_t row = part * rows + i / (S::kBN / 4), col = i % (S::kBN / 4) * 4;
+        const uint32_t at = stages + (row * S::kRow + col) * 4;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t p = 0; p < parts; ++p) {
+            const float4 q = peer_ld(at, p);
+            v[0] = __fadd_rn(v[0], q.x);
+            v[1] = __fadd_rn(v[1], q.y);
+            v[2] = __fadd_rn(v[2], q.z);
+            v[3] = __fadd_rn(v[3], q.w);
         }
-        cluster_sync();   // nobody leaves while its tile is read
+        if (lost) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
+        dw_row<4>(a, m0 + row, n0 + col, v, a.accumulate);
+    }
+    cluster_sync();   // nobody leaves while its tile is read
+    if (warp == kMmaWarp) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(4 * S::kBN));
+    }
+}
+
+// Many tiles: pairs of CTAs walk over tiles of 256 x 256.  Each CTA fills its
+// own 128 rows of X and half of dY's columns; the first one's MMA warp issues
+// products that read both.  Per CTA and step that is 32 KB written to and 32
+// KB read from shared memory under 512 clocks of products, where a CTA alone
+// (128 x 256) would move 96 KB and be bound by it.
+__device__ __forceinline__ void pair_tile(const Args& a, uint32_t t, uint32_t& m, uint32_t& n) {
+    // bands of 8 row tiles, so that the tiles at work at one time share both
+    // their columns of X and of dY in L2
+    const uint32_t band = t / (8 * a.tiles_n), at = t - band * 8 * a.tiles_n;
+    const uint32_t high = min(8u, a.tiles_m - band * 8);
+    n = at / high;
+    m = band * 8 + (at - n * high);
+}
+
+template <class T, int KIND>
+__global__ void __launch_bounds__(kThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
+    using S = Pair;
+    constexpr int kStages = S::kStages;
+    extern __shared__ uint8_t raw[];
+    // full, acc_empty, drain: of the first CTA; the others of each
+    __shared__ uint64_t full[kStages], full_b[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+    __shared__ uint32_t tmem_at;
+    __shared__ int gave_up_s;
+    volatile int* gave_up = &gave_up_s;
+
+    const uint32_t stages = (smem_u32(raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    Work w;
+    w.first = blockIdx.x / 2;
+    w.step = gridDim.x / 2;
+    w.tiles = a.tiles;
+    w.it0 = 0;
+    w.it1 = a.iters;
+    w.chunks = a.chunks;
+
+    if (threadIdx.x == 0) {
+        gave_up_s = 0;
+        for (int s = 0; s < kStages; ++s) {
+            bar_init(smem_u32(full + s), 2 * kTeam);
+            bar_init(smem_u32(full_b + s), 1);
+            bar_init(smem_u32(empty + s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            bar_init(smem_u32(acc_full + b), 1);
+            bar_init(smem_u32(acc_empty + b), 2 * kEpiWarps);
+        }
+        bar_init(smem_u32(&drain), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&tmem_at)),
+                     "r"(2 * S::kBN)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
-    if (warp == kMmaWarp)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+    cluster_sync();   // both CTAs' barriers are there before either is used
+    fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp == kTmaWarp) {
+        if (lane == 0)
+            bring_steps<S::kBBytes, S::kStage, kStages>(
+                &map, w, stages, empty, full_b, gave_up, [&](uint32_t t) {
+                    uint32_t m, n;
+                    pair_tile(a, t, m, n);
+                    return n * S::kBN + rank * (S::kBN / 2);
+                });
+    } else if (warp == kMmaWarp) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t shape = mma_shape<T>(2 * kBM, S::kBN);
+            uint32_t s = 0, phase = 0, buf = 0, bphase = 0;
+            bool ok = true;
+            for (uint32_t t = w.first; ok && t < w.tiles; t += w.step)
+                for (uint32_t c = 0; ok && c < w.chunks; ++c) {
+                    if (!(ok = bar_wait(smem_u32(acc_empty + buf), bphase ^ 1u, gave_up))) break;
+                    fence_after();
+                    const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
+                    for (uint32_t it = from; it < to; ++it) {
+                        if (!(ok = bar_wait(smem_u32(full + s), phase, gave_up))) break;
+                        fence_after();
+                        const uint32_t at = stages + s * S::kStage;
+#pragma unroll
+                        for (int k = 0; k < kBK / 16; ++k)
+                            mma_f16_pair(tmem + buf * S::kBN, operand(at + k * 2048),
+                                         operand(at + kABytes + k * 2048), shape, it > from || k > 0);
+                        mma_commit_pair(smem_u32(empty + s));
+                        if (++s == kStages) s = 0, phase ^= 1u;
+                    }
+                    if (!ok) break;
+                    mma_commit_pair(smem_u32(acc_full + buf));
+                    if (++buf == 2) buf = 0, bphase ^= 1u;
+                }
+            mma_commit_pair(smem_u32(&drain));
+            bar_drain(smem_u32(&drain), 0);
+        }
+    } else if (warp >= kEpiWarps) {
+        fill_stages<T, KIND, S::kStage, kStages>(
+            a, w, stages, empty, gave_up,
+            [&](uint32_t t) {
+                uint32_t m, n;
+                pair_tile(a, t, m, n);
+                return (uint64_t)m * (2 * kBM) + rank * kBM;
+            },
+            [&](uint32_t s, uint32_t phase) {
+                // this CTA's part of dY has landed too: the products wait on one barrier
+                if (warp % kTeam == 0 && !bar_wait(smem_u32(full_b + s), phase, gave_up)) return false;
+                bar_arrive_at(bar_of(smem_u32(full + s), 0));
+                return true;
+            });
+    } else {
+        uint32_t buf = 0, bphase = 0;
+        for (uint32_t t = w.first; t < w.tiles; t += w.step)
+            for (uint32_t k = 0; k < w.chunks; ++k) {
+                const bool ok = warp_wait(smem_u32(acc_full + buf), bphase, gave_up);
+                fence_after();
+                uint32_t m, n;
+                pair_tile(a, t, m, n);
+                const uint32_t row = m * (2 * kBM) + rank * kBM + warp * 32 + lane;
+#pragma unroll 1
+                for (int c = 0; c < S::kBN; c += 32) {
+                    float v[32];
+                    tmem_ld32(tmem + buf * S::kBN + ((uint32_t)(warp * 32) << 16) + c,
+                              reinterpret_cast<uint32_t*>(v));
+                    if (!ok) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        dw_row<8>(a, row, n * S::kBN + c + j, v + j, a.accumulate || k > 0);
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_at(bar_of(smem_u32(acc_empty + buf), 0));
+                if (++buf == 2) buf = 0, bphase ^= 1u;
+            }
+    }
+    __syncwarp();
+    fence_before();
+    cluster_sync();   // no product or barrier of the pair is used after this
+    if (warp == kMmaWarp) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(2 * S::kBN));
+    }
+    cluster_sync();
 }
 
 // dY whose rows TMA cannot address, copied to rows of a multiple of 16 bytes
@@ -541,41 +850,41 @@ bool tma_rows(const void* p, uint64_t ld, uint64_t cols) {
 }
 uint64_t realigned(uint64_t cols) { return (cols + 7) / 8 * 8; }
 
-template <int BN, class T, int KIND, bool SPLIT>
-int launch(const CUtensorMap& map, const Args& a, uint32_t parts, cudaStream_t s) {
-    auto k = wgrad_kernel<BN, T, KIND, SPLIT>;
-    static std::atomic<uint64_t> ready{0};   // devices whose shared-memory limit is raised
+using Kernel = void (*)(const CUtensorMap, const Args);
+
+template <class T, int KIND>
+Kernel kernel_of(bool pair) {
+    return pair ? pair_kernel<T, KIND> : few_kernel<T, KIND>;
+}
+
+int launch(const CUtensorMap& map, const Args& a, int32_t type, int32_t kind, bool pair,
+           uint32_t cluster, uint32_t grid, cudaStream_t s) {
+    const int which = (type == ARK_TYPE_BF16) << 2 | (kind == kInt8) << 1 | (int)pair;
+    const Kernel k = type == ARK_TYPE_F16
+                         ? (kind == kE4M3 ? kernel_of<__half, kE4M3>(pair) : kernel_of<__half, kInt8>(pair))
+                         : (kind == kE4M3 ? kernel_of<__nv_bfloat16, kE4M3>(pair)
+                                          : kernel_of<__nv_bfloat16, kInt8>(pair));
+    const int smem = pair ? Pair::kSmem : Few::kSmem;
+    static std::atomic<uint64_t> ready[8];   // devices whose shared-memory limit is raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ARK_E_CUDA;
-    if (dev >= 64 || !(ready.load() >> dev & 1)) {
-        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 Shape<BN>::kSmem) != cudaSuccess)
+    if (dev >= 64 || !(ready[which].load() >> dev & 1)) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return ARK_E_CUDA;
-        if (dev < 64) ready.fetch_or(1ull << dev);
+        if (dev < 64) ready[which].fetch_or(1ull << dev);
     }
     cudaLaunchConfig_t cfg = {};
-    const uint32_t sms = (uint32_t)sm_count();
-    cfg.gridDim = dim3(SPLIT ? a.tiles * parts : (a.tiles < sms ? a.tiles : sms));
+    cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<BN>::kSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = SPLIT ? parts : 1;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, k, map, a) == cudaSuccess ? ARK_OK : ARK_E_CUDA;
-}
-
-template <int BN, bool SPLIT>
-int dispatch(const CUtensorMap& map, const Args& a, int32_t type, int32_t kind, uint32_t parts,
-             cudaStream_t s) {
-    if (type == ARK_TYPE_F16)
-        return kind == kE4M3 ? launch<BN, __half, kE4M3, SPLIT>(map, a, parts, s)
-                             : launch<BN, __half, kInt8, SPLIT>(map, a, parts, s);
-    return kind == kE4M3 ? launch<BN, __nv_bfloat16, kE4M3, SPLIT>(map, a, parts, s)
-                         : launch<BN, __nv_bfloat16, kInt8, SPLIT>(map, a, parts, s);
 }
 
 }  // namespace
@@ -655,19 +964,25 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return ARK_E_CUDA;
 
-    const uint32_t sms = (uint32_t)sm_count(), tiles_m = (a.m + kBM - 1) / kBM;
-    const uint32_t wide = tiles_m * ((a.n + 255) / 256);
-    if (wide >= sms) {
+    const uint32_t sms = (uint32_t)sm_count();
+    const uint32_t pairs = ((a.m + 255) / 256) * ((a.n + 255) / 256);
+    if (pairs * 2 >= sms * 3 / 4) {
+        a.tiles_m = (a.m + 255) / 256;
         a.tiles_n = (a.n + 255) / 256;
-        a.tiles = wide;
-        return dispatch<256, false>(map, a, dy_type, x->kind, 1, s);
+        a.tiles = pairs;
+        // the tensor cores' FP32 sums are cut off, not rounded: FP32 gradients of
+        // more than 2048 tokens are summed in runs that the epilogue adds
+        a.chunks = a.dw_f32 ? (a.iters + 31) / 32 : 1;
+        return launch(map, a, dy_type, x->kind, true, 2, 2 * (pairs < sms / 2 ? pairs : sms / 2), s);
     }
-    a.tiles_n = (a.n + 127) / 128;
-    a.tiles = tiles_m * a.tiles_n;
+    a.tiles_m = (a.m + kBM - 1) / kBM;
+    a.tiles_n = (a.n + Few::kBN - 1) / Few::kBN;
+    a.tiles = a.tiles_m * a.tiles_n;
     uint32_t parts = 1;
     while (parts < 8 && a.tiles * parts * 2 <= sms && parts * 2 <= a.iters) parts *= 2;
-    if (parts == 1) return dispatch<128, false>(map, a, dy_type, x->kind, 1, s);
-    return dispatch<128, true>(map, a, dy_type, x->kind, parts, s);
+    a.chunks = a.iters / parts / 16;
+    a.chunks = a.chunks < 1 ? 1 : a.chunks > 4 ? 4 : a.chunks;
+    return launch(map, a, dy_type, x->kind, false, parts, a.tiles * parts, s);
 }
 
 }  // extern "C"
