@@ -3,18 +3,24 @@
 //
 // Both operands have the summed dimension (tokens) as their slow one, so both
 // go to the tensor cores MN-major: a stage holds 64 tokens as rows of 128
-// bytes (64 columns), 8 rows to a 1024-byte swizzle atom.  dY comes in that
-// shape by TMA.  X is read as bytes, 16 per thread, turned into FP16 / BF16 in
-// registers (exact: at most 8 significant bits times a power of two) and
-// stored to the same swizzled shape, so the 16-bit X never exists in HBM.
+// bytes (64 columns), 8 rows to a 1024-byte swizzle atom; accumulators are FP32
+// in TMEM.  A byte of X becomes an FP16 / BF16 operand exactly (at most 8
+// significant bits times a power of two).
 //
-// Warp roles (22 warps): 0-3 epilogue, 4-19 turn bytes into operands, 20 TMA,
-// 21 MMA.  One CTA owns a 128 x BN tile; accumulators are FP32 in TMEM.
-// With enough tiles the grid is persistent and two accumulators alternate, so
-// that the epilogue of a tile runs under the products of the next one.  With
-// few tiles the tokens are split over a cluster of up to 8 CTAs whose FP32
-// partial tiles are added over distributed shared memory in rank order: one
-// launch, no workspace, the same bits every time.
+// Many tiles (pair_kernel): X is unpacked once into a 16-bit workspace, then
+// both operands come by TMA to pairs of CTAs with 256 x 256 tiles.  The grid is
+// persistent and two accumulators alternate, so that the epilogue of a tile
+// runs under the products of the next one.  Turning the bytes into operands
+// inside this kernel was built and measured first: every tile of dY's columns
+// turns the same bytes again, and at the power limit each instruction beside
+// the products costs clock: 8192 tokens, 4096 x 11008: 640 us against 488 us
+// for the products alone.
+//
+// Few tiles (few_kernel): latency counts, so one launch does it all.  One CTA
+// per 128 x 128 tile; 8 of its 14 warps read bytes, turn them in registers and
+// store them to the swizzled shape, dY comes by TMA.  The tokens are split over
+// a cluster of up to 8 CTAs whose FP32 partial tiles are added over distributed
+// shared memory in rank order: no workspace, the same bits every time.
 //
 // Every wait is bounded.  One that runs out makes its CTA leave with NaN as
 // its tile, which the step's finite check turns into a skipped step.
@@ -29,12 +35,14 @@ namespace ark {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpiWarps = 4, kTeam = 4, kTeams = 4, kCvtWarps = kTeam * kTeams;
+constexpr int kEpiWarps = 4, kTeam = 4, kTeams = 2, kCvtWarps = kTeam * kTeams;
 constexpr int kThreads = (kEpiWarps + kCvtWarps + 2) * 32;
 constexpr int kTmaWarp = kEpiWarps + kCvtWarps, kMmaWarp = kTmaWarp + 1;
+constexpr int kPairEpiWarps = 8, kPairThreads = (kPairEpiWarps + 2) * 32;
 constexpr int kAtom = kBK * 128;              // 64 tokens x 64 columns of 16 bits
 constexpr int kABytes = kBM / 64 * kAtom;
 constexpr int kAhead = 2;                     // steps of a team in flight
+constexpr uint32_t kSleepNs = 1000000;
 constexpr long long kWaitClocks = 4000000000ll;   // 2 s
 
 struct Few {      // a CTA alone: 128 x 128
@@ -71,9 +79,25 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
+// The instructions below that one lane issues take their operands from uniform
+// registers.  All lanes of the warp run through them and `me` predicates the
+// instruction itself: inside a branch on the lane, each operand would be moved to
+// a uniform register first, and the issuing lane became the bottleneck (640
+// clocks a step, of which the products take 512).
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes, uint32_t me) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+        " @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar),
+        "r"(bytes), "r"(me)
+        : "memory");
+}
+// one lane of a converged warp
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t me;
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(me));
+    return me;
 }
 // an mbarrier's address in the cluster's CTA `rank`
 __device__ __forceinline__ uint32_t bar_of(uint32_t bar, uint32_t rank) {
@@ -81,27 +105,44 @@ __device__ __forceinline__ uint32_t bar_of(uint32_t bar, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(bar), "r"(rank));
     return p;
 }
+// Arrives at a barrier of either CTA of a pair.  What the arrival stands for is
+// an SM's own shared memory or TMEM, read by that SM's tensor cores: the writer's
+// proxy fence (or tcgen05 fence) before it orders that, and a release at cluster
+// scope, which measured 1400 clocks, is not needed for it.
 __device__ __forceinline__ void bar_arrive_at(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
-                 : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
     return ok != 0;
 }
-// false once the wait has run out, or another warp's has
+// a poll that may sleep for kSleepNs
+__device__ __forceinline__ bool bar_sleep(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kSleepNs)
+        : "memory");
+    return ok != 0;
+}
+// False once the wait has run out, or another warp's has.
+enum How { kPoll, kSleep };   // kSleep: for a whole tile
+template <How HOW = kPoll>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
     long long t0 = 0;   // the clock is not read by a wait that ends soon
     for (uint32_t i = 1;; ++i) {
-        if (bar_test(bar, parity)) return true;
-        if ((i & 63u) == 0) {
+        if (HOW == kSleep ? bar_sleep(bar, parity) : bar_test(bar, parity)) return true;
+        if (HOW == kSleep || (i & 63u) == 0) {
             if (*gave_up) return false;
             const long long now = clock64();
             if (!t0) t0 = now;
@@ -119,52 +160,70 @@ __device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
         if (clock64() - t0 > kWaitClocks) break;
 }
 // the first, for all lanes of a warp
+template <How HOW = kPoll>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, gave_up));
+    return __all_sync(0xFFFFFFFFu, bar_wait<HOW>(bar, parity, gave_up));
 }
+// PAIR: the barrier may be the other CTA's
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                         uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
+                                         uint32_t bar, uint32_t me) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+            " @q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%2, %3}], [%4];\n}\n" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar), "r"(me)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+            " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%2, %3}], [%4];\n}\n" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar), "r"(me)
+            : "memory");
 }
 // Shared-memory operand, MN-major, 128-byte swizzle: 64-column atoms kAtom
-// bytes apart, groups of 8 tokens 1024 bytes apart.
+// bytes apart, groups of 8 tokens 1024 bytes apart.  The address field counts 16
+// bytes, so operand(at) + bytes / 16 is the operand `bytes` further on.
 __device__ __forceinline__ uint64_t operand(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(kAtom >> 4) << 16 |
            (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
+// PAIR: a pair of CTAs, M = 256, each CTA holds its 128 rows of A and half of B
+template <bool PAIR>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                        uint32_t add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(add)
-        : "memory");
+                                        uint32_t add, uint32_t me) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(me)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(me)
+            : "memory");
 }
-// a pair of CTAs: M = 256, each CTA holds its 128 rows of A and half of B
-__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                             uint32_t add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(add)
-        : "memory");
-}
-// arrives at the same barrier of both CTAs of the pair
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
-        : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-        : "memory");
+// PAIR: arrives at the same barrier of both CTAs
+template <bool PAIR>
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t me) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+            " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+            "[%0], %1;\n}\n" ::"r"(bar),
+            "h"((uint16_t)3), "r"(me)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+                bar),
+            "r"(me)
+            : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
     asm volatile(
@@ -371,20 +430,16 @@ struct Work {
     __device__ __forceinline__ uint32_t chunk_at(uint32_t c) const {
         return it0 + (uint32_t)((uint64_t)(it1 - it0) * c / chunks);
     }
-    __device__ __forceinline__ uint32_t steps() const {
-        return first < tiles ? ((tiles - 1 - first) / step + 1) * (it1 - it0) : 0;
-    }
 };
 
 // Teams of 4 warps take steps in turn, so that one's waits, fences and
-// instruction latency run under the others' conversions.  A thread turns 16
+// instruction latency run under the other's conversions.  A thread turns 16
 // bytes (half a scale block) of each of four token rows.
-//   column(t): first column of x of this CTA's part of tile t
-//   ready(s, phase): called by one lane once its warp has filled its part
-template <class T, int KIND, int STAGE, int STAGES, class Column, class Ready>
-__device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32_t stages,
-                                            const uint64_t* empty, volatile int* gave_up,
-                                            Column column, Ready ready) {
+//   col: first column of x of this CTA's tile
+template <class T, int KIND, int STAGE, int STAGES>
+__device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32_t col,
+                                            uint32_t stages, const uint64_t* empty,
+                                            const uint64_t* full, volatile int* gave_up) {
     static_assert(STAGES >= kTeams, "a team has a stage of its own");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = (threadIdx.x - kEpiWarps * 32) & (kTeam * 32 - 1);
@@ -393,61 +448,50 @@ __device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32
     const uint32_t atom = unit >> 2, chunk = (unit & 3) * 2;
     uint4 q[kAhead][4];
     uint32_t sc[kAhead][4];
-    // the step that is loaded next, and where this thread's first row of it is
-    uint32_t lt = w.first, lit = w.it0 + team, tok = 0;
-    const uint8_t *xp = nullptr, *sp = nullptr;
-    auto seek = [&] {
-        while (lit >= w.it1 && lt < w.tiles) lit -= w.it1 - w.it0, lt += w.step;
-        tok = a.tokens;
-        if (lt >= w.tiles) return;
-        const uint64_t col = column(lt);
-        if (col >= a.pitch) return;   // the second half of a pair behind the last column
-        tok = lit * kBK + row;
-        xp = a.x + tok * a.pitch + col + unit * 16;
-        sp = a.scale + tok * a.spitch + (col >> 5) + (unit >> 1);
-    };
+    // this thread's first row of the step that is loaded next, and where the
+    // part's rows end
+    uint32_t tok = (w.it0 + team) * kBK + row;
+    const uint32_t end = min(a.tokens, w.it1 * kBK);
+    const uint8_t* xp = a.x + tok * a.pitch + col + unit * 16;
+    const uint8_t* sp = a.scale + tok * a.spitch + (col >> 5) + (unit >> 1);
     const uint64_t next_x = kTeams * kBK * a.pitch, next_s = kTeams * kBK * a.spitch;
     auto load = [&](int p) {
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
             q[p][h] = make_uint4(0u, 0u, 0u, 0u);
             sc[p][h] = 127;
-            if (tok + 16 * h < a.tokens) {
+            if (tok + 16 * h < end) {
                 q[p][h] = __ldg(reinterpret_cast<const uint4*>(xp + h * 16 * a.pitch));
                 sc[p][h] = __ldg(sp + h * 16 * a.spitch);
             }
         }
-        lit += kTeams;
-        if (lit < w.it1) {
-            if (tok < a.tokens) {
-                tok += kTeams * kBK;
-                xp += next_x;
-                sp += next_s;
-            }
-        } else {
-            seek();
-        }
+        tok += kTeams * kBK;
+        xp += next_x;
+        sp += next_s;
     };
-    seek();
 #pragma unroll
     for (int p = 0; p < kAhead; ++p) load(p);
-    uint32_t todo = (w.steps() + kTeams - 1 - team) / kTeams;
+    uint32_t todo = (w.it1 - w.it0 + kTeams - 1 - team) / kTeams;
     uint32_t s = team, phase = 0;
     bool ok = true;
     while (ok && todo) {
 #pragma unroll
         for (int p = 0; p < kAhead; ++p) {
             if (!ok || !todo) break;
+            // converted in registers before the stage is free: a stage is held
+            // only while it is written
+            uint4 lo[4], hi[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) operand16<T, KIND>(q[p][h], sc[p][h], lo[h], hi[h]);
+            load(p);
             if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
             const uint32_t at = stages + s * STAGE + atom * kAtom;
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 const uint32_t r = row + 16 * h;
-                uint4 lo, hi;
-                operand16<T, KIND>(q[p][h], sc[p][h], lo, hi);
                 // the two atoms' threads store their halves in opposite order: 8
                 // neighbouring lanes then cover all 32 banks
-                const uint4 one = atom ? hi : lo, two = atom ? lo : hi;
+                const uint4 one = atom ? hi[h] : lo[h], two = atom ? lo[h] : hi[h];
                 const uint32_t base = at + r * 128;
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
                                  base + (((chunk + atom) ^ (r & 7u)) << 4)),
@@ -458,11 +502,9 @@ __device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32
                              "r"(two.x), "r"(two.y), "r"(two.z), "r"(two.w)
                              : "memory");
             }
-            load(p);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) ok = ready(s, phase);
-            ok = __shfl_sync(0xFFFFFFFFu, (int)ok, 0) != 0;
+            if (lane == 0) bar_arrive(smem_u32(full + s));
             s += kTeams;
             if (s >= STAGES) s -= STAGES, phase ^= 1u;
             --todo;
@@ -478,31 +520,12 @@ __device__ __forceinline__ uint32_t mma_shape(uint32_t m, uint32_t n) {
     return 1u << 4 | type << 7 | type << 10 | 1u << 15 | 1u << 16 | (n >> 3) << 17 | (m >> 4) << 24;
 }
 
-// One lane brings dY's part of every step: columns column(t) on.
-template <int BYTES, int STAGE, int STAGES, class Column>
-__device__ __forceinline__ void bring_steps(const CUtensorMap* map, const Work& w, uint32_t stages,
-                                            const uint64_t* empty, const uint64_t* full_b,
-                                            volatile int* gave_up, Column column) {
-    uint32_t s = 0, phase = 0, loads = 0;
-    bool ok = true;
-    for (uint32_t t = w.first; ok && t < w.tiles; t += w.step) {
-        const int n0 = (int)column(t);
-        for (uint32_t it = w.it0; it < w.it1; ++it) {
-            if (!(ok = bar_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
-            const uint32_t dst = stages + s * STAGE + kABytes, bar = smem_u32(full_b + s);
-            bar_expect(bar, BYTES);
-#pragma unroll
-            for (int j = 0; j < BYTES / kAtom; ++j)
-                tma_load(dst + j * kAtom, map, n0 + 64 * j, (int)(it * kBK), bar);
-            ++loads;
-            if (++s == STAGES) s = 0, phase ^= 1u;
-        }
-    }
-    // the copies in flight land before the CTA may leave
-    for (uint32_t i = 0; i < min(loads, (uint32_t)STAGES); ++i) {
-        const uint32_t l = loads - 1 - i;
-        bar_drain(smem_u32(full_b + l % STAGES), l / STAGES & 1u);
-    }
+// Every copy has landed when the products that read it are done.  Where those
+// were given up, a copy in flight gets far longer than one takes (2 ms) before
+// the CTA may leave.
+__device__ __forceinline__ void settle() {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitClocks / 1000) {}
 }
 
 // Few tiles: one 128 x 128 tile per CTA, the tokens split over the CTAs of a
@@ -514,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using S = Few;
     constexpr int kStages = S::kStages;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[kStages], full_b[kStages], empty[kStages], acc_full, drain;
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full, drain;
     __shared__ uint32_t tmem_at;
     __shared__ int gave_up_s;
     volatile int* gave_up = &gave_up_s;
@@ -535,8 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         gave_up_s = 0;
         for (int s = 0; s < kStages; ++s) {
-            bar_init(smem_u32(full + s), kTeam);
-            bar_init(smem_u32(full_b + s), 1);
+            bar_init(smem_u32(full + s), kTeam + 1);
             bar_init(smem_u32(empty + s), 1);
         }
         bar_init(smem_u32(&acc_full), 1);
@@ -557,44 +579,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = tmem_at;
 
     if (warp == kTmaWarp) {
-        if (lane == 0)
-            bring_steps<S::kBBytes, S::kStage, kStages>(&map, w, stages, empty, full_b, gave_up,
-                                                        [&](uint32_t) { return n0; });
-    } else if (warp == kMmaWarp) {
-        if (lane == 0) {
-            const uint32_t shape = mma_shape<T>(kBM, S::kBN);
-            uint32_t s = 0, phase = 0;
-            bool ok = true;
-            for (uint32_t c = 0; ok && c < w.chunks; ++c) {
-                const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
-                for (uint32_t it = from; it < to; ++it) {
-                    if (!(ok = bar_wait(smem_u32(full + s), phase, gave_up))) break;
-                    fence_after();
-                    const uint32_t at = stages + s * S::kStage;
+        const uint32_t me = elect();
+        uint32_t s = 0, phase = 0;
+        bool ok = true;
+        for (uint32_t it = w.it0; it < w.it1; ++it) {
+            if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
+            const uint32_t dst = stages + s * S::kStage + kABytes, bar = smem_u32(full + s);
+            bar_expect(bar, S::kBBytes, me);
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k)   // 16 tokens: two groups of 8
-                        mma_f16(tmem + c * S::kBN, operand(at + k * 2048),
-                                operand(at + kABytes + k * 2048), shape, it > from || k > 0);
-                    mma_commit(smem_u32(empty + s));
-                    if (++s == kStages) s = 0, phase ^= 1u;
-                }
-            }
-            if (ok) mma_commit(smem_u32(&acc_full));
-            // no product is in flight when the accumulators are given back
-            mma_commit(smem_u32(&drain));
-            bar_drain(smem_u32(&drain), 0);
+            for (int j = 0; j < S::kBBytes / kAtom; ++j)
+                tma_load<false>(dst + j * kAtom, &map, (int)n0 + 64 * j, (int)(it * kBK), bar, me);
+            if (++s == kStages) s = 0, phase ^= 1u;
         }
+        if (!ok) settle();
+    } else if (warp == kMmaWarp) {
+        const uint32_t me = elect(), shape = mma_shape<T>(kBM, S::kBN);
+        uint32_t s = 0, phase = 0;
+        bool ok = true;
+        for (uint32_t c = 0; ok && c < w.chunks; ++c) {
+            const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
+            for (uint32_t it = from; it < to; ++it) {
+                if (!(ok = warp_wait(smem_u32(full + s), phase, gave_up))) break;
+                fence_after();
+                const uint64_t x = operand(stages + s * S::kStage), y = x + kABytes / 16;
+#pragma unroll
+                for (int k = 0; k < kBK / 16; ++k)   // 16 tokens: two groups of 8
+                    mma_f16<false>(tmem + c * S::kBN, x + k * (2048 / 16), y + k * (2048 / 16), shape,
+                                   it > from || k > 0, me);
+                mma_commit<false>(smem_u32(empty + s), me);
+                if (++s == kStages) s = 0, phase ^= 1u;
+            }
+        }
+        if (ok) mma_commit<false>(smem_u32(&acc_full), me);
+        // no product is in flight when the accumulators are given back
+        mma_commit<false>(smem_u32(&drain), me);
+        bar_drain(smem_u32(&drain), 0);
     } else if (warp >= kEpiWarps) {
-        fill_stages<T, KIND, S::kStage, kStages>(
-            a, w, stages, empty, gave_up, [&](uint32_t) { return (uint64_t)m0; },
-            [&](uint32_t s, uint32_t phase) {
-                // dY's part has landed too: the products wait on one barrier
-                if (warp % kTeam == 0 && !bar_wait(smem_u32(full_b + s), phase, gave_up)) return false;
-                bar_arrive(smem_u32(full + s));
-                return true;
-            });
+        fill_stages<T, KIND, S::kStage, kStages>(a, w, m0, stages, empty, full, gave_up);
     } else {
-        const bool ok = warp_wait(smem_u32(&acc_full), 0, gave_up);
+        const bool ok = warp_wait<kSleep>(smem_u32(&acc_full), 0, gave_up);
         fence_after();
         const uint32_t row = warp * 32 + lane;
 #pragma unroll 1
@@ -651,11 +674,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Many tiles: pairs of CTAs walk over tiles of 256 x 256.  Each CTA fills its
-// own 128 rows of X and half of dY's columns; the first one's MMA warp issues
-// products that read both.  Per CTA and step that is 32 KB written to and 32
-// KB read from shared memory under 512 clocks of products, where a CTA alone
-// (128 x 256) would move 96 KB and be bound by it.
+// Many tiles: pairs of CTAs walk over tiles of 256 x 256 of X (turned into
+// 16-bit operands by a pass before) and dY.  Each CTA brings its own 128 columns
+// of X and half of dY's; the first one's MMA warp issues products that read
+// both.  Per CTA and step that is 32 KB written to and 32 KB read from shared
+// memory under 512 clocks of products, where a CTA alone (128 x 256) would move
+// 96 KB and be bound by it.
 __device__ __forceinline__ void pair_tile(const Args& a, uint32_t t, uint32_t& m, uint32_t& n) {
     // bands of 8 row tiles, so that the tiles at work at one time share both
     // their columns of X and of dY in L2
@@ -665,14 +689,15 @@ __device__ __forceinline__ void pair_tile(const Args& a, uint32_t t, uint32_t& m
     m = band * 8 + (at - n * high);
 }
 
-template <class T, int KIND>
-__global__ void __launch_bounds__(kThreads, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap map, const Args a) {
+template <class T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
+                const Args a) {
     using S = Pair;
     constexpr int kStages = S::kStages;
     extern __shared__ uint8_t raw[];
     // full, acc_empty, drain: of the first CTA; the others of each
-    __shared__ uint64_t full[kStages], full_b[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
     __shared__ uint32_t tmem_at;
     __shared__ int gave_up_s;
     volatile int* gave_up = &gave_up_s;
@@ -692,19 +717,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         gave_up_s = 0;
         for (int s = 0; s < kStages; ++s) {
-            bar_init(smem_u32(full + s), 2 * kTeam);
-            bar_init(smem_u32(full_b + s), 1);
+            bar_init(smem_u32(full + s), 1);
             bar_init(smem_u32(empty + s), 1);
         }
         for (int b = 0; b < 2; ++b) {
             bar_init(smem_u32(acc_full + b), 1);
-            bar_init(smem_u32(acc_empty + b), 2 * kEpiWarps);
+            bar_init(smem_u32(acc_empty + b), 2 * kPairEpiWarps);
         }
         bar_init(smem_u32(&drain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == kMmaWarp) {
+    if (warp == kPairEpiWarps) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&tmem_at)),
                      "r"(2 * S::kBN)
@@ -717,69 +741,76 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after();
     const uint32_t tmem = tmem_at;
 
-    if (warp == kTmaWarp) {
-        if (lane == 0)
-            bring_steps<S::kBBytes, S::kStage, kStages>(
-                &map, w, stages, empty, full_b, gave_up, [&](uint32_t t) {
-                    uint32_t m, n;
-                    pair_tile(a, t, m, n);
-                    return n * S::kBN + rank * (S::kBN / 2);
-                });
-    } else if (warp == kMmaWarp) {
-        if (lane == 0 && rank == 0) {
-            const uint32_t shape = mma_shape<T>(2 * kBM, S::kBN);
+    if (warp == kPairEpiWarps + 1) {
+        const uint32_t me = elect();
+        uint32_t s = 0, phase = 0;
+        bool ok = true;
+        for (uint32_t t = w.first; ok && t < w.tiles; t += w.step) {
+            uint32_t m, n;
+            pair_tile(a, t, m, n);
+            const int m0 = (int)(m * 2 * kBM + rank * kBM);
+            const int n0 = (int)(n * S::kBN + rank * (S::kBN / 2));
+            for (uint32_t it = 0; it < a.iters; ++it) {
+                if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
+                const uint32_t dst = stages + s * S::kStage;
+                // both CTAs' copies complete on the first one's barrier
+                bar_expect(smem_u32(full + s), 2 * S::kStage, me & (rank ^ 1u));
+                const uint32_t bar = bar_of(smem_u32(full + s), 0);
+#pragma unroll
+                for (int j = 0; j < kABytes / kAtom; ++j)
+                    tma_load<true>(dst + j * kAtom, &map_x, m0 + 64 * j, (int)(it * kBK), bar, me);
+#pragma unroll
+                for (int j = 0; j < S::kBBytes / kAtom; ++j)
+                    tma_load<true>(dst + kABytes + j * kAtom, &map_dy, n0 + 64 * j, (int)(it * kBK),
+                                   bar, me);
+                if (++s == kStages) s = 0, phase ^= 1u;
+            }
+        }
+        if (!ok) settle();
+    } else if (warp == kPairEpiWarps) {
+        if (rank == 0) {
+            const uint32_t me = elect(), shape = mma_shape<T>(2 * kBM, S::kBN);
             uint32_t s = 0, phase = 0, buf = 0, bphase = 0;
             bool ok = true;
             for (uint32_t t = w.first; ok && t < w.tiles; t += w.step)
                 for (uint32_t c = 0; ok && c < w.chunks; ++c) {
-                    if (!(ok = bar_wait(smem_u32(acc_empty + buf), bphase ^ 1u, gave_up))) break;
+                    if (!(ok = warp_wait(smem_u32(acc_empty + buf), bphase ^ 1u, gave_up))) break;
                     fence_after();
                     const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
                     for (uint32_t it = from; it < to; ++it) {
-                        if (!(ok = bar_wait(smem_u32(full + s), phase, gave_up))) break;
+                        if (!(ok = warp_wait(smem_u32(full + s), phase, gave_up))) break;
                         fence_after();
-                        const uint32_t at = stages + s * S::kStage;
+                        const uint64_t x = operand(stages + s * S::kStage), y = x + kABytes / 16;
 #pragma unroll
-                        for (int k = 0; k < kBK / 16; ++k)
-                            mma_f16_pair(tmem + buf * S::kBN, operand(at + k * 2048),
-                                         operand(at + kABytes + k * 2048), shape, it > from || k > 0);
-                        mma_commit_pair(smem_u32(empty + s));
+                        for (int k = 0; k < kBK / 16; ++k)   // 16 tokens: two groups of 8
+                            mma_f16<true>(tmem + buf * S::kBN, x + k * (2048 / 16),
+                                          y + k * (2048 / 16), shape, it > from || k > 0, me);
+                        mma_commit<true>(smem_u32(empty + s), me);
                         if (++s == kStages) s = 0, phase ^= 1u;
                     }
                     if (!ok) break;
-                    mma_commit_pair(smem_u32(acc_full + buf));
+                    mma_commit<true>(smem_u32(acc_full + buf), me);
                     if (++buf == 2) buf = 0, bphase ^= 1u;
                 }
-            mma_commit_pair(smem_u32(&drain));
+            // no product is in flight when the accumulators are given back
+            mma_commit<true>(smem_u32(&drain), me);
             bar_drain(smem_u32(&drain), 0);
         }
-    } else if (warp >= kEpiWarps) {
-        fill_stages<T, KIND, S::kStage, kStages>(
-            a, w, stages, empty, gave_up,
-            [&](uint32_t t) {
-                uint32_t m, n;
-                pair_tile(a, t, m, n);
-                return (uint64_t)m * (2 * kBM) + rank * kBM;
-            },
-            [&](uint32_t s, uint32_t phase) {
-                // this CTA's part of dY has landed too: the products wait on one barrier
-                if (warp % kTeam == 0 && !bar_wait(smem_u32(full_b + s), phase, gave_up)) return false;
-                bar_arrive_at(bar_of(smem_u32(full + s), 0));
-                return true;
-            });
     } else {
+        // two warps to each quarter of the rows, half of the columns each
+        const uint32_t quarter = warp % 4, c0 = warp / 4 * (S::kBN / 2);
         uint32_t buf = 0, bphase = 0;
         for (uint32_t t = w.first; t < w.tiles; t += w.step)
             for (uint32_t k = 0; k < w.chunks; ++k) {
-                const bool ok = warp_wait(smem_u32(acc_full + buf), bphase, gave_up);
+                const bool ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up);
                 fence_after();
                 uint32_t m, n;
                 pair_tile(a, t, m, n);
-                const uint32_t row = m * (2 * kBM) + rank * kBM + warp * 32 + lane;
+                const uint32_t row = m * (2 * kBM) + rank * kBM + quarter * 32 + lane;
 #pragma unroll 1
-                for (int c = 0; c < S::kBN; c += 32) {
+                for (uint32_t c = c0; c < c0 + S::kBN / 2; c += 32) {
                     float v[32];
-                    tmem_ld32(tmem + buf * S::kBN + ((uint32_t)(warp * 32) << 16) + c,
+                    tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
                     if (!ok) {
 #pragma unroll
@@ -798,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     fence_before();
     cluster_sync();   // no product or barrier of the pair is used after this
-    if (warp == kMmaWarp) {
+    if (warp == kPairEpiWarps) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                      "r"(2 * S::kBN));
@@ -850,32 +881,25 @@ bool tma_rows(const void* p, uint64_t ld, uint64_t cols) {
 }
 uint64_t realigned(uint64_t cols) { return (cols + 7) / 8 * 8; }
 
-using Kernel = void (*)(const CUtensorMap, const Args);
-
-template <class T, int KIND>
-Kernel kernel_of(bool pair) {
-    return pair ? pair_kernel<T, KIND> : few_kernel<T, KIND>;
-}
-
-int launch(const CUtensorMap& map, const Args& a, int32_t type, int32_t kind, bool pair,
-           uint32_t cluster, uint32_t grid, cudaStream_t s) {
-    const int which = (type == ARK_TYPE_BF16) << 2 | (kind == kInt8) << 1 | (int)pair;
-    const Kernel k = type == ARK_TYPE_F16
-                         ? (kind == kE4M3 ? kernel_of<__half, kE4M3>(pair) : kernel_of<__half, kInt8>(pair))
-                         : (kind == kE4M3 ? kernel_of<__nv_bfloat16, kE4M3>(pair)
-                                          : kernel_of<__nv_bfloat16, kInt8>(pair));
-    const int smem = pair ? Pair::kSmem : Few::kSmem;
-    static std::atomic<uint64_t> ready[8];   // devices whose shared-memory limit is raised
+// raises a kernel's shared-memory limit, once per device
+int set_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ARK_E_CUDA;
-    if (dev >= 64 || !(ready[which].load() >> dev & 1)) {
-        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return ARK_E_CUDA;
-        if (dev < 64) ready[which].fetch_or(1ull << dev);
-    }
+    if (dev < 64 && (ready.load() >> dev & 1)) return ARK_OK;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        return ARK_E_CUDA;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+    return ARK_OK;
+}
+
+template <class... P, class... A>
+int launch(void (*k)(P...), uint32_t grid, uint32_t threads, int smem, uint32_t cluster,
+           std::atomic<uint64_t>& ready, cudaStream_t s, const A&... args) {
+    const int rc = set_smem(reinterpret_cast<const void*>(k), smem, ready);
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -884,7 +908,46 @@ int launch(const CUtensorMap& map, const Args& a, int32_t type, int32_t kind, bo
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, map, a) == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+    return cudaLaunchKernelEx(&cfg, k, args...) == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+}
+
+template <class T, int KIND>
+int launch_few(const CUtensorMap& map, const Args& a, uint32_t parts, cudaStream_t s) {
+    static std::atomic<uint64_t> ready{0};
+    return launch(few_kernel<T, KIND>, a.tiles * parts, kThreads, Few::kSmem, parts, ready, s, map, a);
+}
+template <class T>
+int launch_pair(const CUtensorMap& x, const CUtensorMap& dy, const Args& a, cudaStream_t s) {
+    static std::atomic<uint64_t> ready{0};
+    const uint32_t most = (uint32_t)sm_count() / 2, pairs = a.tiles < most ? a.tiles : most;
+    return launch(pair_kernel<T>, pairs * 2, kPairThreads, Pair::kSmem, 2, ready, s, x, dy, a);
+}
+
+// [rows, cols] of 16-bit elements, ld apart, in boxes of 64 columns by 64 rows
+int encode(CUtensorMap* map, int32_t type, const void* p, uint64_t rows, uint64_t cols, uint64_t ld) {
+    const EncodeFn f = encode_fn();
+    if (!f) return ARK_E_CUDA;
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
+    const cuuint32_t box[2] = {64, kBK}, ones[2] = {1, 1};
+    return f(map,
+             type == ARK_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+             2, const_cast<void*>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? ARK_OK
+               : ARK_E_CUDA;
+}
+
+// Pairs when their tiles fill three quarters of the SMs.
+bool use_pairs(uint64_t m, uint64_t n) {
+    return ((m + 255) / 256) * ((n + 255) / 256) * 2 >= (uint64_t)sm_count() * 3 / 4;
+}
+// bytes of the workspace's two parts: X in 16 bits, dY realigned
+uint64_t ws_x(const ark_act8* x, uint64_t n) {
+    return use_pairs(x->cols, n) ? x->rows * act8_pitch(x->cols) * 2 : 0;
+}
+uint64_t ws_dy(const ark_act8* x, const void* dy, uint64_t lddy, uint64_t n) {
+    return tma_rows(dy, lddy, n) ? 0 : x->rows * realigned(n) * 2;
 }
 
 }  // namespace
@@ -894,9 +957,9 @@ using namespace ark;
 
 extern "C" {
 
-uint64_t ark_cuda_weight_grad_workspace(uint64_t tokens, const void* dy, uint64_t lddy,
+uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
                                         uint64_t n_out) {
-    return tma_rows(dy, lddy, n_out) ? 0 : tokens * realigned(n_out) * 2;
+    return x ? ws_x(x, n_out) + ws_dy(x, dy, lddy, n_out) : 0;
 }
 
 int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
@@ -938,42 +1001,40 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
     }
 
-    uint64_t ld = lddy;
-    if (!tma_rows(dy, lddy, n_out)) {
-        ld = realigned(n_out);
-        if (!workspace || workspace_bytes < x->rows * ld * 2) return ARK_E_INVALID_ARG;
+    const uint64_t need_x = ws_x(x, n_out), need_dy = ws_dy(x, dy, lddy, n_out);
+    if (need_x + need_dy) {
+        if (!workspace || workspace_bytes < need_x + need_dy) return ARK_E_INVALID_ARG;
         if (!aligned16(workspace)) return ARK_E_MISALIGNED;
-        const uint64_t blocks = (x->rows * ld / 2 + 255) / 256;
-        const uint64_t most = (uint64_t)sm_count() * 8;
-        realign_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
-            static_cast<const uint16_t*>(dy), lddy, x->rows, a.n, static_cast<uint16_t*>(workspace),
-            (uint32_t)ld);
-        if (cudaGetLastError() != cudaSuccess) return ARK_E_CUDA;
-        dy = workspace;
     }
-    EncodeFn encode = encode_fn();
-    if (!encode) return ARK_E_CUDA;
+    uint64_t ld = lddy;
+    if (need_dy) {
+        ld = realigned(n_out);
+        uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + need_x);
+        const uint64_t blocks = (x->rows * ld / 2 + 255) / 256, most = (uint64_t)sm_count() * 8;
+        realign_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
+            static_cast<const uint16_t*>(dy), lddy, x->rows, a.n, to, (uint32_t)ld);
+        if (cudaGetLastError() != cudaSuccess) return ARK_E_CUDA;
+        dy = to;
+    }
     CUtensorMap map;
-    const cuuint64_t dims[2] = {n_out, x->rows}, strides[1] = {ld * 2};
-    const cuuint32_t box[2] = {64, kBK}, ones[2] = {1, 1};
-    if (encode(&map,
-               dy_type == ARK_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-               2, const_cast<void*>(dy), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return ARK_E_CUDA;
+    int e2 = encode(&map, dy_type, dy, x->rows, n_out, ld);
+    if (e2) return e2;
 
     const uint32_t sms = (uint32_t)sm_count();
-    const uint32_t pairs = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-    if (pairs * 2 >= sms * 3 / 4) {
+    if (need_x) {
         a.tiles_m = (a.m + 255) / 256;
         a.tiles_n = (a.n + 255) / 256;
-        a.tiles = pairs;
+        a.tiles = a.tiles_m * a.tiles_n;
         // the tensor cores' FP32 sums are cut off, not rounded: FP32 gradients of
         // more than 2048 tokens are summed in runs that the epilogue adds
         a.chunks = a.dw_f32 ? (a.iters + 31) / 32 : 1;
-        return launch(map, a, dy_type, x->kind, true, 2, 2 * (pairs < sms / 2 ? pairs : sms / 2), s);
+        e2 = ark_cuda_act8_unpack(x, workspace, dy_type, a.pitch, cuda_stream);
+        if (e2) return e2;
+        CUtensorMap map_x;
+        e2 = encode(&map_x, dy_type, workspace, x->rows, x->cols, a.pitch);
+        if (e2) return e2;
+        return dy_type == ARK_TYPE_F16 ? launch_pair<__half>(map_x, map, a, s)
+                                       : launch_pair<__nv_bfloat16>(map_x, map, a, s);
     }
     a.tiles_m = (a.m + kBM - 1) / kBM;
     a.tiles_n = (a.n + Few::kBN - 1) / Few::kBN;
@@ -982,7 +1043,11 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     while (parts < 8 && a.tiles * parts * 2 <= sms && parts * 2 <= a.iters) parts *= 2;
     a.chunks = a.iters / parts / 16;
     a.chunks = a.chunks < 1 ? 1 : a.chunks > 4 ? 4 : a.chunks;
-    return launch(map, a, dy_type, x->kind, false, parts, a.tiles * parts, s);
+    if (dy_type == ARK_TYPE_F16)
+        return x->kind == kE4M3 ? launch_few<__half, kE4M3>(map, a, parts, s)
+                                : launch_few<__half, kInt8>(map, a, parts, s);
+    return x->kind == kE4M3 ? launch_few<__nv_bfloat16, kE4M3>(map, a, parts, s)
+                            : launch_few<__nv_bfloat16, kInt8>(map, a, parts, s);
 }
 
 }  // extern "C"
