@@ -38,7 +38,7 @@ constexpr int kBM = 128, kBK = 64;
 constexpr int kEpiWarps = 4, kTeam = 4, kTeams = 2, kCvtWarps = kTeam * kTeams;
 constexpr int kThreads = (kEpiWarps + kCvtWarps + 2) * 32;
 constexpr int kTmaWarp = kEpiWarps + kCvtWarps, kMmaWarp = kTmaWarp + 1;
-constexpr int kPairEpiWarps = 8, kPairThreads = (kPairEpiWarps + 2) * 32;
+constexpr int kPairEpiWarps = 16, kPairThreads = (kPairEpiWarps + 2) * 32;
 constexpr int kAtom = kBK * 128;              // 64 tokens x 64 columns of 16 bits
 constexpr int kABytes = kBM / 64 * kAtom;
 constexpr int kAhead = 2;                     // steps of a team in flight
@@ -56,6 +56,12 @@ struct Pair {     // two CTAs: 256 x 256, of which each brings 128 columns of dY
     static constexpr int kStages = 6, kSmem = kStages * kStage + 1024;
 };
 
+struct Out {
+    void* p;
+    uint64_t ld;
+    int f32, bf16, vec;   // vec: rows of whole 16-byte vectors
+};
+
 struct Args {
     const uint8_t* x;
     const uint8_t* scale;
@@ -64,9 +70,11 @@ struct Args {
     uint32_t iters;           // 64-token steps in all
     uint32_t tiles_m, tiles_n, tiles;
     uint32_t chunks;          // runs of steps whose sums are added by the epilogue
-    void* dw;
-    uint64_t ldw;
-    int dw_f32, dw_bf16, accumulate, vec;
+    uint32_t splits;          // pair_kernel: runs of tokens that are tiles of their own,
+    float* partial;           // and where their sums go, [splits][m][n_pad]
+    uint32_t n_pad;
+    Out out;
+    int accumulate;
 };
 
 // ------------------------------------------------------------ PTX
@@ -244,6 +252,10 @@ __device__ __forceinline__ void fence_before() {
 __device__ __forceinline__ void fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
+// everything before this grid in the stream is done and visible
+__device__ __forceinline__ void wait_before() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
@@ -368,76 +380,61 @@ __device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uin
 }
 
 // ------------------------------------------------------------ output
-__device__ __forceinline__ float dw_get(const Args& a, uint64_t i) {
-    if (a.dw_f32) return static_cast<const float*>(a.dw)[i];
-    if (a.dw_bf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.dw)[i]);
-    return __half2float(static_cast<const __half*>(a.dw)[i]);
+__device__ __forceinline__ float out_get(const Out& o, uint64_t i) {
+    if (o.f32) return static_cast<const float*>(o.p)[i];
+    if (o.bf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(o.p)[i]);
+    return __half2float(static_cast<const __half*>(o.p)[i]);
 }
-__device__ __forceinline__ void dw_put(const Args& a, uint64_t i, float v) {
-    if (a.dw_f32)
-        static_cast<float*>(a.dw)[i] = v;
-    else if (a.dw_bf16)
-        static_cast<__nv_bfloat16*>(a.dw)[i] = __float2bfloat16_rn(v);
+__device__ __forceinline__ void out_put(const Out& o, uint64_t i, float v) {
+    if (o.f32)
+        static_cast<float*>(o.p)[i] = v;
+    else if (o.bf16)
+        static_cast<__nv_bfloat16*>(o.p)[i] = __float2bfloat16_rn(v);
     else
-        static_cast<__half*>(a.dw)[i] = __float2half_rn(v);
+        static_cast<__half*>(o.p)[i] = __float2half_rn(v);
 }
-// N (4 or 8) sums of one row, rounded once to the gradient's type
-template <int N>
-__device__ __forceinline__ void dw_row(const Args& a, uint32_t row, uint32_t col, float* v,
-                                       bool accumulate) {
-    if (row >= a.m || col >= a.n) return;
-    const uint64_t i = (uint64_t)row * a.ldw + col;
-    if (a.vec && col + N <= a.n) {
+template <int N, class T>
+__device__ __forceinline__ void out_vec(T* p, float* v, bool accumulate) {
+    if (accumulate) {
         float old[N];
-        if (a.dw_f32) {
-            float* p = static_cast<float*>(a.dw) + i;
-            if (accumulate) {
-                load_vec<N>(p, old);
+        load_vec<N>(p, old);
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
-            }
-            store_vec<N>(p, v);
-        } else if (a.dw_bf16) {
-            __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.dw) + i;
-            if (accumulate) {
-                load_vec<N>(p, old);
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
-            }
-            store_vec<N>(p, v);
-        } else {
-            __half* p = static_cast<__half*>(a.dw) + i;
-            if (accumulate) {
-                load_vec<N>(p, old);
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
-            }
-            store_vec<N>(p, v);
-        }
+        for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
+    }
+    store_vec<N>(p, v);
+}
+// N (4 or 8) sums of one row of an m x n output, rounded once to its type
+template <int N>
+__device__ __forceinline__ void out_row(const Out& o, uint32_t m, uint32_t n, uint32_t row,
+                                        uint32_t col, float* v, bool accumulate) {
+    if (row >= m || col >= n) return;
+    const uint64_t i = (uint64_t)row * o.ld + col;
+    if (o.vec && col + N <= n) {
+        if (o.f32)
+            out_vec<N>(static_cast<float*>(o.p) + i, v, accumulate);
+        else if (o.bf16)
+            out_vec<N>(static_cast<__nv_bfloat16*>(o.p) + i, v, accumulate);
+        else
+            out_vec<N>(static_cast<__half*>(o.p) + i, v, accumulate);
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (col + j < a.n)
-                dw_put(a, i + j, accumulate ? __fadd_rn(v[j], dw_get(a, i + j)) : v[j]);
+            if (col + j < n) out_put(o, i + j, accumulate ? __fadd_rn(v[j], out_get(o, i + j)) : v[j]);
     }
 }
 
 // ------------------------------------------------------------ bytes to a stage
-// Which steps of which tiles a CTA works through, in order.
-struct Work {
-    uint32_t first, step, tiles;      // tiles first, first + step, ... below tiles
-    uint32_t it0, it1, chunks;        // its steps of each, in `chunks` runs
-    __device__ __forceinline__ uint32_t chunk_at(uint32_t c) const {
-        return it0 + (uint32_t)((uint64_t)(it1 - it0) * c / chunks);
-    }
-};
+// where part p of n equal ones begins
+__device__ __forceinline__ uint32_t part_of(uint32_t total, uint32_t p, uint32_t n) {
+    return (uint32_t)((uint64_t)total * p / n);
+}
 
 // Teams of 4 warps take steps in turn, so that one's waits, fences and
 // instruction latency run under the other's conversions.  A thread turns 16
 // bytes (half a scale block) of each of four token rows.
 //   col: first column of x of this CTA's tile
 template <class T, int KIND, int STAGE, int STAGES>
-__device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32_t col,
+__device__ __forceinline__ void fill_stages(const Args& a, uint32_t it0, uint32_t it1, uint32_t col,
                                             uint32_t stages, const uint64_t* empty,
                                             const uint64_t* full, volatile int* gave_up) {
     static_assert(STAGES >= kTeams, "a team has a stage of its own");
@@ -450,8 +447,8 @@ __device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32
     uint32_t sc[kAhead][4];
     // this thread's first row of the step that is loaded next, and where the
     // part's rows end
-    uint32_t tok = (w.it0 + team) * kBK + row;
-    const uint32_t end = min(a.tokens, w.it1 * kBK);
+    uint32_t tok = (it0 + team) * kBK + row;
+    const uint32_t end = min(a.tokens, it1 * kBK);
     const uint8_t* xp = a.x + tok * a.pitch + col + unit * 16;
     const uint8_t* sp = a.scale + tok * a.spitch + (col >> 5) + (unit >> 1);
     const uint64_t next_x = kTeams * kBK * a.pitch, next_s = kTeams * kBK * a.spitch;
@@ -471,7 +468,7 @@ __device__ __forceinline__ void fill_stages(const Args& a, const Work& w, uint32
     };
 #pragma unroll
     for (int p = 0; p < kAhead; ++p) load(p);
-    uint32_t todo = (w.it1 - w.it0 + kTeams - 1 - team) / kTeams;
+    uint32_t todo = (it1 - it0 + kTeams - 1 - team) / kTeams;
     uint32_t s = team, phase = 0;
     bool ok = true;
     while (ok && todo) {
@@ -547,13 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t parts, part;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(part));
-    Work w;
-    w.first = blockIdx.x / parts;
-    w.step = w.tiles = a.tiles;
-    w.it0 = (uint32_t)((uint64_t)a.iters * part / parts);
-    w.it1 = (uint32_t)((uint64_t)a.iters * (part + 1) / parts);
-    w.chunks = a.chunks;
-    const uint32_t m0 = w.first / a.tiles_n * kBM, n0 = w.first % a.tiles_n * S::kBN;
+    const uint32_t it0 = part_of(a.iters, part, parts), it1 = part_of(a.iters, part + 1, parts);
+    const uint32_t tile = blockIdx.x / parts;
+    const uint32_t m0 = tile / a.tiles_n * kBM, n0 = tile % a.tiles_n * S::kBN;
 
     if (threadIdx.x == 0) {
         gave_up_s = 0;
@@ -577,12 +570,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_at;
+    wait_before();
 
     if (warp == kTmaWarp) {
         const uint32_t me = elect();
         uint32_t s = 0, phase = 0;
         bool ok = true;
-        for (uint32_t it = w.it0; it < w.it1; ++it) {
+        for (uint32_t it = it0; it < it1; ++it) {
             if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
             const uint32_t dst = stages + s * S::kStage + kABytes, bar = smem_u32(full + s);
             bar_expect(bar, S::kBBytes, me);
@@ -596,8 +590,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t me = elect(), shape = mma_shape<T>(kBM, S::kBN);
         uint32_t s = 0, phase = 0;
         bool ok = true;
-        for (uint32_t c = 0; ok && c < w.chunks; ++c) {
-            const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
+        for (uint32_t c = 0; ok && c < a.chunks; ++c) {
+            const uint32_t from = it0 + part_of(it1 - it0, c, a.chunks);
+            const uint32_t to = it0 + part_of(it1 - it0, c + 1, a.chunks);
             for (uint32_t it = from; it < to; ++it) {
                 if (!(ok = warp_wait(smem_u32(full + s), phase, gave_up))) break;
                 fence_after();
@@ -615,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit<false>(smem_u32(&drain), me);
         bar_drain(smem_u32(&drain), 0);
     } else if (warp >= kEpiWarps) {
-        fill_stages<T, KIND, S::kStage, kStages>(a, w, m0, stages, empty, full, gave_up);
+        fill_stages<T, KIND, S::kStage, kStages>(a, it0, it1, m0, stages, empty, full, gave_up);
     } else {
         const bool ok = warp_wait<kSleep>(smem_u32(&acc_full), 0, gave_up);
         fence_after();
@@ -625,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float v[32];
             const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + c;
             tmem_ld32(from, reinterpret_cast<uint32_t*>(v));
-            for (uint32_t k = 1; k < w.chunks; ++k) {
+            for (uint32_t k = 1; k < a.chunks; ++k) {
                 float more[32];
                 tmem_ld32(from + k * S::kBN, reinterpret_cast<uint32_t*>(more));
 #pragma unroll
@@ -664,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             v[3] = __fadd_rn(v[3], q.w);
         }
         if (lost) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
-        dw_row<4>(a, m0 + row, n0 + col, v, a.accumulate);
+        out_row<4>(a.out, a.m, a.n, m0 + row, n0 + col, v, a.accumulate);
     }
     cluster_sync();   // nobody leaves while its tile is read
     if (warp == kMmaWarp) {
@@ -706,13 +701,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t rank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    Work w;
-    w.first = blockIdx.x / 2;
-    w.step = gridDim.x / 2;
-    w.tiles = a.tiles;
-    w.it0 = 0;
-    w.it1 = a.iters;
-    w.chunks = a.chunks;
+    // Items: a tile and a run of the tokens; one run's tiles follow each other, so
+    // that the items at work share their rows of X and dY.
+    const uint32_t items = a.tiles * a.splits, pairs = gridDim.x / 2;
+    auto item = [&](uint32_t i, uint32_t& m, uint32_t& n, uint32_t& it0, uint32_t& it1) {
+        const uint32_t run = i / a.tiles;
+        pair_tile(a, i - run * a.tiles, m, n);
+        it0 = part_of(a.iters, run, a.splits);
+        it1 = part_of(a.iters, run + 1, a.splits);
+        return run;
+    };
 
     if (threadIdx.x == 0) {
         gave_up_s = 0;
@@ -740,17 +738,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     cluster_sync();   // both CTAs' barriers are there before either is used
     fence_after();
     const uint32_t tmem = tmem_at;
+    wait_before();
 
     if (warp == kPairEpiWarps + 1) {
         const uint32_t me = elect();
         uint32_t s = 0, phase = 0;
         bool ok = true;
-        for (uint32_t t = w.first; ok && t < w.tiles; t += w.step) {
-            uint32_t m, n;
-            pair_tile(a, t, m, n);
+        for (uint32_t i = blockIdx.x / 2; ok && i < items; i += pairs) {
+            uint32_t m, n, it0, it1;
+            item(i, m, n, it0, it1);
             const int m0 = (int)(m * 2 * kBM + rank * kBM);
             const int n0 = (int)(n * S::kBN + rank * (S::kBN / 2));
-            for (uint32_t it = 0; it < a.iters; ++it) {
+            for (uint32_t it = it0; it < it1; ++it) {
                 if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
                 const uint32_t dst = stages + s * S::kStage;
                 // both CTAs' copies complete on the first one's barrier
@@ -772,11 +771,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t me = elect(), shape = mma_shape<T>(2 * kBM, S::kBN);
             uint32_t s = 0, phase = 0, buf = 0, bphase = 0;
             bool ok = true;
-            for (uint32_t t = w.first; ok && t < w.tiles; t += w.step)
-                for (uint32_t c = 0; ok && c < w.chunks; ++c) {
+            for (uint32_t i = blockIdx.x / 2; ok && i < items; i += pairs) {
+                uint32_t m, n, it0, it1;
+                item(i, m, n, it0, it1);
+                for (uint32_t c = 0; ok && c < a.chunks; ++c) {
                     if (!(ok = warp_wait(smem_u32(acc_empty + buf), bphase ^ 1u, gave_up))) break;
                     fence_after();
-                    const uint32_t from = w.chunk_at(c), to = w.chunk_at(c + 1);
+                    const uint32_t from = it0 + part_of(it1 - it0, c, a.chunks);
+                    const uint32_t to = it0 + part_of(it1 - it0, c + 1, a.chunks);
                     for (uint32_t it = from; it < to; ++it) {
                         if (!(ok = warp_wait(smem_u32(full + s), phase, gave_up))) break;
                         fence_after();
@@ -792,39 +794,73 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     mma_commit<true>(smem_u32(acc_full + buf), me);
                     if (++buf == 2) buf = 0, bphase ^= 1u;
                 }
+            }
             // no product is in flight when the accumulators are given back
             mma_commit<true>(smem_u32(&drain), me);
             bar_drain(smem_u32(&drain), 0);
         }
     } else {
-        // two warps to each quarter of the rows, half of the columns each
-        const uint32_t quarter = warp % 4, c0 = warp / 4 * (S::kBN / 2);
+        // four warps to each quarter of the rows, a quarter of the columns each
+        constexpr int kCols = S::kBN * 4 / kPairEpiWarps;
+        const uint32_t quarter = warp % 4, c0 = warp / 4 * kCols;
         uint32_t buf = 0, bphase = 0;
-        for (uint32_t t = w.first; t < w.tiles; t += w.step)
-            for (uint32_t k = 0; k < w.chunks; ++k) {
-                const bool ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up);
-                fence_after();
-                uint32_t m, n;
-                pair_tile(a, t, m, n);
-                const uint32_t row = m * (2 * kBM) + rank * kBM + quarter * 32 + lane;
-#pragma unroll 1
-                for (uint32_t c = c0; c < c0 + S::kBN / 2; c += 32) {
-                    float v[32];
-                    tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
-                              reinterpret_cast<uint32_t*>(v));
-                    if (!ok) {
+        for (uint32_t i = blockIdx.x / 2; i < items; i += pairs) {
+            uint32_t m, n, it0, it1;
+            const uint32_t run = item(i, m, n, it0, it1);
+            const uint32_t row = m * (2 * kBM) + rank * kBM + quarter * 32 + lane;
+            Out out = a.out;
+            bool accumulate = a.accumulate;
+            if (a.splits > 1) {
+                out = Out{a.partial + (uint64_t)run * a.m * a.n_pad, a.n_pad, 1, 0, 1};
+                accumulate = false;
+            }
+            auto put = [&](uint32_t c, float* v, bool ok) {
+                if (!ok) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        dw_row<8>(a, row, n * S::kBN + c + j, v + j, a.accumulate || k > 0);
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
                 }
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                    out_row<8>(out, a.m, a.n, row, n * S::kBN + c + j, v + j, accumulate);
+            };
+            auto next = [&] {
                 fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive_at(bar_of(smem_u32(acc_empty + buf), 0));
                 if (++buf == 2) buf = 0, bphase ^= 1u;
+            };
+            if (a.chunks == 1) {
+                const bool ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up);
+                fence_after();
+#pragma unroll 1
+                for (uint32_t c = c0; c < c0 + kCols; c += 32) {
+                    float v[32];
+                    tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
+                              reinterpret_cast<uint32_t*>(v));
+                    put(c, v, ok);
+                }
+                next();
+            } else {
+                // the runs' sums are added in registers
+                float sum[kCols / 32][32];
+                bool ok = true;
+                for (uint32_t k = 0; k < a.chunks; ++k) {
+                    ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up) && ok;
+                    fence_after();
+#pragma unroll
+                    for (int c = 0; c < kCols / 32; ++c) {
+                        float v[32];
+                        tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c0 + c * 32,
+                                  reinterpret_cast<uint32_t*>(v));
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[c][j] = k ? __fadd_rn(sum[c][j], v[j]) : v[j];
+                    }
+                    next();
+                }
+#pragma unroll
+                for (int c = 0; c < kCols / 32; ++c) put(c0 + c * 32, sum[c], ok);
             }
+        }
     }
     __syncwarp();
     fence_before();
@@ -853,12 +889,33 @@ __global__ void __launch_bounds__(256) realign_kernel(const uint16_t* __restrict
     }
 }
 
+// the runs' partial sums, added in order: four columns per thread
+__global__ void __launch_bounds__(256) runs_kernel(const Args a) {
+    wait_before();
+    const uint32_t per = a.n_pad / 4;
+    const uint64_t total = (uint64_t)a.m * per, run = (uint64_t)a.m * a.n_pad;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (uint64_t)gridDim.x * 256) {
+        const uint32_t row = (uint32_t)(i / per), col = (uint32_t)(i - (uint64_t)row * per) * 4;
+        const float* p = a.partial + (uint64_t)row * a.n_pad + col;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t k = 0; k < a.splits; ++k) {
+            const float4 q = __ldcs(reinterpret_cast<const float4*>(p + k * run));
+            v[0] = __fadd_rn(v[0], q.x);
+            v[1] = __fadd_rn(v[1], q.y);
+            v[2] = __fadd_rn(v[2], q.z);
+            v[3] = __fadd_rn(v[3], q.w);
+        }
+        out_row<4>(a.out, a.m, a.n, row, col, v, a.accumulate);
+    }
+}
+
 // dW of no tokens
 __global__ void __launch_bounds__(256) zero_kernel(const Args a) {
     const uint64_t total = (uint64_t)a.m * a.n;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total;
          i += (uint64_t)gridDim.x * 256)
-        dw_put(a, i / a.n * a.ldw + i % a.n, 0.0f);
+        out_put(a.out, i / a.n * a.out.ld + i % a.n, 0.0f);
 }
 
 using EncodeFn = decltype(&cuTensorMapEncodeTiled);
@@ -883,6 +940,7 @@ uint64_t realigned(uint64_t cols) { return (cols + 7) / 8 * 8; }
 
 // raises a kernel's shared-memory limit, once per device
 int set_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+    if (bytes <= 48 * 1024) return ARK_OK;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ARK_E_CUDA;
     if (dev < 64 && (ready.load() >> dev & 1)) return ARK_OK;
@@ -902,12 +960,15 @@ int launch(void (*k)(P...), uint32_t grid, uint32_t threads, int smem, uint32_t 
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    // blocks may start while the kernel before ends; they wait for its results
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, k, args...) == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
@@ -919,7 +980,8 @@ int launch_few(const CUtensorMap& map, const Args& a, uint32_t parts, cudaStream
 template <class T>
 int launch_pair(const CUtensorMap& x, const CUtensorMap& dy, const Args& a, cudaStream_t s) {
     static std::atomic<uint64_t> ready{0};
-    const uint32_t most = (uint32_t)sm_count() / 2, pairs = a.tiles < most ? a.tiles : most;
+    const uint32_t most = (uint32_t)sm_count() / 2, items = a.tiles * a.splits;
+    const uint32_t pairs = items < most ? items : most;
     return launch(pair_kernel<T>, pairs * 2, kPairThreads, Pair::kSmem, 2, ready, s, x, dy, a);
 }
 
@@ -938,16 +1000,77 @@ int encode(CUtensorMap* map, int32_t type, const void* p, uint64_t rows, uint64_
                : ARK_E_CUDA;
 }
 
-// Pairs when their tiles fill three quarters of the SMs.
-bool use_pairs(uint64_t m, uint64_t n) {
-    return ((m + 255) / 256) * ((n + 255) / 256) * 2 >= (uint64_t)sm_count() * 3 / 4;
+// Clusters of `parts` CTAs of few_kernel that the device holds at once (a GPC's
+// SMs do not divide evenly), looked up once per device.
+uint32_t few_fit(uint32_t parts) {
+    static std::atomic<uint32_t> known[64][4];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int at = parts == 1 ? 0 : parts == 2 ? 1 : parts == 4 ? 2 : 3;
+    if (dev >= 0 && dev < 64)
+        if (const uint32_t n = known[dev][at].load()) return n;
+    auto k = few_kernel<__half, kE4M3>;
+    cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Few::kSmem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(parts);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Few::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = sm_count() / (int)parts / 2 + 1;
+    }
+    if (dev >= 0 && dev < 64) known[dev][at].store((uint32_t)n);
+    return (uint32_t)n;
 }
-// bytes of the workspace's two parts: X in 16 bits, dY realigned
-uint64_t ws_x(const ark_act8* x, uint64_t n) {
-    return use_pairs(x->cols, n) ? x->rows * act8_pitch(x->cols) * 2 : 0;
+
+// How a gradient is computed, by what each way was measured to take (ns):
+//   few_kernel   every wave of CTAs 6500 + 370 for each 64 tokens;
+//   pair_kernel  unpack 3000 + its bytes at 5 TB/s; every wave 1500 + 330 for
+//                each 64 tokens, 5000 once; split tokens: 3000 + the FP32
+//                partial sums written and read at 8 TB/s.
+// 512 tokens, 768 x 768: 8.5 us in 72 CTAs of clusters of 2, 13.8 in clusters of
+// 4 (144 CTAs, which do not all fit); 8192 tokens: few 30.7, pairs in 8 runs
+// 24.3; 8192, 4096 x 4096: pairs 210, few above 600.
+struct Way {
+    bool pairs;
+    uint32_t parts;    // few: CTAs of a cluster
+    uint32_t splits;   // pairs: runs of tokens
+    uint64_t x_bytes, partial_bytes;
+};
+Way way_of(uint64_t tokens, uint64_t m, uint64_t n) {
+    const uint64_t iters = (tokens + kBK - 1) / kBK, sms = (uint64_t)sm_count();
+    const uint64_t few = (m + 127) / 128 * ((n + 127) / 128);
+    const uint64_t tiles = (m + 255) / 256 * ((n + 255) / 256);
+    auto ceil_div = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
+    Way w = {false, 1, 1, 0, 0};
+    uint64_t best = ~0ull;
+    for (uint32_t p = 1; p <= 8 && p <= iters; p *= 2) {
+        const uint64_t t = ceil_div(few, few_fit(p)) * (6500 + 370 * ceil_div(iters, p));
+        if (t < best) best = t, w.parts = p;
+    }
+    const uint64_t x_bytes = tokens * act8_pitch(m) * 2, run = m * ((n + 3) / 4 * 4) * 4;
+    for (uint32_t r = 1; r <= 16 && (r == 1 || r * 8 <= iters); ++r) {
+        const uint64_t waves = ceil_div(tiles * r, sms / 2);
+        const uint64_t t = 8000 + x_bytes * 3 / 2 / 5000 + waves * (1500 + 330 * ceil_div(iters, r)) +
+                           (r > 1 ? 3000 + 2 * r * run / 8000 : 0);
+        if (t < best) best = t, w.pairs = true, w.splits = r;
+    }
+    if (w.pairs) {
+        w.x_bytes = x_bytes;
+        w.partial_bytes = w.splits > 1 ? w.splits * run : 0;
+    }
+    return w;
 }
-uint64_t ws_dy(const ark_act8* x, const void* dy, uint64_t lddy, uint64_t n) {
-    return tma_rows(dy, lddy, n) ? 0 : x->rows * realigned(n) * 2;
+// the workspace's last part: dY realigned
+uint64_t ws_dy(uint64_t tokens, const void* dy, uint64_t lddy, uint64_t n) {
+    return tma_rows(dy, lddy, n) ? 0 : tokens * realigned(n) * 2;
 }
 
 }  // namespace
@@ -959,7 +1082,9 @@ extern "C" {
 
 uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
                                         uint64_t n_out) {
-    return x ? ws_x(x, n_out) + ws_dy(x, dy, lddy, n_out) : 0;
+    if (!x || !x->rows || !x->cols || !n_out) return 0;
+    const Way w = way_of(x->rows, x->cols, n_out);
+    return w.x_bytes + w.partial_bytes + ws_dy(x->rows, dy, lddy, n_out);
 }
 
 int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
@@ -988,12 +1113,9 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     a.m = (uint32_t)x->cols;
     a.n = (uint32_t)n_out;
     a.iters = (a.tokens + kBK - 1) / kBK;
-    a.dw = dw;
-    a.ldw = lddw;
-    a.dw_f32 = dw_type == ARK_TYPE_F32;
-    a.dw_bf16 = dw_type == ARK_TYPE_BF16;
+    a.out = Out{dw, lddw, dw_type == ARK_TYPE_F32, dw_type == ARK_TYPE_BF16,
+                aligned16(dw) && lddw * e % 16 == 0};
     a.accumulate = accumulate != 0;
-    a.vec = aligned16(dw) && lddw * e % 16 == 0;
     if (x->rows == 0) {
         if (accumulate) return ARK_OK;
         const uint64_t blocks = ((uint64_t)a.m * a.n + 255) / 256;
@@ -1001,15 +1123,18 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
     }
 
-    const uint64_t need_x = ws_x(x, n_out), need_dy = ws_dy(x, dy, lddy, n_out);
-    if (need_x + need_dy) {
-        if (!workspace || workspace_bytes < need_x + need_dy) return ARK_E_INVALID_ARG;
+    const Way w = way_of(x->rows, x->cols, n_out);
+    const uint64_t need_dy = ws_dy(x->rows, dy, lddy, n_out);
+    const uint64_t need = w.x_bytes + w.partial_bytes + need_dy;
+    if (need) {
+        if (!workspace || workspace_bytes < need) return ARK_E_INVALID_ARG;
         if (!aligned16(workspace)) return ARK_E_MISALIGNED;
     }
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint64_t ld = lddy;
     if (need_dy) {
         ld = realigned(n_out);
-        uint16_t* to = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + need_x);
+        uint16_t* to = reinterpret_cast<uint16_t*>(ws + w.x_bytes + w.partial_bytes);
         const uint64_t blocks = (x->rows * ld / 2 + 255) / 256, most = (uint64_t)sm_count() * 8;
         realign_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
             static_cast<const uint16_t*>(dy), lddy, x->rows, a.n, to, (uint32_t)ld);
@@ -1020,27 +1145,33 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     int e2 = encode(&map, dy_type, dy, x->rows, n_out, ld);
     if (e2) return e2;
 
-    const uint32_t sms = (uint32_t)sm_count();
-    if (need_x) {
+    if (w.pairs) {
         a.tiles_m = (a.m + 255) / 256;
         a.tiles_n = (a.n + 255) / 256;
         a.tiles = a.tiles_m * a.tiles_n;
+        a.splits = w.splits;
+        a.partial = reinterpret_cast<float*>(ws + w.x_bytes);
+        a.n_pad = (a.n + 3) / 4 * 4;
         // the tensor cores' FP32 sums are cut off, not rounded: FP32 gradients of
         // more than 2048 tokens are summed in runs that the epilogue adds
-        a.chunks = a.dw_f32 ? (a.iters + 31) / 32 : 1;
-        e2 = ark_cuda_act8_unpack(x, workspace, dy_type, a.pitch, cuda_stream);
+        const uint32_t run = (a.iters + a.splits - 1) / a.splits;
+        a.chunks = a.out.f32 ? (run + 31) / 32 : 1;
+        e2 = ark_cuda_act8_unpack(x, ws, dy_type, a.pitch, cuda_stream);
         if (e2) return e2;
         CUtensorMap map_x;
-        e2 = encode(&map_x, dy_type, workspace, x->rows, x->cols, a.pitch);
+        e2 = encode(&map_x, dy_type, ws, x->rows, x->cols, a.pitch);
         if (e2) return e2;
-        return dy_type == ARK_TYPE_F16 ? launch_pair<__half>(map_x, map, a, s)
-                                       : launch_pair<__nv_bfloat16>(map_x, map, a, s);
+        e2 = dy_type == ARK_TYPE_F16 ? launch_pair<__half>(map_x, map, a, s)
+                                     : launch_pair<__nv_bfloat16>(map_x, map, a, s);
+        if (e2 || a.splits == 1) return e2;
+        const uint64_t blocks = ((uint64_t)a.m * a.n_pad / 4 + 255) / 256, most = (uint64_t)sm_count() * 8;
+        static std::atomic<uint64_t> ready{0};
+        return launch(runs_kernel, (uint32_t)(blocks < most ? blocks : most), 256, 0, 1, ready, s, a);
     }
     a.tiles_m = (a.m + kBM - 1) / kBM;
     a.tiles_n = (a.n + Few::kBN - 1) / Few::kBN;
     a.tiles = a.tiles_m * a.tiles_n;
-    uint32_t parts = 1;
-    while (parts < 8 && a.tiles * parts * 2 <= sms && parts * 2 <= a.iters) parts *= 2;
+    const uint32_t parts = w.parts;
     a.chunks = a.iters / parts / 16;
     a.chunks = a.chunks < 1 ? 1 : a.chunks > 4 ? 4 : a.chunks;
     if (dy_type == ARK_TYPE_F16)
