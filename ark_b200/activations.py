@@ -241,7 +241,8 @@ def weight_grad(x, dy, out=None, accumulate=False, dtype=None):
             if dtype is not None and out.dtype != dtype:
                 raise ValueError(f"out: expected {dtype}, got {out.dtype}")
             po, ldo = _rows(out, "out", x.cols, n, written=True)
-        need = _lib.lib().ark_cuda_weight_grad_workspace(hx, p, ld, n)
+        need = _lib.lib().ark_cuda_weight_grad_workspace(hx, p, ld, n, po, TYPES[out.dtype],
+                                                                  ldo)
         ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
         _call("ark_cuda_weight_grad", hx, p, TYPES[dy.dtype], ld, n, po, TYPES[out.dtype], ldo,
               1 if accumulate else 0, ws.data_ptr() if need else None, need, s)

@@ -3,11 +3,16 @@
 // and written once and a column block's scale is formed in registers, so HBM
 // bounds them.
 //
-// One thread holds 8 consecutive columns (16 bytes of a 16-bit type), so 4
-// neighbouring lanes hold the 32 columns of a scale block and two shuffles
-// give its largest magnitude.  A row has pitch/8 such chunks, a multiple of
-// 16, so a scale block never straddles two warps; the padded columns are
-// chunks like the others that read as zero.
+// One thread holds 16 consecutive columns, so 2 neighbouring lanes hold the 32
+// columns of a scale block and one shuffle gives its largest magnitude.  A row
+// has pitch/16 such chunks, a multiple of 8, so a scale block never straddles
+// two warps; the padded columns are chunks like the others that read as zero.
+// The instructions per element bound these kernels before HBM does, so the
+// 16-bit types keep to pairs: the largest magnitude by integer maxima of two,
+// and FP16 is scaled and rounded to 8 bits as FP16 pairs where the block's scale
+// is an FP16 number.
+#include <type_traits>
+
 #include "ark_act8.cuh"
 
 namespace ark {
@@ -26,7 +31,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Chunk (row, column) of a thread in a grid-stride walk over rows * per_row
+// Place (row, chunk) of a thread in a grid-stride walk over rows * per_row
 // chunks: one division at the start, none in the loop.
 struct Walk {
     uint64_t row, drow;
@@ -47,41 +52,284 @@ struct Walk {
     }
 };
 
-// the largest magnitude of the block that 4 neighbouring lanes hold
-__device__ __forceinline__ uint32_t block_max(uint32_t m) {
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    return max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-}
-
-// one thread's 8 columns of a checkpoint
-template <int KIND>
-__device__ __forceinline__ void put(uint8_t* data, uint8_t* scale, uint64_t chunk, const float* v,
-                                    uint32_t byte) {
-    *reinterpret_cast<uint2*>(data + chunk * 8) = quant8<KIND>(v, byte);
-    if ((threadIdx.x & 3) == 0) scale[chunk >> 2] = (uint8_t)byte;
-}
-
+// columns of a row from col on, as far as a thread asks (32)
 __device__ __forceinline__ int left(uint32_t cols, uint32_t col) {
-    return col < cols ? (int)min(cols - col, 8u) : 0;
+    return col < cols ? (int)min(cols - col, 32u) : 0;
+}
+
+// ------------------------------------------------------------ words of a thread
+__device__ __forceinline__ void load32(const void* p, uint32_t* w) {   // 32-byte aligned
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                   "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ void load16(const void* p, uint32_t* w) {
+    const uint4 q = *static_cast<const uint4*>(p);
+    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+}
+__device__ __forceinline__ void store16(void* p, const uint32_t* w) {
+    *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// W + 4 words, of which the W from byte `by` (0 to 16) on come to the front
+template <int W>
+__device__ __forceinline__ void shift(uint32_t* v, uint32_t by) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = by & 16 ? v[i + 4] : v[i];
+#pragma unroll
+    for (int i = 0; i < W + 2; ++i) v[i] = by & 8 ? v[i + 2] : v[i];
+#pragma unroll
+    for (int i = 0; i < W + 1; ++i) v[i] = by & 4 ? v[i + 1] : v[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = by & 2 ? __funnelshift_r(v[i], v[i + 1], 16) : v[i];
+}
+
+// How a tensor's rows lie: kStraight32 / kStraight16: every row starts on a 32- /
+// 16-byte boundary; kAny: on any element.  The last is served by whole 16-byte
+// vectors too, shifted in registers: a thread reads the vectors around its
+// columns where those lie inside the row, and writes whole vectors with the end
+// of its neighbour's columns, which it gets by a shuffle (2-byte accesses 32
+// bytes apart took 570 us where this takes 62: unpack, 8192 x 11003 to FP16).
+enum Lie { kAny, kStraight16, kStraight32 };
+
+template <int W>
+__device__ __forceinline__ bool load_words(const void* p, uint32_t col, int n, int lie, uint32_t* w) {
+    if (lie == kStraight32 && n >= 16) {
+#pragma unroll
+        for (int i = 0; i < W; i += 8) load32(static_cast<const uint32_t*>(p) + i, w + i);
+        return true;
+    }
+    if (lie == kStraight16 && n >= 16) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) load16(static_cast<const uint32_t*>(p) + i, w + i);
+        return true;
+    }
+    // 8 columns to each side are the row's
+    if (lie == kAny && col > 0 && n >= 24) {
+        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 15u);
+        const char* from = static_cast<const char*>(p) - off;
+        uint32_t v[W + 4];
+#pragma unroll
+        for (int i = 0; i < W; i += 4) load16(from + 4 * i, v + i);
+        v[W] = v[W + 1] = v[W + 2] = v[W + 3] = 0;
+        if (off) load16(from + 4 * W, v + W);
+        shift<W>(v, off);
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = v[i];
+        return true;
+    }
+    return false;
+}
+// All lanes of a warp take part.  E: bytes of an element.
+template <int W, int E>
+__device__ __forceinline__ void store_words(void* p, uint32_t col, int n, int lie, const uint32_t* w) {
+    char* q = static_cast<char*>(p);
+    auto some = [&](int lo, int hi) {   // elements lo to hi - 1, one by one
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i >= lo && i < hi) {
+                if (E == 4)
+                    reinterpret_cast<uint32_t*>(q)[i] = w[i];
+                else
+                    reinterpret_cast<uint16_t*>(q)[i] = i & 1 ? hi16(w[i >> 1]) : lo16(w[i >> 1]);
+            }
+    };
+    if (lie != kAny) {
+        if (n < 16) {
+            some(0, n);
+        } else if (lie == kStraight32) {
+#pragma unroll
+            for (int i = 0; i < W; i += 8) store32(q + 4 * i, w + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) store16(q + 4 * i, w + i);
+        }
+        return;
+    }
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(q) & 15u);
+    const int lane = threadIdx.x & 31;
+    const bool whole = n >= 16;
+    // the lane before holds the columns before mine, whole; the same behind me
+    const uint32_t wholes = __ballot_sync(0xFFFFFFFFu, whole);
+    const uint32_t starts = __ballot_sync(0xFFFFFFFFu, col == 0);
+    const bool before = lane > 0 && (wholes >> (lane - 1) & 1) && col > 0;
+    const bool behind = lane < 31 && (wholes >> (lane + 1) & 1) && !(starts >> (lane + 1) & 1);
+    uint32_t v[W + 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __shfl_up_sync(0xFFFFFFFFu, w[W - 4 + i], 1);
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[4 + i] = w[i];
+    if (!whole) {
+        some(0, n);
+        return;
+    }
+    shift<W>(v, 16 - off);
+    const bool head = off == 0 || before;   // all of the first vector is known
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+        if (i > 0 || head) store16(q - off + 4 * i, v + i);
+    if (!head) some(0, (int)(16 - off) / E);
+    if (off && !behind) some(16 - (int)off / E, 16);
+}
+
+// ------------------------------------------------------------ 16 columns of a thread
+template <class T>
+struct Chunk {   // a 16-bit type: pairs
+    uint32_t w[8];
+
+    __device__ __forceinline__ void load(const T* p, uint32_t col, int n, int lie) {
+        if (load_words<8>(p + col, col, n, lie, w)) return;
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + col;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            w[i] = pack16(2 * i < n ? q[2 * i] : (uint16_t)0, 2 * i + 1 < n ? q[2 * i + 1] : (uint16_t)0);
+    }
+    __device__ __forceinline__ void store(T* p, uint32_t col, int n, int lie) const {
+        store_words<8, 2>(p + col, col, n, lie, w);
+    }
+    __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) widen2(w[i], v[2 * i], v[2 * i + 1], T());
+    }
+    __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = narrow2(v[2 * i], v[2 * i + 1], T());
+    }
+    // FP32 bits of the largest magnitude of the block that two lanes hold
+    __device__ __forceinline__ uint32_t block_max() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        const uint32_t top = max(m & 0xFFFFu, m >> 16);
+        float a, b;
+        widen2(top, a, b, T());
+        return __float_as_uint(a);
+    }
+    template <int KIND>
+    __device__ __forceinline__ uint4 quant(uint32_t byte) const {
+        if constexpr (std::is_same<T, __half>::value) {
+            // 2^-k is an FP16 number, and x * 2^-k as FP16 keeps every bit that
+            // rounding to 8 bits looks at: below 2^-14, where it may not, all
+            // values round to 0
+            if (byte >= 127 - 15 && byte <= 127 + 14) {
+                const __half2 inv = __float2half2_rn(inv_scale(byte));
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __half2 a = *reinterpret_cast<const __half2*>(&w[2 * i]);
+                    const __half2 b = *reinterpret_cast<const __half2*>(&w[2 * i + 1]);
+                    if constexpr (KIND == kE4M3) {
+                        const __half2 x = __hmul2_rn(a, inv), y = __hmul2_rn(b, inv);
+                        uint16_t lo, hi;
+                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;"
+                            : "=h"(lo)
+                            : "r"(*reinterpret_cast<const uint32_t*>(&x)));
+                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;"
+                            : "=h"(hi)
+                            : "r"(*reinterpret_cast<const uint32_t*>(&y)));
+                        o[i] = pack16(lo, hi);
+                    } else {
+                        // 1536 + x * 2^-k rounds once, to a whole number; its low byte
+                        // is the integer's two's complement
+                        const __half2 magic = __float2half2_rn(1536.0f);
+                        const __half2 x = __hfma2(a, inv, magic), y = __hfma2(b, inv, magic);
+                        o[i] = __byte_perm(*reinterpret_cast<const uint32_t*>(&x),
+                                           *reinterpret_cast<const uint32_t*>(&y), 0x6420);
+                    }
+                }
+                return make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        if (byte == kActBad) return make_uint4(0u, 0u, 0u, 0u);
+        float v[16];
+        get(v);
+        const float inv = inv_scale(byte);
+        return make_uint4(quant4<KIND>(v, inv), quant4<KIND>(v + 4, inv), quant4<KIND>(v + 8, inv),
+                          quant4<KIND>(v + 12, inv));
+    }
+};
+template <>
+struct Chunk<float> {
+    float f[16];
+
+    __device__ __forceinline__ void load(const float* p, uint32_t col, int n, int lie) {
+        uint32_t w[16];
+        if (load_words<16>(p + col, col, n, lie, w)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(w[i]);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = i < n ? p[col + i] : 0.0f;
+    }
+    __device__ __forceinline__ void store(float* p, uint32_t col, int n, int lie) const {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(f[i]);
+        store_words<16, 4>(p + col, col, n, lie, w);
+    }
+    __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = f[i];
+    }
+    __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = v[i];
+    }
+    __device__ __forceinline__ uint32_t block_max() const {
+        const uint32_t m = abs_max<16>(f);
+        return max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    }
+    template <int KIND>
+    __device__ __forceinline__ uint4 quant(uint32_t byte) const {
+        if (byte == kActBad) return make_uint4(0u, 0u, 0u, 0u);
+        const float inv = inv_scale(byte);
+        return make_uint4(quant4<KIND>(f, inv), quant4<KIND>(f + 4, inv), quant4<KIND>(f + 8, inv),
+                          quant4<KIND>(f + 12, inv));
+    }
+};
+
+// one thread's 16 columns of a checkpoint; all lanes of a warp take part
+template <int KIND, class T>
+__device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t chunk, bool on,
+                                     const Chunk<T>& c) {
+    const uint32_t byte = scale_byte<KIND>(c.block_max());
+    if (!on) return;
+    *reinterpret_cast<uint4*>(data + chunk * 16) = c.template quant<KIND>(byte);
+    if ((threadIdx.x & 1) == 0) scale[chunk >> 1] = (uint8_t)byte;
+}
+
+// 16 stored columns as FP32
+template <int KIND>
+__device__ __forceinline__ void held(const uint8_t* data, const uint8_t* scale, uint64_t chunk,
+                                     float* v) {
+    const uint4 q = *reinterpret_cast<const uint4*>(data + chunk * 16);
+    const uint32_t byte = scale[chunk >> 1];
+    dequant8<KIND>(make_uint2(q.x, q.y), byte, v);
+    dequant8<KIND>(make_uint2(q.z, q.w), byte, v + 8);
 }
 
 // ------------------------------------------------------------ pack, unpack
 template <class T, int KIND>
 __global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x, uint64_t ldx,
                                                         uint64_t rows, uint32_t cols,
-                                                        uint32_t per_row, bool vec,
+                                                        uint32_t per_row, int lie,
                                                         uint8_t* __restrict__ data,
                                                         uint8_t* __restrict__ scale) {
     const uint64_t stride = (uint64_t)gridDim.x * kThreads;
-    const uint64_t total = rows * per_row;   // a multiple of 16: lanes of a block leave together
+    const uint64_t total = rows * per_row;   // a multiple of 8: lanes of a block leave together
     const uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
     Walk w(first, stride, per_row);
     for (uint64_t i = first; (i & ~31ull) < total; i += stride, w.next()) {
-        float v[8];
-        const int n = i < total ? left(cols, w.chunk * 8) : 0;
-        load8(x + w.row * ldx + w.chunk * 8, n, vec, v);
-        const uint32_t byte = scale_byte<KIND>(block_max(abs_max<8>(v)));
-        if (i < total) put<KIND>(data, scale, i, v, byte);
+        Chunk<T> c;
+        c.load(x + w.row * ldx, w.chunk * 16, i < total ? left(cols, w.chunk * 16) : 0, lie);
+        hold<KIND>(data, scale, i, i < total, c);
     }
 }
 
@@ -89,20 +337,44 @@ template <class T, int KIND>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restrict__ data,
                                                           const uint8_t* __restrict__ scale,
                                                           uint64_t rows, uint32_t cols,
-                                                          uint32_t per_row, bool vec,
+                                                          uint32_t per_row, int lie,
                                                           T* __restrict__ y, uint64_t ldy) {
     const uint64_t stride = (uint64_t)gridDim.x * kThreads;
     const uint64_t total = rows * per_row;
     const uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
     Walk w(first, stride, per_row);
-    for (uint64_t i = first; i < total; i += stride, w.next()) {
-        const int n = left(cols, w.chunk * 8);
-        if (n == 0) continue;
-        float v[8];
-        dequant8<KIND>(*reinterpret_cast<const uint2*>(data + i * 8), scale[i >> 2], v);
+    for (uint64_t i = first; (i & ~31ull) < total; i += stride, w.next()) {
+        const uint32_t col = w.chunk * 16;
+        const int n = i < total ? left(cols, col) : 0;
+        const uint64_t at = i < total ? i : 0;
+        Chunk<T> c;
+        if constexpr (std::is_same<T, float>::value) {
+            held<KIND>(data, scale, at, c.f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = saturate<T>(v[j]);
-        store8(y + w.row * ldy + w.chunk * 8, n, vec, v);
+            for (int j = 0; j < 16; ++j) c.f[j] = saturate<float>(c.f[j]);
+        } else {
+            uint4 lo, hi;
+            operand16<T, KIND>(*reinterpret_cast<const uint4*>(data + at * 16), scale[at >> 1], lo, hi);
+            c.w[0] = lo.x, c.w[1] = lo.y, c.w[2] = lo.z, c.w[3] = lo.w;
+            c.w[4] = hi.x, c.w[5] = hi.y, c.w[6] = hi.z, c.w[7] = hi.w;
+        }
+        c.store(y + w.row * ldy, col, n, lie);
+    }
+}
+
+// 16-bit rows from any boundary to 16-byte ones
+__global__ void __launch_bounds__(kThreads) realign_kernel(const __half* __restrict__ src, uint64_t ld,
+                                                           uint64_t rows, uint32_t cols,
+                                                           uint32_t per_row, __half* __restrict__ dst,
+                                                           uint64_t ldd) {
+    const uint64_t stride = (uint64_t)gridDim.x * kThreads, total = rows * per_row;
+    const uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+    Walk w(first, stride, per_row);
+    for (uint64_t i = first; i < total; i += stride, w.next()) {
+        const uint32_t col = w.chunk * 16;
+        Chunk<__half> c;
+        c.load(src + w.row * ld, col, left(cols, col), kAny);
+        c.store(dst + w.row * ldd, col, left(cols, col), kStraight16);
     }
 }
 
@@ -112,40 +384,42 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restr
 // 1 - s come without cancellation and keep their small end.
 __device__ __forceinline__ void sigmoid(float a, float& s, float& rest) {
     const float e = __expf(-fabsf(a));
-    const float r = __fdividef(1.0f, __fadd_rn(1.0f, e)), t = __fmul_rn(e, r);
+    float r;   // of 1 to 2
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
+    const float t = __fmul_rn(e, r);
     s = a < 0.0f ? t : r;
     rest = a < 0.0f ? r : t;
 }
 
 template <class T, int KIND, bool HOLD>
 __global__ void __launch_bounds__(kThreads) swiglu_kernel(
-    const T* a, uint64_t lda, const T* b, uint64_t ldb, uint64_t rows,
-    uint32_t cols, uint32_t per_row, bool vec, T* y, uint64_t ldy, uint8_t* __restrict__ a8,
+    const T* a, uint64_t lda, const T* b, uint64_t ldb, uint64_t rows, uint32_t cols,
+    uint32_t per_row, int lie, T* y, uint64_t ldy, uint8_t* __restrict__ a8,
     uint8_t* __restrict__ sa, uint8_t* __restrict__ b8, uint8_t* __restrict__ sb) {
     const uint64_t stride = (uint64_t)gridDim.x * kThreads;
     const uint64_t total = rows * per_row;
     const uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
     Walk w(first, stride, per_row);
     for (uint64_t i = first; (i & ~31ull) < total; i += stride, w.next()) {
-        float u[8], v[8], o[8];
-        const uint32_t col = w.chunk * 8;
+        const uint32_t col = w.chunk * 16;
         const int n = i < total ? left(cols, col) : 0;
-        load8(a + w.row * lda + col, n, vec, u);
-        load8(b + w.row * ldb + col, n, vec, v);
+        Chunk<T> ca, cb, cy;
+        ca.load(a + w.row * lda, col, n, lie);
+        cb.load(b + w.row * ldb, col, n, lie);
+        float u[16], v[16];
+        ca.get(u);
+        cb.get(v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float p, rest;
-            sigmoid(u[j], p, rest);
-            o[j] = __fmul_rn(__fmul_rn(u[j], p), v[j]);
+        for (int j = 0; j < 16; ++j) {
+            float s, rest;
+            sigmoid(u[j], s, rest);
+            u[j] = __fmul_rn(__fmul_rn(u[j], s), v[j]);
         }
-        store8(y + w.row * ldy + col, n, vec, o);
+        cy.set(u);
+        cy.store(y + w.row * ldy, col, n, lie);
         if (HOLD) {
-            const uint32_t ba = scale_byte<KIND>(block_max(abs_max<8>(u)));
-            const uint32_t bb = scale_byte<KIND>(block_max(abs_max<8>(v)));
-            if (i < total) {
-                put<KIND>(a8, sa, i, u, ba);
-                put<KIND>(b8, sb, i, v, bb);
-            }
+            hold<KIND>(a8, sa, i, i < total, ca);
+            hold<KIND>(b8, sb, i, i < total, cb);
         }
     }
 }
@@ -156,45 +430,54 @@ template <class T, int KIND, bool REMAKE>
 __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
     const T* dy, uint64_t lddy, const uint8_t* __restrict__ a8, const uint8_t* __restrict__ sa,
     const uint8_t* __restrict__ b8, const uint8_t* __restrict__ sb, uint64_t rows, uint32_t cols,
-    uint32_t per_row, bool vec, T* da, uint64_t ldda, T* db, uint64_t lddb,
+    uint32_t per_row, int lie, T* da, uint64_t ldda, T* db, uint64_t lddb,
     uint8_t* __restrict__ y8, uint8_t* __restrict__ sy) {
     const uint64_t stride = (uint64_t)gridDim.x * kThreads;
     const uint64_t total = rows * per_row;
     const uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
     Walk w(first, stride, per_row);
     for (uint64_t i = first; (i & ~31ull) < total; i += stride, w.next()) {
-        float u[8], v[8], g[8], o[8];
-        const uint32_t col = w.chunk * 8;
+        const uint32_t col = w.chunk * 16;
         const int n = i < total ? left(cols, col) : 0;
         const uint64_t at = i < total ? i : 0;
-        load8(dy + w.row * lddy + col, n, vec, g);
-        dequant8<KIND>(*reinterpret_cast<const uint2*>(a8 + at * 8), sa[at >> 2], u);
-        dequant8<KIND>(*reinterpret_cast<const uint2*>(b8 + at * 8), sb[at >> 2], v);
+        Chunk<T> g, cy;
+        g.load(dy + w.row * lddy, col, n, lie);
+        float u[16], v[16], d[16], o[16];
+        held<KIND>(a8, sa, at, u);
+        held<KIND>(b8, sb, at, v);
+        g.get(d);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 16; ++j) {
             float s, rest;
             sigmoid(u[j], s, rest);
             const float t = __fmul_rn(u[j], s);
             const float slope = __fmul_rn(s, __fmaf_rn(u[j], rest, 1.0f));
-            u[j] = __fmul_rn(__fmul_rn(g[j], v[j]), slope);
-            o[j] = j < n ? Elem<T>::to_f(Elem<T>::from_f(__fmul_rn(t, v[j]))) : 0.0f;
-            v[j] = __fmul_rn(g[j], t);
+            o[j] = __fmul_rn(t, v[j]);
+            u[j] = __fmul_rn(__fmul_rn(d[j], v[j]), slope);
+            v[j] = __fmul_rn(d[j], t);
         }
-        store8(da + w.row * ldda + col, n, vec, u);
-        store8(db + w.row * lddb + col, n, vec, v);
+        g.set(u);
+        g.store(da + w.row * ldda, col, n, lie);
+        g.set(v);
+        g.store(db + w.row * lddb, col, n, lie);
         if (REMAKE) {
-            const uint32_t byte = scale_byte<KIND>(block_max(abs_max<8>(o)));
-            if (i < total) put<KIND>(y8, sy, i, o, byte);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = j < n ? o[j] : 0.0f;
+            cy.set(o);
+            hold<KIND>(y8, sy, i, i < total, cy);
         }
     }
 }
 
 template <class T>
-bool rows_vec(const T* p, uint64_t ld) {
-    return aligned16(p) && ld * sizeof(T) % 16 == 0;
+int lie_of(const T* p, uint64_t ld) {
+    return aligned_to(p, 32) && ld * sizeof(T) % 32 == 0 ? kStraight32
+           : aligned16(p) && ld * sizeof(T) % 16 == 0    ? kStraight16
+                                                         : kAny;
 }
+int least(int a, int b) { return a < b ? a : b; }
 
-// rows of 16-byte chunks: cols elements, ld apart
+// rows of cols elements, ld apart
 bool shape_ok(uint64_t rows, uint64_t cols, uint64_t ld) {
     return cols < (1ull << 31) && rows < (1ull << 40) && (rows <= 1 || ld >= cols || ld == 0);
 }
@@ -207,30 +490,30 @@ unsigned grid_of(uint64_t work) {
 
 template <class T, int KIND>
 int pack_t(const T* x, uint64_t ldx, const ark_act8* o, cudaStream_t s) {
-    const uint32_t per = (uint32_t)(act8_pitch(o->cols) / 8);
+    const uint32_t per = (uint32_t)(act8_pitch(o->cols) / 16);
     auto k = pack_kernel<T, KIND>;
     k<<<grid_of(o->rows * per), kThreads, 0, s>>>(x, ldx, o->rows, (uint32_t)o->cols, per,
-                                                     rows_vec(x, ldx), o->data, o->scale);
+                                                     lie_of(x, ldx), o->data, o->scale);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
 template <class T, int KIND>
 int unpack_t(const ark_act8* c, T* y, uint64_t ldy, cudaStream_t s) {
-    const uint32_t per = (uint32_t)(act8_pitch(c->cols) / 8);
+    const uint32_t per = (uint32_t)(act8_pitch(c->cols) / 16);
     auto k = unpack_kernel<T, KIND>;
     k<<<grid_of(c->rows * per), kThreads, 0, s>>>(c->data, c->scale, c->rows, (uint32_t)c->cols,
-                                                     per, rows_vec(y, ldy), y, ldy);
+                                                     per, lie_of(y, ldy), y, ldy);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
 template <class T, int KIND, bool HOLD>
 int swiglu_t(const T* a, uint64_t lda, const T* b, uint64_t ldb, uint64_t rows, uint64_t cols, T* y,
              uint64_t ldy, const ark_act8* a8, const ark_act8* b8, cudaStream_t s) {
-    const uint32_t per = (uint32_t)(act8_pitch(cols) / 8);
-    const bool vec = rows_vec(a, lda) && rows_vec(b, ldb) && rows_vec(y, ldy);
+    const uint32_t per = (uint32_t)(act8_pitch(cols) / 16);
+    const int lie = least(least(lie_of(a, lda), lie_of(b, ldb)), lie_of(y, ldy));
     auto k = swiglu_kernel<T, KIND, HOLD>;
     k<<<grid_of(rows * per), kThreads, 0, s>>>(
-        a, lda, b, ldb, rows, (uint32_t)cols, per, vec, y, ldy, HOLD ? a8->data : nullptr,
+        a, lda, b, ldb, rows, (uint32_t)cols, per, lie, y, ldy, HOLD ? a8->data : nullptr,
         HOLD ? a8->scale : nullptr, HOLD ? b8->data : nullptr, HOLD ? b8->scale : nullptr);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
@@ -238,11 +521,11 @@ int swiglu_t(const T* a, uint64_t lda, const T* b, uint64_t ldb, uint64_t rows, 
 template <class T, int KIND, bool REMAKE>
 int swiglu_back_t(const T* dy, uint64_t lddy, const ark_act8* a8, const ark_act8* b8, T* da,
                   uint64_t ldda, T* db, uint64_t lddb, const ark_act8* y8, cudaStream_t s) {
-    const uint32_t per = (uint32_t)(act8_pitch(a8->cols) / 8);
-    const bool vec = rows_vec(dy, lddy) && rows_vec(da, ldda) && rows_vec(db, lddb);
+    const uint32_t per = (uint32_t)(act8_pitch(a8->cols) / 16);
+    const int lie = least(least(lie_of(dy, lddy), lie_of(da, ldda)), lie_of(db, lddb));
     auto k = swiglu_back_kernel<T, KIND, REMAKE>;
     k<<<grid_of(a8->rows * per), kThreads, 0, s>>>(
-        dy, lddy, a8->data, a8->scale, b8->data, b8->scale, a8->rows, (uint32_t)a8->cols, per, vec,
+        dy, lddy, a8->data, a8->scale, b8->data, b8->scale, a8->rows, (uint32_t)a8->cols, per, lie,
         da, ldda, db, lddb, REMAKE ? y8->data : nullptr, REMAKE ? y8->scale : nullptr);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
@@ -252,6 +535,15 @@ bool same_shape(const ark_act8* a, const ark_act8* b) {
 }
 
 }  // namespace
+
+int realign_rows(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, void* dst, uint64_t ldd,
+                 cudaStream_t s) {
+    const uint32_t per = (cols + 15) / 16;
+    realign_kernel<<<grid_of(rows * per), kThreads, 0, s>>>(
+        static_cast<const __half*>(src), ld, rows, cols, per, static_cast<__half*>(dst), ldd);
+    return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+}
+
 }  // namespace ark
 
 using namespace ark;

@@ -224,6 +224,130 @@ __device__ __forceinline__ void dequant8(uint2 w, uint32_t byte, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], s);
 }
 
+// ------------------------------------------------------------ bytes to 16-bit values
+// Two FP32 values to a pair of T, saturating (a NaN stays one).
+__device__ __forceinline__ uint32_t pair_of(float a, float b, __half) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// Scale bytes between which q * 2^k needs neither saturation nor a scale
+// outside of T; every block of ordinary activations lies between them.  The
+// others (and NaN blocks) go through FP32.
+template <class T, int KIND>
+struct Fast;
+template <>
+struct Fast<__half, kE4M3> {
+    // 2^-24 is the smallest FP16; 448 * 2^7 is below 65504
+    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 7;
+    __half2 s;
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        s = __float2half2_rn(__uint_as_float(byte << 23));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {   // bytes at, at + 1
+        uint32_t h;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (8 * at))));
+        const __half2 r = __hmul2_rn(*reinterpret_cast<__half2*>(&h), s);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <>
+struct Fast<__half, kInt8> {
+    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 5;
+    __half2 s, t;   // 2^k and -1152 * 2^k
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        const float f = __uint_as_float(byte << 23);
+        s = __float2half2_rn(f);
+        t = __float2half2_rn(__fmul_rn(f, -1152.0f));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
+        // (q + 128) as the low byte of 1024 is 1152 + q: one fused operation
+        // takes the offset off and scales, exactly
+        const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, at ? 0x4342 : 0x4140);
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&h), s, t);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <>
+struct Fast<__nv_bfloat16, kE4M3> {
+    // exponent and mantissa of e4m3 moved to BF16's, whose bias is 120 larger:
+    // the value times 2^-120, subnormals included
+    static constexpr uint32_t kLo = 1, kHi = 127 + 7;
+    __nv_bfloat162 s;
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        s = __float2bfloat162_rn(__uint_as_float((byte + 120u) << 23));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
+        const uint32_t h = __byte_perm(w, 0u, at ? 0x3424 : 0x1404);   // bytes to the high halves
+        const uint32_t v = (h & 0x80008000u) | ((h >> 4) & 0x07F007F0u);
+        const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&v), s);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+template <>
+struct Fast<__nv_bfloat16, kInt8> {
+    static constexpr uint32_t kLo = 1, kHi = 127 + 120;
+    __nv_bfloat162 s;
+    __device__ __forceinline__ explicit Fast(uint32_t byte) {
+        s = __float2bfloat162_rn(__uint_as_float(byte << 23));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
+        // under the exponent of 128 the low 7 bits are 128 + (q mod 128), and the
+        // sign bit alone is 128 or 256: their difference is q
+        const uint32_t h = __byte_perm(w, 0x43434343u, at ? 0x4342 : 0x4140);
+        const uint32_t lo = h & 0xFF7FFF7Fu, hi = h & 0xFF80FF80u;
+        const __nv_bfloat162 r =
+            __hmul2_rn(__hsub2_rn(*reinterpret_cast<const __nv_bfloat162*>(&lo),
+                                  *reinterpret_cast<const __nv_bfloat162*>(&hi)),
+                       s);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+};
+// Sixteen bytes of one block to 16-bit values in order.
+template <class T, int KIND>
+__device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uint4& hi) {
+    if (byte >= Fast<T, KIND>::kLo && byte <= Fast<T, KIND>::kHi) {
+        const Fast<T, KIND> f(byte);
+        lo = make_uint4(f.pair(w.x, 0), f.pair(w.x, 2), f.pair(w.y, 0), f.pair(w.y, 2));
+        hi = make_uint4(f.pair(w.z, 0), f.pair(w.z, 2), f.pair(w.w, 0), f.pair(w.w, 2));
+    } else {
+        float v[8];
+        dequant8<KIND>(make_uint2(w.x, w.y), byte, v);
+        lo = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
+                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+        dequant8<KIND>(make_uint2(w.z, w.w), byte, v);
+        hi = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
+                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+    }
+}
+
+// ------------------------------------------------------------ pairs of FP32
+// One instruction for two products or sums, each rounded as the single one is.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // ------------------------------------------------------------ host checks
 inline uint64_t type_size(int32_t type) {
     return type == ARK_TYPE_F32 ? 4u : (type == ARK_TYPE_F16 || type == ARK_TYPE_BF16) ? 2u : 0u;
@@ -242,5 +366,8 @@ int by_type(int32_t type, F f) {
 
 // null data is fine for an empty checkpoint
 int act8_check(const ark_act8* c);
+// 16-bit rows that start on any element, copied to rows of whole 16-byte vectors
+int realign_rows(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, void* dst, uint64_t ldd,
+                 cudaStream_t s);
 
 }  // namespace ark

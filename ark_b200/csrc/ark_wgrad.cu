@@ -71,7 +71,7 @@ struct Args {
     uint32_t tiles_m, tiles_n, tiles;
     uint32_t chunks;          // runs of steps whose sums are added by the epilogue
     uint32_t splits;          // pair_kernel: runs of tokens that are tiles of their own,
-    float* partial;           // and where their sums go, [splits][m][n_pad]
+    float* partial;           // and where their FP32 sums go, [splits][m][n_pad], or null
     uint32_t n_pad;
     Out out;
     int accumulate;
@@ -246,6 +246,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
         : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -275,108 +285,6 @@ __device__ __forceinline__ float4 peer_ld(uint32_t addr, uint32_t rank) {
                  : "r"(p)
                  : "memory");
     return v;
-}
-
-// ------------------------------------------------------------ bytes to operands
-// Two FP32 values to a pair of T, saturating (a NaN stays one).
-__device__ __forceinline__ uint32_t pair_of(float a, float b, __half) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-__device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-
-// Scale bytes between which q * 2^k needs neither saturation nor a scale
-// outside of T; every block of ordinary activations lies between them.  The
-// others (and NaN blocks) go through FP32.
-template <class T, int KIND>
-struct Fast;
-template <>
-struct Fast<__half, kE4M3> {
-    // 2^-24 is the smallest FP16; 448 * 2^7 is below 65504
-    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 7;
-    __half2 s;
-    __device__ __forceinline__ explicit Fast(uint32_t byte) {
-        s = __float2half2_rn(__uint_as_float(byte << 23));
-    }
-    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {   // bytes at, at + 1
-        uint32_t h;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (8 * at))));
-        const __half2 r = __hmul2_rn(*reinterpret_cast<__half2*>(&h), s);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-};
-template <>
-struct Fast<__half, kInt8> {
-    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 5;
-    __half2 s, t;   // 2^k and -1152 * 2^k
-    __device__ __forceinline__ explicit Fast(uint32_t byte) {
-        const float f = __uint_as_float(byte << 23);
-        s = __float2half2_rn(f);
-        t = __float2half2_rn(__fmul_rn(f, -1152.0f));
-    }
-    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
-        // (q + 128) as the low byte of 1024 is 1152 + q: one fused operation
-        // takes the offset off and scales, exactly
-        const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, at ? 0x4342 : 0x4140);
-        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&h), s, t);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-};
-template <>
-struct Fast<__nv_bfloat16, kE4M3> {
-    // exponent and mantissa of e4m3 moved to BF16's, whose bias is 120 larger:
-    // the value times 2^-120, subnormals included
-    static constexpr uint32_t kLo = 1, kHi = 127 + 7;
-    __nv_bfloat162 s;
-    __device__ __forceinline__ explicit Fast(uint32_t byte) {
-        s = __float2bfloat162_rn(__uint_as_float((byte + 120u) << 23));
-    }
-    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
-        const uint32_t h = __byte_perm(w, 0u, at ? 0x3424 : 0x1404);   // bytes to the high halves
-        const uint32_t v = (h & 0x80008000u) | ((h >> 4) & 0x07F007F0u);
-        const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&v), s);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-};
-template <>
-struct Fast<__nv_bfloat16, kInt8> {
-    static constexpr uint32_t kLo = 1, kHi = 127 + 120;
-    __nv_bfloat162 s;
-    __device__ __forceinline__ explicit Fast(uint32_t byte) {
-        s = __float2bfloat162_rn(__uint_as_float(byte << 23));
-    }
-    __device__ __forceinline__ uint32_t pair(uint32_t w, int at) const {
-        // under the exponent of 128 the low 7 bits are 128 + (q mod 128), and the
-        // sign bit alone is 128 or 256: their difference is q
-        const uint32_t h = __byte_perm(w, 0x43434343u, at ? 0x4342 : 0x4140);
-        const uint32_t lo = h & 0xFF7FFF7Fu, hi = h & 0xFF80FF80u;
-        const __nv_bfloat162 r =
-            __hmul2_rn(__hsub2_rn(*reinterpret_cast<const __nv_bfloat162*>(&lo),
-                                  *reinterpret_cast<const __nv_bfloat162*>(&hi)),
-                       s);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    }
-};
-template <class T, int KIND>
-__device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uint4& hi) {
-    if (byte >= Fast<T, KIND>::kLo && byte <= Fast<T, KIND>::kHi) {
-        const Fast<T, KIND> f(byte);
-        lo = make_uint4(f.pair(w.x, 0), f.pair(w.x, 2), f.pair(w.y, 0), f.pair(w.y, 2));
-        hi = make_uint4(f.pair(w.z, 0), f.pair(w.z, 2), f.pair(w.w, 0), f.pair(w.w, 2));
-    } else {
-        float v[8];
-        dequant8<KIND>(make_uint2(w.x, w.y), byte, v);
-        lo = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
-                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
-        dequant8<KIND>(make_uint2(w.z, w.w), byte, v);
-        hi = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
-                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
-    }
 }
 
 // ------------------------------------------------------------ output
@@ -684,7 +592,8 @@ __device__ __forceinline__ void pair_tile(const Args& a, uint32_t t, uint32_t& m
     m = band * 8 + (at - n * high);
 }
 
-template <class T>
+// RUNS: FP32 sums of several runs of an item's tokens, added by the epilogue.
+template <class T, bool RUNS>
 __global__ void __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
                 const Args a) {
@@ -810,18 +719,23 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t row = m * (2 * kBM) + rank * kBM + quarter * 32 + lane;
             Out out = a.out;
             bool accumulate = a.accumulate;
-            if (a.splits > 1) {
+            if (a.partial) {
                 out = Out{a.partial + (uint64_t)run * a.m * a.n_pad, a.n_pad, 1, 0, 1};
                 accumulate = false;
             }
+            // 16 columns from c on
             auto put = [&](uint32_t c, float* v, bool ok) {
-                if (!ok) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
+                for (int j = 0; j < 16; ++j) v[j] = ok ? v[j] : __uint_as_float(0x7FC00000u);
+#pragma unroll
+                for (int j = 0; j < 16; j += 8) {
+                    const uint32_t col = n * S::kBN + c + j;
+                    if (RUNS && row < a.m && col + 8 <= a.n && out.vec)
+                        out_vec<8>(static_cast<float*>(out.p) + (uint64_t)row * out.ld + col, v + j,
+                                   accumulate);
+                    else
+                        out_row<8>(out, a.m, a.n, row, col, v + j, accumulate);
                 }
-#pragma unroll
-                for (int j = 0; j < 32; j += 8)
-                    out_row<8>(out, a.m, a.n, row, n * S::kBN + c + j, v + j, accumulate);
             };
             auto next = [&] {
                 fence_before();
@@ -829,7 +743,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if (lane == 0) bar_arrive_at(bar_of(smem_u32(acc_empty + buf), 0));
                 if (++buf == 2) buf = 0, bphase ^= 1u;
             };
-            if (a.chunks == 1) {
+            if constexpr (!RUNS) {
                 const bool ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up);
                 fence_after();
 #pragma unroll 1
@@ -838,27 +752,28 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
                     put(c, v, ok);
+                    put(c + 16, v + 16, ok);
                 }
                 next();
             } else {
                 // the runs' sums are added in registers
-                float sum[kCols / 32][32];
+                float sum[kCols / 16][16];
                 bool ok = true;
                 for (uint32_t k = 0; k < a.chunks; ++k) {
                     ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up) && ok;
                     fence_after();
 #pragma unroll
-                    for (int c = 0; c < kCols / 32; ++c) {
-                        float v[32];
-                        tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c0 + c * 32,
+                    for (int c = 0; c < kCols / 16; ++c) {
+                        float v[16];
+                        tmem_ld16(tmem + buf * S::kBN + (quarter * 32 << 16) + c0 + c * 16,
                                   reinterpret_cast<uint32_t*>(v));
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[c][j] = k ? __fadd_rn(sum[c][j], v[j]) : v[j];
+                        for (int j = 0; j < 16; ++j) sum[c][j] = k ? __fadd_rn(sum[c][j], v[j]) : v[j];
                     }
                     next();
                 }
 #pragma unroll
-                for (int c = 0; c < kCols / 32; ++c) put(c0 + c * 32, sum[c], ok);
+                for (int c = 0; c < kCols / 16; ++c) put(c0 + c * 16, sum[c], ok);
             }
         }
     }
@@ -871,22 +786,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                      "r"(2 * S::kBN));
     }
     cluster_sync();
-}
-
-// dY whose rows TMA cannot address, copied to rows of a multiple of 16 bytes
-__global__ void __launch_bounds__(256) realign_kernel(const uint16_t* __restrict__ src, uint64_t ld,
-                                                      uint64_t rows, uint32_t cols,
-                                                      uint16_t* __restrict__ dst, uint32_t ldd) {
-    const uint32_t per = ldd / 2;
-    const uint64_t total = rows * per;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-         i += (uint64_t)gridDim.x * 256) {
-        const uint64_t r = i / per;
-        const uint32_t c = (uint32_t)(i - r * per) * 2;
-        const uint16_t lo = c < cols ? src[r * ld + c] : (uint16_t)0;
-        const uint16_t hi = c + 1 < cols ? src[r * ld + c + 1] : (uint16_t)0;
-        *reinterpret_cast<uint32_t*>(dst + r * ldd + c) = pack16(lo, hi);
-    }
 }
 
 // the runs' partial sums, added in order: four columns per thread
@@ -979,10 +878,12 @@ int launch_few(const CUtensorMap& map, const Args& a, uint32_t parts, cudaStream
 }
 template <class T>
 int launch_pair(const CUtensorMap& x, const CUtensorMap& dy, const Args& a, cudaStream_t s) {
-    static std::atomic<uint64_t> ready{0};
+    static std::atomic<uint64_t> ready{0}, runs{0};
     const uint32_t most = (uint32_t)sm_count() / 2, items = a.tiles * a.splits;
     const uint32_t pairs = items < most ? items : most;
-    return launch(pair_kernel<T>, pairs * 2, kPairThreads, Pair::kSmem, 2, ready, s, x, dy, a);
+    if (a.chunks > 1)
+        return launch(pair_kernel<T, true>, pairs * 2, kPairThreads, Pair::kSmem, 2, runs, s, x, dy, a);
+    return launch(pair_kernel<T, false>, pairs * 2, kPairThreads, Pair::kSmem, 2, ready, s, x, dy, a);
 }
 
 // [rows, cols] of 16-bit elements, ld apart, in boxes of 64 columns by 64 rows
@@ -1044,7 +945,7 @@ struct Way {
     uint32_t splits;   // pairs: runs of tokens
     uint64_t x_bytes, partial_bytes;
 };
-Way way_of(uint64_t tokens, uint64_t m, uint64_t n) {
+Way way_of(uint64_t tokens, uint64_t m, uint64_t n, bool vec) {
     const uint64_t iters = (tokens + kBK - 1) / kBK, sms = (uint64_t)sm_count();
     const uint64_t few = (m + 127) / 128 * ((n + 127) / 128);
     const uint64_t tiles = (m + 255) / 256 * ((n + 255) / 256);
@@ -1059,14 +960,20 @@ Way way_of(uint64_t tokens, uint64_t m, uint64_t n) {
     for (uint32_t r = 1; r <= 16 && (r == 1 || r * 8 <= iters); ++r) {
         const uint64_t waves = ceil_div(tiles * r, sms / 2);
         const uint64_t t = 8000 + x_bytes * 3 / 2 / 5000 + waves * (1500 + 330 * ceil_div(iters, r)) +
-                           (r > 1 ? 3000 + 2 * r * run / 8000 : 0);
+                           (r > 1 || !vec ? 3000 + 2 * r * run / 8000 : 0);
         if (t < best) best = t, w.pairs = true, w.splits = r;
     }
     if (w.pairs) {
         w.x_bytes = x_bytes;
-        w.partial_bytes = w.splits > 1 ? w.splits * run : 0;
+        // rows of an output that vectors cannot write go through the FP32 buffer
+        // too: an accumulator's lane holds one row, and element by element 32 rows
+        // at a time 4096 tokens, 2048 x 5501 took 225 us
+        w.partial_bytes = w.splits > 1 || !vec ? w.splits * run : 0;
     }
     return w;
+}
+bool out_vec_rows(const void* dw, int32_t type, uint64_t ld) {
+    return aligned16(dw) && ld * type_size(type) % 16 == 0;
 }
 // the workspace's last part: dY realigned
 uint64_t ws_dy(uint64_t tokens, const void* dy, uint64_t lddy, uint64_t n) {
@@ -1081,9 +988,10 @@ using namespace ark;
 extern "C" {
 
 uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
-                                        uint64_t n_out) {
+                                        uint64_t n_out, const void* dw, int32_t dw_type,
+                                        uint64_t lddw) {
     if (!x || !x->rows || !x->cols || !n_out) return 0;
-    const Way w = way_of(x->rows, x->cols, n_out);
+    const Way w = way_of(x->rows, x->cols, n_out, out_vec_rows(dw, dw_type, lddw));
     return w.x_bytes + w.partial_bytes + ws_dy(x->rows, dy, lddy, n_out);
 }
 
@@ -1114,7 +1022,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     a.n = (uint32_t)n_out;
     a.iters = (a.tokens + kBK - 1) / kBK;
     a.out = Out{dw, lddw, dw_type == ARK_TYPE_F32, dw_type == ARK_TYPE_BF16,
-                aligned16(dw) && lddw * e % 16 == 0};
+                out_vec_rows(dw, dw_type, lddw)};
     a.accumulate = accumulate != 0;
     if (x->rows == 0) {
         if (accumulate) return ARK_OK;
@@ -1123,7 +1031,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
     }
 
-    const Way w = way_of(x->rows, x->cols, n_out);
+    const Way w = way_of(x->rows, x->cols, n_out, a.out.vec);
     const uint64_t need_dy = ws_dy(x->rows, dy, lddy, n_out);
     const uint64_t need = w.x_bytes + w.partial_bytes + need_dy;
     if (need) {
@@ -1134,36 +1042,33 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     uint64_t ld = lddy;
     if (need_dy) {
         ld = realigned(n_out);
-        uint16_t* to = reinterpret_cast<uint16_t*>(ws + w.x_bytes + w.partial_bytes);
-        const uint64_t blocks = (x->rows * ld / 2 + 255) / 256, most = (uint64_t)sm_count() * 8;
-        realign_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
-            static_cast<const uint16_t*>(dy), lddy, x->rows, a.n, to, (uint32_t)ld);
-        if (cudaGetLastError() != cudaSuccess) return ARK_E_CUDA;
+        void* to = ws + w.x_bytes + w.partial_bytes;
+        if (const int rc2 = realign_rows(dy, lddy, x->rows, a.n, to, ld, s)) return rc2;
         dy = to;
     }
     CUtensorMap map;
-    int e2 = encode(&map, dy_type, dy, x->rows, n_out, ld);
-    if (e2) return e2;
+    int failed = encode(&map, dy_type, dy, x->rows, n_out, ld);
+    if (failed) return failed;
 
     if (w.pairs) {
         a.tiles_m = (a.m + 255) / 256;
         a.tiles_n = (a.n + 255) / 256;
         a.tiles = a.tiles_m * a.tiles_n;
         a.splits = w.splits;
-        a.partial = reinterpret_cast<float*>(ws + w.x_bytes);
+        a.partial = w.partial_bytes ? reinterpret_cast<float*>(ws + w.x_bytes) : nullptr;
         a.n_pad = (a.n + 3) / 4 * 4;
         // the tensor cores' FP32 sums are cut off, not rounded: FP32 gradients of
         // more than 2048 tokens are summed in runs that the epilogue adds
         const uint32_t run = (a.iters + a.splits - 1) / a.splits;
         a.chunks = a.out.f32 ? (run + 31) / 32 : 1;
-        e2 = ark_cuda_act8_unpack(x, ws, dy_type, a.pitch, cuda_stream);
-        if (e2) return e2;
+        failed = ark_cuda_act8_unpack(x, ws, dy_type, a.pitch, cuda_stream);
+        if (failed) return failed;
         CUtensorMap map_x;
-        e2 = encode(&map_x, dy_type, ws, x->rows, x->cols, a.pitch);
-        if (e2) return e2;
-        e2 = dy_type == ARK_TYPE_F16 ? launch_pair<__half>(map_x, map, a, s)
+        failed = encode(&map_x, dy_type, ws, x->rows, x->cols, a.pitch);
+        if (failed) return failed;
+        failed = dy_type == ARK_TYPE_F16 ? launch_pair<__half>(map_x, map, a, s)
                                      : launch_pair<__nv_bfloat16>(map_x, map, a, s);
-        if (e2 || a.splits == 1) return e2;
+        if (failed || !a.partial) return failed;
         const uint64_t blocks = ((uint64_t)a.m * a.n_pad / 4 + 255) / 256, most = (uint64_t)sm_count() * 8;
         static std::atomic<uint64_t> ready{0};
         return launch(runs_kernel, (uint32_t)(blocks < most ? blocks : most), 256, 0, 1, ready, s, a);

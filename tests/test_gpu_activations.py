@@ -341,3 +341,33 @@ def test_qk_no_tokens():
     out = ab.qk_norm_rope_backward(e, e[:, :2], y[2], y[3], g, g, plan)
     assert (out[2] == 0).all() and (out[3] == 0).all()
     assert ab.rope(e, None, plan)[0].shape == (0, 4, 32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,extra,off", [(511, 0, 0), (700, 1, 1), (1000, 3, 2), (129, 0, 3), (513, 2, 5), (2000, 7, 7), (40, 1, 1),
+                                            (24, 9, 1), (17, 0, 0), (600, 8, 8), (600, 8, 4)])
+def test_rows_on_any_boundary(cols, extra, off, dtype):
+    """Rows that start anywhere: every value right, and nothing written beside them."""
+    rows, width = 37, cols + extra + off
+    g = rng(cols)
+    x = torch.randn(rows, width, generator=g).to(dtype).cuda()[:, off: off + cols]
+    c = ab.act8_pack(x, "int8")
+    data, scale = ref.pack(x.cpu(), "int8")
+    assert torch.equal(c.data.cpu(), data) and torch.equal(c.scale.cpu(), scale)
+    guard = torch.full((rows + 2, width), 9.0, dtype=dtype, device="cuda")
+    out = guard[1: rows + 1, off: off + cols]
+    ab.act8_unpack(c, out=out)
+    assert torch.equal(out.cpu(), ref.values(data, scale, cols, "int8").to(dtype))
+    aligned = [t.contiguous() for t in (x, x.flip(0))]
+    y, ca, cb = ab.swiglu(*aligned, checkpoint="int8")
+    z = torch.empty(rows, width, dtype=dtype, device="cuda")[:, off: off + cols]
+    z.copy_(aligned[1])
+    got, da, db = ab.swiglu(x, z, checkpoint="int8", out=out)
+    assert torch.equal(out, y) and torch.equal(da.data, ca.data) and torch.equal(db.data, cb.data)
+    ga, gb = ab.swiglu_backward(aligned[0], ca, cb)
+    ab.swiglu_backward(x, ca, cb, out=(out, z))
+    assert torch.equal(out, ga) and torch.equal(z, gb)
+    ab.swiglu(x, aligned[1], out=x)                                  # in place
+    assert torch.equal(x, y)
+    out.fill_(9)
+    assert (guard == 9).all()
