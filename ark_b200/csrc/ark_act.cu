@@ -11,8 +11,6 @@
 // 16-bit types keep to pairs: the largest magnitude by integer maxima of two,
 // and FP16 is scaled and rounded to 8 bits as FP16 pairs where the block's scale
 // is an FP16 number.
-#include <type_traits>
-
 #include "ark_act8.cuh"
 
 namespace ark {
@@ -202,56 +200,15 @@ struct Chunk {   // a 16-bit type: pairs
     }
     // FP32 bits of the largest magnitude of the block that two lanes hold
     __device__ __forceinline__ uint32_t block_max() const {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        uint32_t m = pairs_max<8>(w);
         m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        const uint32_t top = max(m & 0xFFFFu, m >> 16);
-        float a, b;
-        widen2(top, a, b, T());
-        return __float_as_uint(a);
+        return pairs_bits(m, T());
     }
     template <int KIND>
     __device__ __forceinline__ uint4 quant(uint32_t byte) const {
-        if constexpr (std::is_same<T, __half>::value) {
-            // 2^-k is an FP16 number, and x * 2^-k as FP16 keeps every bit that
-            // rounding to 8 bits looks at: below 2^-14, where it may not, all
-            // values round to 0
-            if (byte >= 127 - 15 && byte <= 127 + 14) {
-                const __half2 inv = __float2half2_rn(inv_scale(byte));
-                uint32_t o[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const __half2 a = *reinterpret_cast<const __half2*>(&w[2 * i]);
-                    const __half2 b = *reinterpret_cast<const __half2*>(&w[2 * i + 1]);
-                    if constexpr (KIND == kE4M3) {
-                        const __half2 x = __hmul2_rn(a, inv), y = __hmul2_rn(b, inv);
-                        uint16_t lo, hi;
-                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;"
-                            : "=h"(lo)
-                            : "r"(*reinterpret_cast<const uint32_t*>(&x)));
-                        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;"
-                            : "=h"(hi)
-                            : "r"(*reinterpret_cast<const uint32_t*>(&y)));
-                        o[i] = pack16(lo, hi);
-                    } else {
-                        // 1536 + x * 2^-k rounds once, to a whole number; its low byte
-                        // is the integer's two's complement
-                        const __half2 magic = __float2half2_rn(1536.0f);
-                        const __half2 x = __hfma2(a, inv, magic), y = __hfma2(b, inv, magic);
-                        o[i] = __byte_perm(*reinterpret_cast<const uint32_t*>(&x),
-                                           *reinterpret_cast<const uint32_t*>(&y), 0x6420);
-                    }
-                }
-                return make_uint4(o[0], o[1], o[2], o[3]);
-            }
-        }
-        if (byte == kActBad) return make_uint4(0u, 0u, 0u, 0u);
-        float v[16];
-        get(v);
-        const float inv = inv_scale(byte);
-        return make_uint4(quant4<KIND>(v, inv), quant4<KIND>(v + 4, inv), quant4<KIND>(v + 8, inv),
-                          quant4<KIND>(v + 12, inv));
+        uint32_t o[4];
+        quant_words<T, KIND, 8>(w, byte, o);
+        return make_uint4(o[0], o[1], o[2], o[3]);
     }
 };
 template <>

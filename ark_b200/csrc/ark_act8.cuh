@@ -19,6 +19,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ark_device.cuh"
 #include "ark_internal.h"
 
@@ -327,6 +329,66 @@ __device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uin
     }
 }
 
+// ------------------------------------------------------------ 16-bit values to bytes
+// The largest magnitudes of N words' low and high halves.
+template <int N>
+__device__ __forceinline__ uint32_t pairs_max(const uint32_t* w) {
+    uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    return m;
+}
+// The FP32 bits of the larger half.
+template <class T>
+__device__ __forceinline__ uint32_t pairs_bits(uint32_t m, T) {
+    float a, b;
+    widen2(max(m & 0xFFFFu, m >> 16), a, b, T());
+    return __float_as_uint(a);
+}
+// N words of two values of a block with scale byte `byte` to N / 2 words of four bytes.
+template <class T, int KIND, int N>
+__device__ __forceinline__ void quant_words(const uint32_t* w, uint32_t byte, uint32_t* o) {
+    if constexpr (std::is_same<T, __half>::value) {
+        // 2^-k is an FP16 number, and x * 2^-k as FP16 keeps every bit that rounding
+        // to 8 bits looks at: below 2^-14, where it may not, all values round to 0
+        if (byte >= 127 - 15 && byte <= 127 + 14) {
+            const __half2 inv = __float2half2_rn(inv_scale(byte));
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const __half2 a = *reinterpret_cast<const __half2*>(&w[2 * i]);
+                const __half2 b = *reinterpret_cast<const __half2*>(&w[2 * i + 1]);
+                if constexpr (KIND == kE4M3) {
+                    const __half2 x = __hmul2_rn(a, inv), y = __hmul2_rn(b, inv);
+                    uint16_t lo, hi;
+                    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;"
+                        : "=h"(lo)
+                        : "r"(*reinterpret_cast<const uint32_t*>(&x)));
+                    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;"
+                        : "=h"(hi)
+                        : "r"(*reinterpret_cast<const uint32_t*>(&y)));
+                    o[i] = pack16(lo, hi);
+                } else {
+                    // 1536 + x * 2^-k rounds once, to a whole number; its low byte is
+                    // the integer's two's complement
+                    const __half2 magic = __float2half2_rn(1536.0f);
+                    const __half2 x = __hfma2(a, inv, magic), y = __hfma2(b, inv, magic);
+                    o[i] = __byte_perm(*reinterpret_cast<const uint32_t*>(&x),
+                                       *reinterpret_cast<const uint32_t*>(&y), 0x6420);
+                }
+            }
+            return;
+        }
+    }
+    const float inv = inv_scale(byte);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        float v[4];
+        widen2(w[2 * i], v[0], v[1], T());
+        widen2(w[2 * i + 1], v[2], v[3], T());
+        o[i] = byte == kActBad ? 0u : quant4<KIND>(v, inv);
+    }
+}
+
 // ------------------------------------------------------------ pairs of FP32
 // One instruction for two products or sums, each rounded as the single one is.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
@@ -336,6 +398,13 @@ __device__ __forceinline__ uint64_t pair(float a, float b) {
 }
 __device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pair(a, a); }
+__device__ __forceinline__ uint64_t neg2(uint64_t v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ float sum2(uint64_t v) {
+    float a, b;
+    unpair(v, a, b);
+    return __fadd_rn(a, b);
 }
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     uint64_t r;

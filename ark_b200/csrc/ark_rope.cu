@@ -76,71 +76,179 @@ __device__ __forceinline__ int64_t position(const Args& a, uint64_t t) {
                    : (int64_t) static_cast<const int*>(a.pos)[t];
 }
 
-// cos and sin (times the plan's gain) of `pairs` from the first on, at position p
-template <int N>
-__device__ __forceinline__ void angles(const Args& a, const uint64_t* turns, int64_t p, float2* cs) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        // the top 32 bits of the turn, signed: [-1/2, 1/2) of a turn
-        const int32_t top = (int32_t)(((uint64_t)p * turns[i]) >> 32);
-        float s, c;
-        sincospif(__fmul_rn((float)top, 4.656612873077392578125e-10f), &s, &c);
-        if (a.inverse) s = -s;
-        cs[i] = make_float2(__fmul_rn(c, a.plan.gain), __fmul_rn(s, a.plan.gain));
-    }
-}
+// ------------------------------------------------------------ a lane's part of a head
+// A unit is two chunks of VEC elements: VEC pairs of FP32 for the packed
+// instructions, the first chunk's in front (VEC = 1: one pair, the two chunks).
 
-// the two chunks of unit u: where they start and whether they are there
+// where unit u's chunks start and whether they are there
+struct Unit {
+    uint32_t o1, o2, at;   // at: first rotated pair
+    bool h1, h2, turned;
+};
 template <int VEC>
-__device__ __forceinline__ void chunks(const Deal& d, uint32_t u, uint32_t& o1, uint32_t& o2,
-                                       bool& h1, bool& h2, bool& turned) {
-    turned = u < d.rot_units;
-    if (turned && !d.interleaved) {
-        o1 = u * VEC;
-        o2 = d.half + u * VEC;
+__device__ __forceinline__ Unit unit_of(const Deal& d, uint32_t u) {
+    Unit r;
+    r.turned = u < d.rot_units;
+    r.at = u * VEC;
+    if (r.turned && !d.interleaved) {
+        r.o1 = u * VEC;
+        r.o2 = d.half + u * VEC;
     } else {
-        o1 = turned ? u * 2 * VEC : d.rot + (u - d.rot_units) * 2 * VEC;
-        o2 = o1 + VEC;
+        r.o1 = r.turned ? u * 2 * VEC : d.rot + (u - d.rot_units) * 2 * VEC;
+        r.o2 = r.o1 + VEC;
     }
-    h1 = u < d.units && o1 < d.dim;
-    h2 = u < d.units && o2 < d.dim;
+    r.h1 = u < d.units && r.o1 < d.dim;
+    r.h2 = u < d.units && r.o2 < d.dim;
+    return r;
 }
 
-template <int VEC, class T>
-__device__ __forceinline__ void load_chunk(const T* p, bool there, float* v) {
+// the elements as they lie in memory: VEC of each chunk
+template <class T, int VEC>
+struct Raw {   // 16-bit types
+    static constexpr int N = VEC == 1 ? 1 : VEC / 2;
+    uint32_t w[2 * N];
+    __device__ __forceinline__ void load(const T* p, const Unit& u, bool on) {
+        if constexpr (VEC == 1) {
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+            w[0] = on && u.h1 ? q[u.o1] : 0;
+            w[1] = on && u.h2 ? q[u.o2] : 0;
+        } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
-    if (!there) return;
-    if constexpr (VEC == 1)
-        v[0] = Elem<T>::to_f(*p);
-    else
-        load_vec<VEC>(p, v);
-}
-template <int VEC, class T>
-__device__ __forceinline__ void store_chunk(T* p, bool there, const float* v) {
-    if (!there) return;
-    if constexpr (VEC == 1)
-        *p = Elem<T>::from_f(v[0]);
-    else
-        store_vec<VEC>(p, v);
-}
-
-// rotate the pairs of a unit in place: x holds chunk 1 then chunk 2
+            for (int i = 0; i < 2 * N; ++i) w[i] = 0;
+            if (on && u.h1) part(p + u.o1, w);
+            if (on && u.h2) part(p + u.o2, w + N);
+        }
+    }
+    static __device__ __forceinline__ void part(const T* p, uint32_t* w) {
+        if constexpr (VEC == 8) {
+            const uint4 q = *reinterpret_cast<const uint4*>(p);
+            w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            w[0] = q.x, w[1] = q.y;
+        }
+    }
+    __device__ __forceinline__ void get(uint64_t* v) const {
+        if constexpr (VEC == 1) {
+            float a, b, none;
+            widen2(w[0], a, none, T());
+            widen2(w[1], b, none, T());
+            v[0] = pair(a, b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float a, b;
+                widen2(w[i], a, b, T());
+                v[i] = pair(a, b);
+            }
+        }
+    }
+    static __device__ __forceinline__ void put(T* p, const Unit& u, bool on, const uint64_t* v) {
+        float a, b;
+        if constexpr (VEC == 1) {
+            unpair(v[0], a, b);
+            if (on && u.h1) p[u.o1] = Elem<T>::from_f(a);
+            if (on && u.h2) p[u.o2] = Elem<T>::from_f(b);
+        } else {
+            uint32_t w[2 * N];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                unpair(v[i], a, b);
+                w[i] = narrow2(a, b, T());
+            }
+            if constexpr (VEC == 8) {
+                if (on && u.h1) *reinterpret_cast<uint4*>(p + u.o1) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (on && u.h2) *reinterpret_cast<uint4*>(p + u.o2) = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+                if (on && u.h1) *reinterpret_cast<uint2*>(p + u.o1) = make_uint2(w[0], w[1]);
+                if (on && u.h2) *reinterpret_cast<uint2*>(p + u.o2) = make_uint2(w[2], w[3]);
+            }
+        }
+    }
+};
 template <int VEC>
-__device__ __forceinline__ void rotate(const Deal& d, const float2* cs, float* x) {
-    auto turn = [&](int p, int q, float2 c) {
-        const float a = x[p], b = x[q];
-        x[p] = __fmaf_rn(a, c.x, -__fmul_rn(b, c.y));
-        x[q] = __fmaf_rn(b, c.x, __fmul_rn(a, c.y));
-    };
-    if (d.interleaved) {
+struct Raw<float, VEC> {
+    float f[2 * VEC];
+    __device__ __forceinline__ void load(const float* p, const Unit& u, bool on) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) turn(2 * i, 2 * i + 1, cs[i]);
+        for (int i = 0; i < 2 * VEC; ++i) f[i] = 0.0f;
+        if constexpr (VEC == 1) {
+            if (on && u.h1) f[0] = p[u.o1];
+            if (on && u.h2) f[1] = p[u.o2];
+        } else {
+            if (on && u.h1) load_vec<VEC>(p + u.o1, f);
+            if (on && u.h2) load_vec<VEC>(p + u.o2, f + VEC);
+        }
+    }
+    __device__ __forceinline__ void get(uint64_t* v) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
+    }
+    static __device__ __forceinline__ void put(float* p, const Unit& u, bool on, const uint64_t* v) {
+        float f[2 * VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) unpair(v[i], f[2 * i], f[2 * i + 1]);
+        if constexpr (VEC == 1) {
+            if (on && u.h1) p[u.o1] = f[0];
+            if (on && u.h2) p[u.o2] = f[1];
+        } else {
+            if (on && u.h1) store_vec<VEC>(p + u.o1, f);
+            if (on && u.h2) store_vec<VEC>(p + u.o2, f + VEC);
+        }
+    }
+};
+
+// FP32 of shared memory (zero where the head ends) as a unit's pairs
+template <int VEC>
+__device__ __forceinline__ void unit_floats(const float* p, const Unit& u, uint64_t* v) {
+    if constexpr (VEC == 1) {
+        v[0] = pair(u.h1 ? p[u.o1] : 0.0f, u.h2 ? p[u.o2] : 0.0f);
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) turn(i, i + VEC, cs[i]);
+        for (int i = 0; i < VEC / 2; i += 2) {
+            const float4 a = u.h1 ? *reinterpret_cast<const float4*>(p + u.o1 + 2 * i) : float4{};
+            const float4 b = u.h2 ? *reinterpret_cast<const float4*>(p + u.o2 + 2 * i) : float4{};
+            v[i] = pair(a.x, a.y), v[i + 1] = pair(a.z, a.w);
+            v[VEC / 2 + i] = pair(b.x, b.y), v[VEC / 2 + i + 1] = pair(b.z, b.w);
+        }
     }
 }
+
+// cos and sin (times the plan's gain) of a unit's VEC rotated pairs
+template <int VEC>
+struct Turn {
+    float c[VEC], s[VEC];
+    __device__ __forceinline__ void set(const Args& a, const uint64_t* turns, int64_t p) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            // the top 32 bits of the turn, signed: [-1/2, 1/2) of a turn
+            const int32_t top = (int32_t)(((uint64_t)p * turns[i]) >> 32);
+            sincospif(__fmul_rn((float)top, 4.656612873077392578125e-10f), &s[i], &c[i]);
+            c[i] = __fmul_rn(c[i], a.plan.gain);
+            s[i] = __fmul_rn(a.inverse ? -s[i] : s[i], a.plan.gain);
+        }
+    }
+    // rotate a unit's pairs in place
+    __device__ __forceinline__ void operator()(const Deal& d, uint64_t* v) const {
+        if (VEC == 1 || d.interleaved) {   // both of a rotated pair in one register pair
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float x, y;
+                unpair(v[i], x, y);
+                v[i] = pair(__fmaf_rn(x, c[i], -__fmul_rn(y, s[i])),
+                            __fmaf_rn(y, c[i], __fmul_rn(x, s[i])));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                const uint64_t x = v[i], y = v[i + VEC / 2];
+                const uint64_t cc = pair(c[2 * i], c[2 * i + 1]), ss = pair(s[2 * i], s[2 * i + 1]);
+                v[i] = fma2(x, cc, neg2(mul2(y, ss)));
+                v[i + VEC / 2] = fma2(y, cc, mul2(x, ss));
+            }
+        }
+    }
+};
 
 __device__ __forceinline__ float group_sum(float v, uint32_t group) {
     for (uint32_t o = group >> 1; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
@@ -148,23 +256,45 @@ __device__ __forceinline__ float group_sum(float v, uint32_t group) {
 }
 
 // Checkpoint the two chunks of 8 of a lane.  A scale block is 4 lanes' chunks
-// of one half (half layout), or both chunks of 2 lanes.
-template <int KIND>
-__device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col, uint32_t o1,
-                                     uint32_t o2, bool there, const float* x) {
-    uint32_t m1 = there ? abs_max<8>(x) : 0, m2 = there ? abs_max<8>(x + 8) : 0;
-    const bool next = o2 == o1 + 8;
-    if (next) m1 = m2 = max(m1, m2);
-    m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, 1));
-    m2 = max(m2, __shfl_xor_sync(0xFFFFFFFFu, m2, 1));
+// of one half (half layout), or both chunks of 2 lanes (then they adjoin).
+template <int KIND, class T>
+__device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col, const Unit& u,
+                                     bool on, const Raw<T, 8>& x) {
+    const bool next = u.o2 == u.o1 + 8;
+    uint32_t m1, m2;
+    auto most = [&](uint32_t a, uint32_t b) {
+        if constexpr (std::is_same<T, float>::value)
+            return max(a, b);
+        else
+            return __vmaxu2(a, b);
+    };
+    if constexpr (std::is_same<T, float>::value) {
+        m1 = abs_max<8>(x.f);
+        m2 = abs_max<8>(x.f + 8);
+    } else {
+        m1 = pairs_max<4>(x.w);
+        m2 = pairs_max<4>(x.w + 4);
+    }
+    if (next) m1 = m2 = most(m1, m2);
+    m1 = most(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, 1));
+    m2 = most(m2, __shfl_xor_sync(0xFFFFFFFFu, m2, 1));
     const uint32_t n1 = __shfl_xor_sync(0xFFFFFFFFu, m1, 2), n2 = __shfl_xor_sync(0xFFFFFFFFu, m2, 2);
-    if (!next) m1 = max(m1, n1), m2 = max(m2, n2);
-    if (!there) return;
-    const uint32_t b1 = scale_byte<KIND>(m1), b2 = scale_byte<KIND>(m2);
-    *reinterpret_cast<uint2*>(data + col + o1) = quant8<KIND>(x, b1);
-    *reinterpret_cast<uint2*>(data + col + o2) = quant8<KIND>(x + 8, b2);
-    if ((o1 & 31u) == 0) scale[(col + o1) >> 5] = (uint8_t)b1;
-    if ((o2 & 31u) == 0) scale[(col + o2) >> 5] = (uint8_t)b2;
+    if (!next) m1 = most(m1, n1), m2 = most(m2, n2);
+    if (!on || !u.h1) return;
+    uint32_t q[4], b1, b2;
+    if constexpr (std::is_same<T, float>::value) {
+        b1 = scale_byte<KIND>(m1), b2 = scale_byte<KIND>(m2);
+        const uint2 a = quant8<KIND>(x.f, b1), b = quant8<KIND>(x.f + 8, b2);
+        q[0] = a.x, q[1] = a.y, q[2] = b.x, q[3] = b.y;
+    } else {
+        b1 = scale_byte<KIND>(pairs_bits(m1, T())), b2 = scale_byte<KIND>(pairs_bits(m2, T()));
+        quant_words<T, KIND, 4>(x.w, b1, q);
+        quant_words<T, KIND, 4>(x.w + 4, b2, q + 2);
+    }
+    *reinterpret_cast<uint2*>(data + col + u.o1) = make_uint2(q[0], q[1]);
+    *reinterpret_cast<uint2*>(data + col + u.o2) = make_uint2(q[2], q[3]);
+    if ((u.o1 & 31u) == 0) scale[(col + u.o1) >> 5] = (uint8_t)b1;
+    if ((u.o2 & 31u) == 0) scale[(col + u.o2) >> 5] = (uint8_t)b2;
 }
 
 // a row's columns behind the last head, up to the pitch
@@ -177,15 +307,33 @@ __device__ __forceinline__ void hold_rest(uint8_t* data, uint8_t* scale, uint64_
     }
 }
 
+// A warp takes as many tasks (a token, a split of its heads) as it has groups;
+// all its lanes take every round, since groups shuffle together.
+struct Task {
+    uint64_t t;
+    uint32_t lo, hi;   // heads
+    int64_t p;         // position
+    bool on, live;
+    __device__ __forceinline__ Task(const Args& a, uint64_t task, uint32_t heads, uint32_t splits) {
+        on = task < a.tokens * splits;
+        t = on ? (splits == 1 ? task : task / splits) : 0;
+        const uint32_t per = (heads + splits - 1) / splits;
+        lo = on ? (uint32_t)(task - t * splits) * per : 0;
+        hi = on ? min(lo + per, heads) : 0;
+        p = on ? position(a, t) : -1;
+        live = p >= 0;
+    }
+};
+
 // ------------------------------------------------------------ forward
 // HOLD: 0 no checkpoint, 1 e4m3, 2 int8.  A padding token's outputs are zero,
 // and so is its checkpoint.
 template <class T, int VEC, int NU, bool NORM, int HOLD>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NU == 1 ? 6 : 4) forward_kernel(const __grid_constant__ Args a) {
     // two heads in flight per lane, where a head is few registers
-    constexpr int kHeads = NU == 1 ? 2 : 1;
+    constexpr int kHeads = NU == 1 && sizeof(T) == 2 ? 2 : 1;
     __shared__ uint64_t turns[kMaxDim / 2];
-    __shared__ float gains[NORM ? 2 * kMaxDim : 1];
+    __shared__ __align__(16) float gains[NORM ? 2 * kMaxDim : 4];
     const Deal& d = a.d;
     for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
     if (NORM)
@@ -196,236 +344,284 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     __syncthreads();
     const uint32_t lane = threadIdx.x & (d.group - 1), in_warp = 32 / d.group;
     const uint32_t hq = (uint32_t)a.q.heads, heads = hq + (uint32_t)a.k.heads;
-    const uint32_t per_split = (heads + a.splits - 1) / a.splits;
     const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
-    uint32_t o1[NU], o2[NU];
-    bool h1[NU], h2[NU], turned[NU];
+    Unit u[NU];
 #pragma unroll
-    for (int n = 0; n < NU; ++n)
-        chunks<VEC>(d, lane + n * d.group, o1[n], o2[n], h1[n], h2[n], turned[n]);
+    for (int n = 0; n < NU; ++n) u[n] = unit_of<VEC>(d, lane + n * d.group);
 
-    // A warp takes as many tasks (a token, a split of its heads) as it has
-    // groups; all its lanes take every round, since groups shuffle together.
     const uint64_t tasks = a.tokens * a.splits;
     const uint64_t stride = (uint64_t)gridDim.x * (kThreads / 32) * in_warp;
     uint64_t first = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * in_warp;
     for (; first < tasks; first += stride) {
-        const uint64_t task = first + (threadIdx.x & 31) / d.group;
-        const bool on = task < tasks;
-        const uint64_t t = on ? task / a.splits : 0;
-        const uint32_t lo = on ? (uint32_t)(task - t * a.splits) * per_split : 0;
-        const uint32_t hi = on ? min(lo + per_split, heads) : 0;
-        const int64_t p = on ? position(a, t) : -1;
-        const bool live = p >= 0;
-        float2 cs[NU][VEC];
+        const Task k(a, first + (threadIdx.x & 31) / d.group, heads, a.splits);
+        Turn<VEC> turn[NU];
 #pragma unroll
         for (int n = 0; n < NU; ++n)
-            if (turned[n] && h1[n]) angles<VEC>(a, turns + (lane + n * d.group) * VEC, p, cs[n]);
-        for (uint32_t step = 0; step < per_split; step += kHeads) {
-            float v[kHeads][NU][2 * VEC];
+            if (u[n].turned && u[n].h1) turn[n].set(a, turns + u[n].at, k.p);
+        // the queries among the task's heads, then the keys
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+            const uint32_t from = part ? max(k.lo, hq) - hq : min(k.lo, hq);
+            const uint32_t to = part ? max(k.hi, hq) - hq : min(k.hi, hq);
+            const uint32_t rounds = __reduce_max_sync(0xFFFFFFFFu, to - from);
+            if (!rounds) continue;
+            const Heads& in = part ? a.k : a.q;
+            const Heads& out = part ? a.ok : a.oq;
+            const T* x = static_cast<const T*>(in.p) + k.t * in.ts + from * in.hs;
+            T* y = static_cast<T*>(out.p) + k.t * out.ts + from * out.hs;
+            const uint64_t pitch = part ? a.pk : a.pq;
+            uint8_t* data = (part ? a.k8 : a.q8) + k.t * pitch;
+            uint8_t* scale = (part ? a.sk : a.sq) + k.t * (pitch >> 5);
+            uint64_t col = (uint64_t)from * d.dim;
+            const float* g = gains + (part ? kMaxDim : 0);
+            for (uint32_t h = 0; h < rounds; h += kHeads) {
+                Raw<T, VEC> raw[kHeads][NU];
 #pragma unroll
-            for (int j = 0; j < kHeads; ++j) {
-                const uint32_t h = lo + step + j;
-                const bool here = h < hi && live;
-                const Heads& in = h < hq ? a.q : a.k;
-                const T* x = static_cast<const T*>(in.p) + t * in.ts + (h < hq ? h : h - hq) * in.hs;
-#pragma unroll
-                for (int n = 0; n < NU; ++n) {
-                    load_chunk<VEC>(x + o1[n], here && h1[n], v[j][n]);
-                    load_chunk<VEC>(x + o2[n], here && h2[n], v[j][n] + VEC);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kHeads; ++j) {
-                const uint32_t h = lo + step + j;
-                const bool here = h < hi, is_q = h < hq;
-                const uint32_t hh = is_q ? h : h - hq;
-                if constexpr (HOLD != 0 && VEC == 8) {
-                    const uint64_t pitch = is_q ? a.pq : a.pk;
-                    hold<HOLD - 1>((is_q ? a.q8 : a.k8) + t * pitch,
-                                   (is_q ? a.sq : a.sk) + t * (pitch >> 5), (uint64_t)hh * d.dim,
-                                   o1[0], o2[0], here && h1[0], v[j][0]);
-                }
-                if (NORM) {
-                    float ss = 0.0f;
+                for (int j = 0; j < kHeads; ++j)
 #pragma unroll
                     for (int n = 0; n < NU; ++n)
+                        raw[j][n].load(x + j * in.hs, u[n], k.live && from + h + j < to);
 #pragma unroll
-                        for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(v[j][n][i], v[j][n][i], ss);
-                    ss = group_sum(ss, d.group);
-                    const float r = rsqrtf(__fmaf_rn(ss, inv_dim, a.eps));
-                    const float* g = gains + (is_q ? 0 : kMaxDim);
+                for (int j = 0; j < kHeads; ++j) {
+                    const bool here = from + h + j < to;
+                    if constexpr (HOLD != 0 && VEC == 8)
+                        hold<HOLD - 1>(data, scale, col, u[0], here, raw[j][0]);
+                    uint64_t v[NU][VEC];
 #pragma unroll
-                    for (int n = 0; n < NU; ++n)
+                    for (int n = 0; n < NU; ++n) raw[j][n].get(v[n]);
+                    if (NORM) {
+                        uint64_t ss = 0;
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            if (h1[n])
-                                v[j][n][i] = __fmul_rn(__fmul_rn(v[j][n][i], r), g[o1[n] + i]);
-                            if (h2[n])
-                                v[j][n][VEC + i] =
-                                    __fmul_rn(__fmul_rn(v[j][n][VEC + i], r), g[o2[n] + i]);
+                        for (int n = 0; n < NU; ++n)
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) ss = fma2(v[n][i], v[n][i], ss);
+                        const float all = group_sum(sum2(ss), d.group);
+                        const uint64_t r = twice(rsqrtf(__fmaf_rn(all, inv_dim, a.eps)));
+#pragma unroll
+                        for (int n = 0; n < NU; ++n) {
+                            uint64_t gain[VEC];
+                            unit_floats<VEC>(g, u[n], gain);
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) v[n][i] = mul2(mul2(v[n][i], r), gain[i]);
                         }
-                }
-                const Heads& out = is_q ? a.oq : a.ok;
-                T* y = static_cast<T*>(out.p) + t * out.ts + hh * out.hs;
-#pragma unroll
-                for (int n = 0; n < NU; ++n) {
-                    if (turned[n]) rotate<VEC>(d, cs[n], v[j][n]);
-                    if (!live) {
-#pragma unroll
-                        for (int i = 0; i < 2 * VEC; ++i) v[j][n][i] = 0.0f;
                     }
-                    store_chunk<VEC>(y + o1[n], here && h1[n], v[j][n]);
-                    store_chunk<VEC>(y + o2[n], here && h2[n], v[j][n] + VEC);
+#pragma unroll
+                    for (int n = 0; n < NU; ++n) {
+                        if (u[n].turned) turn[n](d, v[n]);
+                        if (!k.live) {
+#pragma unroll
+                            for (int i = 0; i < VEC; ++i) v[n][i] = 0;
+                        }
+                        Raw<T, VEC>::put(y, u[n], here, v[n]);
+                    }
+                    x += in.hs;
+                    y += out.hs;
+                    col += d.dim;
                 }
             }
         }
         if constexpr (HOLD != 0 && VEC == 8) {
-            if (on && lo == 0) {
-                hold_rest(a.q8 + t * a.pq, a.sq + t * (a.pq >> 5), a.q.heads * d.dim, a.pq, lane, d.group);
+            if (k.on && k.lo == 0) {
+                hold_rest(a.q8 + k.t * a.pq, a.sq + k.t * (a.pq >> 5), a.q.heads * d.dim, a.pq, lane,
+                          d.group);
                 if (a.k.heads)
-                    hold_rest(a.k8 + t * a.pk, a.sk + t * (a.pk >> 5), a.k.heads * d.dim, a.pk, lane, d.group);
+                    hold_rest(a.k8 + k.t * a.pk, a.sk + k.t * (a.pk >> 5), a.k.heads * d.dim, a.pk, lane,
+                              d.group);
             }
         }
     }
 }
 
 // ------------------------------------------------------------ backward
-template <int VEC, int KIND>
-__device__ __forceinline__ void held_chunk(const uint8_t* data, const uint8_t* scale, uint64_t col,
-                                           bool there, float* v) {
+// A unit's stored bytes as they lie in memory, and its two scale bytes.
+template <int VEC>
+struct Bytes {
+    uint32_t w[VEC == 8 ? 4 : 2];
+    uint32_t s1, s2;
+    __device__ __forceinline__ void load(const uint8_t* data, const uint8_t* scale, uint64_t col,
+                                         const Unit& u, bool on) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
-    if (!there) return;
-    const uint32_t byte = scale[col >> 5];
-    if constexpr (VEC == 8) {
-        dequant8<KIND>(*reinterpret_cast<const uint2*>(data + col), byte, v);
-    } else if constexpr (VEC == 4) {
-        bytes4<KIND>(*reinterpret_cast<const uint32_t*>(data + col), v);
-        const float s = scale_of(byte);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __fmul_rn(v[i], s);
-    } else {
-        float w[4];
-        bytes4<KIND>(data[col], w);
-        v[0] = __fmul_rn(w[0], scale_of(byte));
+        for (int i = 0; i < (VEC == 8 ? 4 : 2); ++i) w[i] = 0;
+        s1 = s2 = 127;
+        if (on && u.h1) {
+            s1 = scale[(col + u.o1) >> 5];
+            if constexpr (VEC == 8) {
+                const uint2 q = *reinterpret_cast<const uint2*>(data + col + u.o1);
+                w[0] = q.x, w[1] = q.y;
+            } else if constexpr (VEC == 4) {
+                w[0] = *reinterpret_cast<const uint32_t*>(data + col + u.o1);
+            } else {
+                w[0] = data[col + u.o1];
+            }
+        }
+        if (on && u.h2) {
+            s2 = scale[(col + u.o2) >> 5];
+            if constexpr (VEC == 8) {
+                const uint2 q = *reinterpret_cast<const uint2*>(data + col + u.o2);
+                w[2] = q.x, w[3] = q.y;
+            } else if constexpr (VEC == 4) {
+                w[1] = *reinterpret_cast<const uint32_t*>(data + col + u.o2);
+            } else {
+                w[1] = data[col + u.o2];
+            }
+        }
     }
-}
+    template <int KIND>
+    __device__ __forceinline__ void get(uint64_t* v) const {
+        const uint64_t f1 = twice(scale_of(s1)), f2 = twice(scale_of(s2));
+        float b[4];
+        if constexpr (VEC == 1) {
+            float c[4];
+            bytes4<KIND>(w[0], b);
+            bytes4<KIND>(w[1], c);
+            v[0] = pair(__fmul_rn(b[0], scale_of(s1)), __fmul_rn(c[0], scale_of(s2)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                bytes4<KIND>(w[i], b);
+                const uint64_t f = i < VEC / 4 ? f1 : f2;
+                v[2 * i] = mul2(pair(b[0], b[1]), f);
+                v[2 * i + 1] = mul2(pair(b[2], b[3]), f);
+            }
+        }
+    }
+};
+template <class T, int VEC, int SRC>
+struct Source {   // x as T
+    Raw<T, VEC> r;
+    __device__ __forceinline__ void get(uint64_t* v) const { r.get(v); }
+};
+template <class T, int VEC>
+struct Source<T, VEC, 1> {
+    Bytes<VEC> r;
+    __device__ __forceinline__ void get(uint64_t* v) const { r.template get<kE4M3>(v); }
+};
+template <class T, int VEC>
+struct Source<T, VEC, 2> {
+    Bytes<VEC> r;
+    __device__ __forceinline__ void get(uint64_t* v) const { r.template get<kInt8>(v); }
+};
 
 // The blocks below a.q_blocks take the queries, the others the keys, so that a
 // lane's running gradient belongs to one gain.  Each block leaves its sums in
-// a.partial; gains_kernel adds them in block order.
+// a.partial; gains_kernel adds them in block order.  The next head's loads are
+// issued before a head is worked on.
 // SRC: 0 x as T, 1 e4m3, 2 int8.
 template <class T, int VEC, int NU, int SRC>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
+    backward_kernel(const __grid_constant__ Args a) {
     __shared__ uint64_t turns[kMaxDim / 2];
+    __shared__ __align__(16) float gains[kMaxDim];
     extern __shared__ float sums[];   // at the end [groups][dim]
     const Deal& d = a.d;
-    for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
-    __syncthreads();
     const bool is_q = blockIdx.x < a.q_blocks;
+    const void* gain = is_q ? a.gq : a.gk;
+    for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
+    for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) gains[i] = gain_at(gain, a.gain_type, i);
+    __syncthreads();
     const uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
     const uint32_t blocks = is_q ? a.q_blocks : gridDim.x - a.q_blocks;
-    const Heads in = is_q ? a.q : a.k, out = is_q ? a.oq : a.ok, src = is_q ? a.xq : a.xk;
-    const uint32_t heads = (uint32_t)in.heads;
-    const void* gain = is_q ? a.gq : a.gk;
-    const uint8_t* data = is_q ? a.q8 : a.k8;
-    const uint8_t* scale = is_q ? a.sq : a.sk;
+    const Heads &in = is_q ? a.q : a.k, &out = is_q ? a.oq : a.ok, &src = is_q ? a.xq : a.xk;
+    const uint32_t heads = (uint32_t)in.heads, splits = is_q ? a.q_splits : a.k_splits;
     const uint64_t pitch = is_q ? a.pq : a.pk;
-    const uint32_t splits = is_q ? a.q_splits : a.k_splits, per_split = (heads + splits - 1) / splits;
 
     const uint32_t lane = threadIdx.x & (d.group - 1), in_warp = 32 / d.group;
     const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
-    uint32_t o1[NU], o2[NU];
-    bool h1[NU], h2[NU], turned[NU];
-    float g[NU][2 * VEC], dg[NU][2 * VEC];
+    Unit u[NU];
+    uint64_t dg[NU][VEC];
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
-        chunks<VEC>(d, lane + n * d.group, o1[n], o2[n], h1[n], h2[n], turned[n]);
+        u[n] = unit_of<VEC>(d, lane + n * d.group);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            g[n][i] = h1[n] ? gain_at(gain, a.gain_type, o1[n] + i) : 0.0f;
-            g[n][VEC + i] = h2[n] ? gain_at(gain, a.gain_type, o2[n] + i) : 0.0f;
-            dg[n][i] = dg[n][VEC + i] = 0.0f;
-        }
+        for (int i = 0; i < VEC; ++i) dg[n][i] = 0;
     }
     const uint64_t tasks = a.tokens * splits;
     const uint64_t stride = (uint64_t)blocks * (kThreads / 32) * in_warp;
     uint64_t first = ((uint64_t)block * (kThreads / 32) + (threadIdx.x >> 5)) * in_warp;
     for (; first < tasks; first += stride) {
-        const uint64_t task = first + (threadIdx.x & 31) / d.group;
-        const bool on = task < tasks;
-        const uint64_t t = on ? task / splits : 0;
-        const uint32_t lo = on ? (uint32_t)(task - t * splits) * per_split : 0;
-        const uint32_t hi = on ? min(lo + per_split, heads) : 0;
-        const int64_t p = on ? position(a, t) : -1;
-        const bool live = p >= 0;
-        float2 cs[NU][VEC];
-#pragma unroll
-        for (int n = 0; n < NU; ++n)
-            if (turned[n] && h1[n]) angles<VEC>(a, turns + (lane + n * d.group) * VEC, p, cs[n]);
-        for (uint32_t step = 0; step < per_split; ++step) {
-            const uint32_t h = lo + step;
-            const bool here = h < hi, read = here && live;
-            const T* dy = static_cast<const T*>(in.p) + t * in.ts + h * in.hs;
-            float u[NU][2 * VEC], x[NU][2 * VEC];
+        const Task k(a, first + (threadIdx.x & 31) / d.group, heads, splits);
+        const uint32_t count = k.hi - k.lo, rounds = __reduce_max_sync(0xFFFFFFFFu, count);
+        const T* dy = static_cast<const T*>(in.p) + k.t * in.ts + k.lo * in.hs;
+        const T* xp = static_cast<const T*>(src.p) + k.t * src.ts + k.lo * src.hs;
+        const uint8_t* data = (is_q ? a.q8 : a.k8) + k.t * pitch;
+        const uint8_t* scale = (is_q ? a.sq : a.sk) + k.t * (pitch >> 5);
+        uint64_t col = (uint64_t)k.lo * d.dim;
+        T* dx = static_cast<T*>(out.p) + k.t * out.ts + k.lo * out.hs;
+        Raw<T, VEC> g0[NU];
+        Source<T, VEC, SRC> x0[NU];
+        auto load = [&](uint32_t h) {
+            const bool read = k.live && h < count;
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
-                load_chunk<VEC>(dy + o1[n], read && h1[n], u[n]);
-                load_chunk<VEC>(dy + o2[n], read && h2[n], u[n] + VEC);
-                if constexpr (SRC == 0) {
-                    const T* xp = static_cast<const T*>(src.p) + t * src.ts + h * src.hs;
-                    load_chunk<VEC>(xp + o1[n], read && h1[n], x[n]);
-                    load_chunk<VEC>(xp + o2[n], read && h2[n], x[n] + VEC);
-                } else {
-                    const uint8_t* row = data + t * pitch;
-                    const uint8_t* srow = scale + t * (pitch >> 5);
-                    const uint64_t col = (uint64_t)h * d.dim;
-                    held_chunk<VEC, SRC - 1>(row, srow, col + o1[n], read && h1[n], x[n]);
-                    held_chunk<VEC, SRC - 1>(row, srow, col + o2[n], read && h2[n], x[n] + VEC);
-                }
+                g0[n].load(dy, u[n], read);
+                if constexpr (SRC == 0)
+                    x0[n].r.load(xp, u[n], read);
+                else
+                    x0[n].r.load(data, scale, col, u[n], read);
             }
-            float ss = 0.0f;
+            dy += in.hs;
+            if (SRC == 0) xp += src.hs;
+            col += d.dim;
+        };
+        load(0);
+        Turn<VEC> turn[NU];
+#pragma unroll
+        for (int n = 0; n < NU; ++n)
+            if (u[n].turned && u[n].h1) turn[n].set(a, turns + u[n].at, k.p);
+        for (uint32_t h = 0; h < rounds; ++h) {
+            const bool here = h < count, read = here && k.live;
+            uint64_t v[NU][VEC], x[NU][VEC];
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+                g0[n].get(v[n]);
+                x0[n].get(x[n]);
+            }
+            load(h + 1);
+            uint64_t ss = 0;
 #pragma unroll
             for (int n = 0; n < NU; ++n)
 #pragma unroll
-                for (int i = 0; i < 2 * VEC; ++i) ss = __fmaf_rn(x[n][i], x[n][i], ss);
-            ss = group_sum(ss, d.group);
+                for (int i = 0; i < VEC; ++i) ss = fma2(x[n][i], x[n][i], ss);
+            const float all = group_sum(sum2(ss), d.group);
             // nothing of a padding token may reach the sums, not even 0 * rsqrt(0)
-            const float r = read ? rsqrtf(__fmaf_rn(ss, inv_dim, a.eps)) : 0.0f;
-            float dot = 0.0f;
+            const uint64_t r = twice(read ? rsqrtf(__fmaf_rn(all, inv_dim, a.eps)) : 0.0f);
+            uint64_t dot2 = 0;
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
-                if (turned[n] && read) rotate<VEC>(d, cs[n], u[n]);
+                if (u[n].turned && read) turn[n](d, v[n]);
+                uint64_t g[VEC];
+                unit_floats<VEC>(gains, u[n], g);
 #pragma unroll
-                for (int i = 0; i < 2 * VEC; ++i) {
-                    x[n][i] = __fmul_rn(x[n][i], r);
-                    dg[n][i] = __fmaf_rn(u[n][i], x[n][i], dg[n][i]);
-                    u[n][i] = __fmul_rn(u[n][i], g[n][i]);
-                    dot = __fmaf_rn(u[n][i], x[n][i], dot);
+                for (int i = 0; i < VEC; ++i) {
+                    x[n][i] = mul2(x[n][i], r);
+                    dg[n][i] = fma2(v[n][i], x[n][i], dg[n][i]);
+                    v[n][i] = mul2(v[n][i], g[i]);
+                    dot2 = fma2(v[n][i], x[n][i], dot2);
                 }
             }
-            dot = __fmul_rn(group_sum(dot, d.group), inv_dim);
-            T* dx = static_cast<T*>(out.p) + t * out.ts + h * out.hs;
+            const uint64_t dot = twice(-__fmul_rn(group_sum(sum2(dot2), d.group), inv_dim));
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
 #pragma unroll
-                for (int i = 0; i < 2 * VEC; ++i)
-                    u[n][i] = __fmul_rn(__fmaf_rn(-x[n][i], dot, u[n][i]), r);
-                store_chunk<VEC>(dx + o1[n], here && h1[n], u[n]);
-                store_chunk<VEC>(dx + o2[n], here && h2[n], u[n] + VEC);
+                for (int i = 0; i < VEC; ++i) v[n][i] = mul2(fma2(x[n][i], dot, v[n][i]), r);
+                Raw<T, VEC>::put(dx, u[n], here, v[n]);
             }
+            dx += out.hs;
         }
     }
     // the groups' sums, added in group order
     const uint32_t mine = threadIdx.x / d.group, groups = kThreads / d.group;
 #pragma unroll
-    for (int n = 0; n < NU; ++n)
+    for (int n = 0; n < NU; ++n) {
+        float f[2 * VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) unpair(dg[n][i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            if (h1[n]) sums[mine * d.dim + o1[n] + i] = dg[n][i];
-            if (h2[n]) sums[mine * d.dim + o2[n] + i] = dg[n][VEC + i];
+            if (u[n].h1) sums[mine * d.dim + u[n].o1 + i] = f[i];
+            if (u[n].h2) sums[mine * d.dim + u[n].o2 + i] = f[VEC + i];
         }
+    }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) {
         float s = 0.0f;
