@@ -329,6 +329,34 @@ __device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uin
     }
 }
 
+// ------------------------------------------------------------ pairs of FP32
+// One instruction for two products or sums, each rounded as the single one is.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pair(a, a); }
+__device__ __forceinline__ uint64_t neg2(uint64_t v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ float sum2(uint64_t v) {
+    float a, b;
+    unpair(v, a, b);
+    return __fadd_rn(a, b);
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // ------------------------------------------------------------ 16-bit values to bytes
 // The largest magnitudes of N words' low and high halves.
 template <int N>
@@ -379,42 +407,33 @@ __device__ __forceinline__ void quant_words(const uint32_t* w, uint32_t byte, ui
             return;
         }
     }
-    const float inv = inv_scale(byte);
+    if (byte == kActBad) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) o[i] = 0;
+        return;
+    }
+    const uint64_t inv = twice(inv_scale(byte));
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-        float v[4];
-        widen2(w[2 * i], v[0], v[1], T());
-        widen2(w[2 * i + 1], v[2], v[3], T());
-        o[i] = byte == kActBad ? 0u : quant4<KIND>(v, inv);
+        float a, b, c, d;
+        widen2(w[2 * i], a, b, T());
+        widen2(w[2 * i + 1], c, d, T());
+        if constexpr (KIND == kE4M3) {
+            unpair(mul2(pair(a, b), inv), a, b);
+            unpair(mul2(pair(c, d), inv), c, d);
+            uint16_t lo, hi;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+            o[i] = pack16(lo, hi);
+        } else {
+            // as quant4, the product exact and the sum rounded once
+            const uint64_t magic = twice(12582912.0f);
+            unpair(fma2(pair(a, b), inv, magic), a, b);
+            unpair(fma2(pair(c, d), inv, magic), c, d);
+            o[i] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                               __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+        }
     }
-}
-
-// ------------------------------------------------------------ pairs of FP32
-// One instruction for two products or sums, each rounded as the single one is.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t twice(float a) { return pair(a, a); }
-__device__ __forceinline__ uint64_t neg2(uint64_t v) { return v ^ 0x8000000080000000ull; }
-__device__ __forceinline__ float sum2(uint64_t v) {
-    float a, b;
-    unpair(v, a, b);
-    return __fadd_rn(a, b);
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
 }
 
 // ------------------------------------------------------------ host checks

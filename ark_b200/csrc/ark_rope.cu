@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMaxDim = ARK_ROPE_MAX_DIM;
+constexpr int kBlocksPerSm = 6;
 
 struct Heads {
     void* p;
@@ -307,29 +308,38 @@ __device__ __forceinline__ void hold_rest(uint8_t* data, uint8_t* scale, uint64_
     }
 }
 
-// A warp takes as many tasks (a token, a split of its heads) as it has groups;
-// all its lanes take every round, since groups shuffle together.
+// What a group of lanes does at a time: a token, a split of its heads.  The groups
+// of a warp take neighbouring tokens and the same split, so that they go through
+// queries and keys together; all its lanes take every round, since groups shuffle
+// together.
 struct Task {
     uint64_t t;
     uint32_t lo, hi;   // heads
     int64_t p;         // position
     bool on, live;
-    __device__ __forceinline__ Task(const Args& a, uint64_t task, uint32_t heads, uint32_t splits) {
-        on = task < a.tokens * splits;
-        t = on ? (splits == 1 ? task : task / splits) : 0;
+    __device__ __forceinline__ Task(const Args& a, uint64_t warp, uint32_t heads, uint32_t splits) {
+        const uint64_t block = splits == 1 ? warp : warp / splits;
+        const uint32_t split = (uint32_t)(warp - block * splits);
+        t = block * (32 / a.d.group) + (threadIdx.x & 31) / a.d.group;
+        on = t < a.tokens;
+        if (!on) t = 0;
         const uint32_t per = (heads + splits - 1) / splits;
-        lo = on ? (uint32_t)(task - t * splits) * per : 0;
+        lo = on ? min(split * per, heads) : 0;
         hi = on ? min(lo + per, heads) : 0;
         p = on ? position(a, t) : -1;
         live = p >= 0;
     }
 };
+__device__ __forceinline__ uint64_t warp_tasks(const Args& a, uint32_t splits) {
+    const uint32_t in_warp = 32 / a.d.group;
+    return (a.tokens + in_warp - 1) / in_warp * splits;
+}
 
 // ------------------------------------------------------------ forward
 // HOLD: 0 no checkpoint, 1 e4m3, 2 int8.  A padding token's outputs are zero,
 // and so is its checkpoint.
 template <class T, int VEC, int NU, bool NORM, int HOLD>
-__global__ void __launch_bounds__(kThreads, NU == 1 ? 6 : 4) forward_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_kernel(const __grid_constant__ Args a) {
     // two heads in flight per lane, where a head is few registers
     constexpr int kHeads = NU == 1 && sizeof(T) == 2 ? 2 : 1;
     __shared__ uint64_t turns[kMaxDim / 2];
@@ -342,18 +352,16 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? 6 : 4) forward_kernel(cons
             gains[kMaxDim + i] = a.k.heads ? gain_at(a.gk, a.gain_type, i) : 0.0f;
         }
     __syncthreads();
-    const uint32_t lane = threadIdx.x & (d.group - 1), in_warp = 32 / d.group;
+    const uint32_t lane = threadIdx.x & (d.group - 1);
     const uint32_t hq = (uint32_t)a.q.heads, heads = hq + (uint32_t)a.k.heads;
     const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
     Unit u[NU];
 #pragma unroll
     for (int n = 0; n < NU; ++n) u[n] = unit_of<VEC>(d, lane + n * d.group);
 
-    const uint64_t tasks = a.tokens * a.splits;
-    const uint64_t stride = (uint64_t)gridDim.x * (kThreads / 32) * in_warp;
-    uint64_t first = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * in_warp;
-    for (; first < tasks; first += stride) {
-        const Task k(a, first + (threadIdx.x & 31) / d.group, heads, a.splits);
+    const uint64_t tasks = warp_tasks(a, a.splits), stride = (uint64_t)gridDim.x * (kThreads / 32);
+    for (uint64_t w = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < tasks; w += stride) {
+        const Task k(a, w, heads, a.splits);
         Turn<VEC> turn[NU];
 #pragma unroll
         for (int n = 0; n < NU; ++n)
@@ -525,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
     const uint32_t heads = (uint32_t)in.heads, splits = is_q ? a.q_splits : a.k_splits;
     const uint64_t pitch = is_q ? a.pq : a.pk;
 
-    const uint32_t lane = threadIdx.x & (d.group - 1), in_warp = 32 / d.group;
+    const uint32_t lane = threadIdx.x & (d.group - 1);
     const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
     Unit u[NU];
     uint64_t dg[NU][VEC];
@@ -535,11 +543,9 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dg[n][i] = 0;
     }
-    const uint64_t tasks = a.tokens * splits;
-    const uint64_t stride = (uint64_t)blocks * (kThreads / 32) * in_warp;
-    uint64_t first = ((uint64_t)block * (kThreads / 32) + (threadIdx.x >> 5)) * in_warp;
-    for (; first < tasks; first += stride) {
-        const Task k(a, first + (threadIdx.x & 31) / d.group, heads, splits);
+    const uint64_t tasks = warp_tasks(a, splits), stride = (uint64_t)blocks * (kThreads / 32);
+    for (uint64_t w = (uint64_t)block * (kThreads / 32) + (threadIdx.x >> 5); w < tasks; w += stride) {
+        const Task k(a, w, heads, splits);
         const uint32_t count = k.hi - k.lo, rounds = __reduce_max_sync(0xFFFFFFFFu, count);
         const T* dy = static_cast<const T*>(in.p) + k.t * in.ts + k.lo * in.hs;
         const T* xp = static_cast<const T*>(src.p) + k.t * src.ts + k.lo * src.hs;
@@ -734,25 +740,30 @@ int common_ok(const Args& a, uint64_t e, uint64_t dim, int pos_type) {
     return rc;
 }
 
-// Groups that share a token's heads: one, unless that leaves an SM with fewer
-// than 16 warps; then up to one per head.
+// Groups that share a token's heads.  More of them level the SMs' loads, and each
+// forms the token's angles again, which costs as much as one to two heads: three
+// tasks for each group that fits, as long as a task keeps 8 heads; with fewer
+// tokens than that, as many as fill the device, down to one head.
 uint32_t splits_of(uint64_t tokens, uint64_t heads, uint32_t group) {
-    const uint64_t want = (uint64_t)sm_count() * 16 * (32 / group);
-    if (heads < 2 || tokens >= want) return 1;
-    const uint64_t n = (want + tokens - 1) / tokens;
-    return (uint32_t)(n < heads ? n : heads);
+    const uint64_t fit = (uint64_t)sm_count() * kBlocksPerSm * (kThreads / group);
+    uint64_t n = (3 * fit + tokens - 1) / tokens;
+    if (n > heads / 8) n = heads / 8;
+    const uint64_t fill = fit / tokens;   // without a second round
+    if (n < fill) n = fill < heads ? fill : heads;
+    return (uint32_t)(n ? n : 1);
 }
 
-// blocks that `tasks` groups of lanes fill, at most `most`
-uint32_t blocks_of(uint64_t tasks, uint32_t group, uint64_t most) {
-    const uint64_t per = kThreads / group, need = (tasks + per - 1) / per;
+// blocks that the tokens' tasks fill, at most `most`
+uint32_t blocks_of(uint64_t tokens, uint32_t splits, uint32_t group, uint64_t most) {
+    const uint64_t in_warp = 32 / group, warps = (tokens + in_warp - 1) / in_warp * splits;
+    const uint64_t need = (warps + kThreads / 32 - 1) / (kThreads / 32);
     return (uint32_t)(need < most ? need : most);
 }
 
 template <class T, int VEC, int NU, bool NORM, int HOLD>
 int forward_t(Args& a, cudaStream_t s) {
     a.splits = splits_of(a.tokens, a.q.heads + a.k.heads, a.d.group);
-    const uint32_t grid = blocks_of(a.tokens * a.splits, a.d.group, (uint64_t)sm_count() * 16);
+    const uint32_t grid = blocks_of(a.tokens, a.splits, a.d.group, (uint64_t)sm_count() * 16);
     forward_kernel<T, VEC, NU, NORM, HOLD><<<grid, kThreads, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
@@ -789,8 +800,8 @@ uint32_t back_blocks(Args& a) {
     uint64_t bq = hq ? most * hq / (hq + hk) : 0, bk = hk ? most - bq : 0;
     if (hq && !bq) bq = 1;
     if (hk && !bk) bk = 1;
-    a.q_blocks = hq ? blocks_of(tokens * a.q_splits, a.d.group, bq) : 0;
-    return a.q_blocks + (hk ? blocks_of(tokens * a.k_splits, a.d.group, bk) : 0);
+    a.q_blocks = hq ? blocks_of(tokens, a.q_splits, a.d.group, bq) : 0;
+    return a.q_blocks + (hk ? blocks_of(tokens, a.k_splits, a.d.group, bk) : 0);
 }
 
 void fill_positions(Args& a, const void* positions, int32_t type, uint64_t seq) {
