@@ -82,24 +82,35 @@ __device__ __forceinline__ int64_t position(const Args& a, uint64_t t) {
 // instructions, the first chunk's in front (VEC = 1: one pair, the two chunks).
 
 // where unit u's chunks start and whether they are there
+template <bool FULL>
 struct Unit {
     uint32_t o1, o2, at;   // at: first rotated pair
     bool h1, h2, turned;
 };
-template <int VEC>
-__device__ __forceinline__ Unit unit_of(const Deal& d, uint32_t u) {
-    Unit r;
-    r.turned = u < d.rot_units;
+template <>
+struct Unit<true> {        // the whole head is rotated, and no lane is without a unit
+    uint32_t o1, o2, at;
+    static constexpr bool h1 = true, h2 = true, turned = true;
+};
+template <int VEC, int G>
+__device__ __forceinline__ Unit<(G > 0)> unit_of(const Deal& d, uint32_t u) {
+    Unit<(G > 0)> r;
     r.at = u * VEC;
-    if (r.turned && !d.interleaved) {
-        r.o1 = u * VEC;
-        r.o2 = d.half + u * VEC;
+    if constexpr (G > 0) {
+        r.o1 = d.interleaved ? u * 2 * VEC : u * VEC;
+        r.o2 = d.interleaved ? r.o1 + VEC : G * VEC + u * VEC;
     } else {
-        r.o1 = r.turned ? u * 2 * VEC : d.rot + (u - d.rot_units) * 2 * VEC;
-        r.o2 = r.o1 + VEC;
+        r.turned = u < d.rot_units;
+        if (r.turned && !d.interleaved) {
+            r.o1 = u * VEC;
+            r.o2 = d.half + u * VEC;
+        } else {
+            r.o1 = r.turned ? u * 2 * VEC : d.rot + (u - d.rot_units) * 2 * VEC;
+            r.o2 = r.o1 + VEC;
+        }
+        r.h1 = u < d.units && r.o1 < d.dim;
+        r.h2 = u < d.units && r.o2 < d.dim;
     }
-    r.h1 = u < d.units && r.o1 < d.dim;
-    r.h2 = u < d.units && r.o2 < d.dim;
     return r;
 }
 
@@ -108,7 +119,8 @@ template <class T, int VEC>
 struct Raw {   // 16-bit types
     static constexpr int N = VEC == 1 ? 1 : VEC / 2;
     uint32_t w[2 * N];
-    __device__ __forceinline__ void load(const T* p, const Unit& u, bool on) {
+    template <class U>
+    __device__ __forceinline__ void load(const T* p, const U& u, bool on) {
         if constexpr (VEC == 1) {
             const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
             w[0] = on && u.h1 ? q[u.o1] : 0;
@@ -124,9 +136,11 @@ struct Raw {   // 16-bit types
         if constexpr (VEC == 8) {
             const uint4 q = *reinterpret_cast<const uint4*>(p);
             w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
-        } else {
+        } else if constexpr (VEC == 4) {
             const uint2 q = *reinterpret_cast<const uint2*>(p);
             w[0] = q.x, w[1] = q.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
     }
     __device__ __forceinline__ void get(uint64_t* v) const {
@@ -144,7 +158,8 @@ struct Raw {   // 16-bit types
             }
         }
     }
-    static __device__ __forceinline__ void put(T* p, const Unit& u, bool on, const uint64_t* v) {
+    template <class U>
+    static __device__ __forceinline__ void put(T* p, const U& u, bool on, const uint64_t* v) {
         float a, b;
         if constexpr (VEC == 1) {
             unpair(v[0], a, b);
@@ -160,9 +175,12 @@ struct Raw {   // 16-bit types
             if constexpr (VEC == 8) {
                 if (on && u.h1) *reinterpret_cast<uint4*>(p + u.o1) = make_uint4(w[0], w[1], w[2], w[3]);
                 if (on && u.h2) *reinterpret_cast<uint4*>(p + u.o2) = make_uint4(w[4], w[5], w[6], w[7]);
-            } else {
+            } else if constexpr (VEC == 4) {
                 if (on && u.h1) *reinterpret_cast<uint2*>(p + u.o1) = make_uint2(w[0], w[1]);
                 if (on && u.h2) *reinterpret_cast<uint2*>(p + u.o2) = make_uint2(w[2], w[3]);
+            } else {
+                if (on && u.h1) *reinterpret_cast<uint32_t*>(p + u.o1) = w[0];
+                if (on && u.h2) *reinterpret_cast<uint32_t*>(p + u.o2) = w[1];
             }
         }
     }
@@ -170,12 +188,16 @@ struct Raw {   // 16-bit types
 template <int VEC>
 struct Raw<float, VEC> {
     float f[2 * VEC];
-    __device__ __forceinline__ void load(const float* p, const Unit& u, bool on) {
+    template <class U>
+    __device__ __forceinline__ void load(const float* p, const U& u, bool on) {
 #pragma unroll
         for (int i = 0; i < 2 * VEC; ++i) f[i] = 0.0f;
-        if constexpr (VEC == 1) {
-            if (on && u.h1) f[0] = p[u.o1];
-            if (on && u.h2) f[1] = p[u.o2];
+        if constexpr (VEC <= 2) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if (on && u.h1) f[i] = p[u.o1 + i];
+                if (on && u.h2) f[VEC + i] = p[u.o2 + i];
+            }
         } else {
             if (on && u.h1) load_vec<VEC>(p + u.o1, f);
             if (on && u.h2) load_vec<VEC>(p + u.o2, f + VEC);
@@ -185,13 +207,17 @@ struct Raw<float, VEC> {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = pair(f[2 * i], f[2 * i + 1]);
     }
-    static __device__ __forceinline__ void put(float* p, const Unit& u, bool on, const uint64_t* v) {
+    template <class U>
+    static __device__ __forceinline__ void put(float* p, const U& u, bool on, const uint64_t* v) {
         float f[2 * VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) unpair(v[i], f[2 * i], f[2 * i + 1]);
-        if constexpr (VEC == 1) {
-            if (on && u.h1) p[u.o1] = f[0];
-            if (on && u.h2) p[u.o2] = f[1];
+        if constexpr (VEC <= 2) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if (on && u.h1) p[u.o1 + i] = f[i];
+                if (on && u.h2) p[u.o2 + i] = f[VEC + i];
+            }
         } else {
             if (on && u.h1) store_vec<VEC>(p + u.o1, f);
             if (on && u.h2) store_vec<VEC>(p + u.o2, f + VEC);
@@ -200,10 +226,14 @@ struct Raw<float, VEC> {
 };
 
 // FP32 of shared memory (zero where the head ends) as a unit's pairs
-template <int VEC>
-__device__ __forceinline__ void unit_floats(const float* p, const Unit& u, uint64_t* v) {
+template <int VEC, class U>
+__device__ __forceinline__ void unit_floats(const float* p, const U& u, uint64_t* v) {
     if constexpr (VEC == 1) {
         v[0] = pair(u.h1 ? p[u.o1] : 0.0f, u.h2 ? p[u.o2] : 0.0f);
+    } else if constexpr (VEC == 2) {
+        const float2 a = u.h1 ? *reinterpret_cast<const float2*>(p + u.o1) : float2{};
+        const float2 b = u.h2 ? *reinterpret_cast<const float2*>(p + u.o2) : float2{};
+        v[0] = pair(a.x, a.y), v[1] = pair(b.x, b.y);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC / 2; i += 2) {
@@ -244,51 +274,55 @@ struct Turn {
             for (int i = 0; i < VEC / 2; ++i) {
                 const uint64_t x = v[i], y = v[i + VEC / 2];
                 const uint64_t cc = pair(c[2 * i], c[2 * i + 1]), ss = pair(s[2 * i], s[2 * i + 1]);
-                v[i] = fma2(x, cc, neg2(mul2(y, ss)));
+                v[i] = fma2(y, neg2(ss), mul2(x, cc));
                 v[i + VEC / 2] = fma2(y, cc, mul2(x, ss));
             }
         }
     }
 };
 
+// G: the group's lanes, 0 where they are not known before the launch
+template <int G>
 __device__ __forceinline__ float group_sum(float v, uint32_t group) {
-    for (uint32_t o = group >> 1; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    if constexpr (G > 0) {
+#pragma unroll
+        for (int o = G >> 1; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    } else {
+        for (uint32_t o = group >> 1; o; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    }
     return v;
 }
 
 // Checkpoint the two chunks of 8 of a lane.  A scale block is 4 lanes' chunks
 // of one half (half layout), or both chunks of 2 lanes (then they adjoin).
-template <int KIND, class T>
-__device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col, const Unit& u,
-                                     bool on, const Raw<T, 8>& x) {
+template <int KIND, class T, class U>
+__device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col, const U& u, bool on,
+                                     const Raw<T, 8>& x) {
     const bool next = u.o2 == u.o1 + 8;
-    uint32_t m1, m2;
-    auto most = [&](uint32_t a, uint32_t b) {
-        if constexpr (std::is_same<T, float>::value)
-            return max(a, b);
-        else
-            return __vmaxu2(a, b);
-    };
-    if constexpr (std::is_same<T, float>::value) {
-        m1 = abs_max<8>(x.f);
-        m2 = abs_max<8>(x.f + 8);
-    } else {
-        m1 = pairs_max<4>(x.w);
-        m2 = pairs_max<4>(x.w + 4);
-    }
-    if (next) m1 = m2 = most(m1, m2);
-    m1 = most(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, 1));
-    m2 = most(m2, __shfl_xor_sync(0xFFFFFFFFu, m2, 1));
-    const uint32_t n1 = __shfl_xor_sync(0xFFFFFFFFu, m1, 2), n2 = __shfl_xor_sync(0xFFFFFFFFu, m2, 2);
-    if (!next) m1 = most(m1, n1), m2 = most(m2, n2);
-    if (!on || !u.h1) return;
     uint32_t q[4], b1, b2;
     if constexpr (std::is_same<T, float>::value) {
+        uint32_t m1 = abs_max<8>(x.f), m2 = abs_max<8>(x.f + 8);
+        if (next) m1 = m2 = max(m1, m2);
+        m1 = max(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, 1));
+        m2 = max(m2, __shfl_xor_sync(0xFFFFFFFFu, m2, 1));
+        const uint32_t n1 = __shfl_xor_sync(0xFFFFFFFFu, m1, 2), n2 = __shfl_xor_sync(0xFFFFFFFFu, m2, 2);
+        if (!next) m1 = max(m1, n1), m2 = max(m2, n2);
+        if (!on || !u.h1) return;
         b1 = scale_byte<KIND>(m1), b2 = scale_byte<KIND>(m2);
         const uint2 a = quant8<KIND>(x.f, b1), b = quant8<KIND>(x.f + 8, b2);
         q[0] = a.x, q[1] = a.y, q[2] = b.x, q[3] = b.y;
     } else {
-        b1 = scale_byte<KIND>(pairs_bits(m1, T())), b2 = scale_byte<KIND>(pairs_bits(m2, T()));
+        // the chunks' maxima as the two halves of a word
+        const uint32_t a = pairs_max<4>(x.w), b = pairs_max<4>(x.w + 4);
+        uint32_t m = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+        if (next) m = __vmaxu2(m, __byte_perm(m, m, 0x1032));
+        m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        const uint32_t n = __shfl_xor_sync(0xFFFFFFFFu, m, 2);
+        if (!next) m = __vmaxu2(m, n);
+        if (!on || !u.h1) return;
+        float f1, f2;
+        widen2(m, f1, f2, T());
+        b1 = scale_byte<KIND>(__float_as_uint(f1)), b2 = scale_byte<KIND>(__float_as_uint(f2));
         quant_words<T, KIND, 4>(x.w, b1, q);
         quant_words<T, KIND, 4>(x.w + 4, b2, q + 2);
     }
@@ -317,10 +351,11 @@ struct Task {
     uint32_t lo, hi;   // heads
     int64_t p;         // position
     bool on, live;
-    __device__ __forceinline__ Task(const Args& a, uint64_t warp, uint32_t heads, uint32_t splits) {
+    __device__ __forceinline__ Task(const Args& a, uint32_t group, uint64_t warp, uint32_t heads,
+                                    uint32_t splits) {
         const uint64_t block = splits == 1 ? warp : warp / splits;
         const uint32_t split = (uint32_t)(warp - block * splits);
-        t = block * (32 / a.d.group) + (threadIdx.x & 31) / a.d.group;
+        t = block * (32 / group) + (threadIdx.x & 31) / group;
         on = t < a.tokens;
         if (!on) t = 0;
         const uint32_t per = (heads + splits - 1) / splits;
@@ -338,30 +373,33 @@ __device__ __forceinline__ uint64_t warp_tasks(const Args& a, uint32_t splits) {
 // ------------------------------------------------------------ forward
 // HOLD: 0 no checkpoint, 1 e4m3, 2 int8.  A padding token's outputs are zero,
 // and so is its checkpoint.
-template <class T, int VEC, int NU, bool NORM, int HOLD>
+// G: lanes of a group where the whole head is rotated and 16 G long, else 0: then
+// nothing of a head's shape is known before the launch.
+template <class T, int VEC, int NU, int G, bool NORM, int HOLD>
 __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_kernel(const __grid_constant__ Args a) {
     // two heads in flight per lane, where a head is few registers
     constexpr int kHeads = NU == 1 && sizeof(T) == 2 ? 2 : 1;
     __shared__ uint64_t turns[kMaxDim / 2];
     __shared__ __align__(16) float gains[NORM ? 2 * kMaxDim : 4];
     const Deal& d = a.d;
+    const uint32_t group = G > 0 ? G : d.group, dim = G > 0 ? 2 * VEC * G : d.dim;
     for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
     if (NORM)
-        for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < dim; i += kThreads) {
             gains[i] = gain_at(a.gq, a.gain_type, i);
             gains[kMaxDim + i] = a.k.heads ? gain_at(a.gk, a.gain_type, i) : 0.0f;
         }
     __syncthreads();
-    const uint32_t lane = threadIdx.x & (d.group - 1);
+    const uint32_t lane = threadIdx.x & (group - 1);
     const uint32_t hq = (uint32_t)a.q.heads, heads = hq + (uint32_t)a.k.heads;
-    const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
-    Unit u[NU];
+    const float inv_dim = __fdiv_rn(1.0f, (float)dim);
+    Unit<(G > 0)> u[NU];
 #pragma unroll
-    for (int n = 0; n < NU; ++n) u[n] = unit_of<VEC>(d, lane + n * d.group);
+    for (int n = 0; n < NU; ++n) u[n] = unit_of<VEC, G>(d, lane + n * group);
 
     const uint64_t tasks = warp_tasks(a, a.splits), stride = (uint64_t)gridDim.x * (kThreads / 32);
     for (uint64_t w = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < tasks; w += stride) {
-        const Task k(a, w, heads, a.splits);
+        const Task k(a, group, w, heads, a.splits);
         Turn<VEC> turn[NU];
 #pragma unroll
         for (int n = 0; n < NU; ++n)
@@ -380,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_
             const uint64_t pitch = part ? a.pk : a.pq;
             uint8_t* data = (part ? a.k8 : a.q8) + k.t * pitch;
             uint8_t* scale = (part ? a.sk : a.sq) + k.t * (pitch >> 5);
-            uint64_t col = (uint64_t)from * d.dim;
+            uint64_t col = (uint64_t)from * dim;
             const float* g = gains + (part ? kMaxDim : 0);
             for (uint32_t h = 0; h < rounds; h += kHeads) {
                 Raw<T, VEC> raw[kHeads][NU];
@@ -403,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_
                         for (int n = 0; n < NU; ++n)
 #pragma unroll
                             for (int i = 0; i < VEC; ++i) ss = fma2(v[n][i], v[n][i], ss);
-                        const float all = group_sum(sum2(ss), d.group);
+                        const float all = group_sum<G>(sum2(ss), group);
                         const uint64_t r = twice(rsqrtf(__fmaf_rn(all, inv_dim, a.eps)));
 #pragma unroll
                         for (int n = 0; n < NU; ++n) {
@@ -424,17 +462,17 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_
                     }
                     x += in.hs;
                     y += out.hs;
-                    col += d.dim;
+                    col += dim;
                 }
             }
         }
         if constexpr (HOLD != 0 && VEC == 8) {
             if (k.on && k.lo == 0) {
-                hold_rest(a.q8 + k.t * a.pq, a.sq + k.t * (a.pq >> 5), a.q.heads * d.dim, a.pq, lane,
-                          d.group);
+                hold_rest(a.q8 + k.t * a.pq, a.sq + k.t * (a.pq >> 5), a.q.heads * dim, a.pq, lane,
+                          group);
                 if (a.k.heads)
-                    hold_rest(a.k8 + k.t * a.pk, a.sk + k.t * (a.pk >> 5), a.k.heads * d.dim, a.pk, lane,
-                              d.group);
+                    hold_rest(a.k8 + k.t * a.pk, a.sk + k.t * (a.pk >> 5), a.k.heads * dim, a.pk, lane,
+                              group);
             }
         }
     }
@@ -442,72 +480,85 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_
 
 // ------------------------------------------------------------ backward
 // A unit's stored bytes as they lie in memory, and its two scale bytes.
-template <int VEC>
+template <int VEC, int G>
 struct Bytes {
     uint32_t w[VEC == 8 ? 4 : 2];
     uint32_t s1, s2;
-    __device__ __forceinline__ void load(const uint8_t* data, const uint8_t* scale, uint64_t col,
-                                         const Unit& u, bool on) {
-#pragma unroll
-        for (int i = 0; i < (VEC == 8 ? 4 : 2); ++i) w[i] = 0;
-        s1 = s2 = 127;
-        if (on && u.h1) {
-            s1 = scale[(col + u.o1) >> 5];
-            if constexpr (VEC == 8) {
-                const uint2 q = *reinterpret_cast<const uint2*>(data + col + u.o1);
-                w[0] = q.x, w[1] = q.y;
-            } else if constexpr (VEC == 4) {
-                w[0] = *reinterpret_cast<const uint32_t*>(data + col + u.o1);
-            } else {
-                w[0] = data[col + u.o1];
-            }
-        }
-        if (on && u.h2) {
-            s2 = scale[(col + u.o2) >> 5];
-            if constexpr (VEC == 8) {
-                const uint2 q = *reinterpret_cast<const uint2*>(data + col + u.o2);
-                w[2] = q.x, w[3] = q.y;
-            } else if constexpr (VEC == 4) {
-                w[1] = *reinterpret_cast<const uint32_t*>(data + col + u.o2);
-            } else {
-                w[1] = data[col + u.o2];
-            }
+    static __device__ __forceinline__ void part(const uint8_t* p, uint32_t* w) {
+        if constexpr (VEC == 8) {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            w[0] = q.x, w[1] = q.y;
+        } else if constexpr (VEC == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (VEC == 2) {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        } else {
+            w[0] = *p;
         }
     }
+    template <class U>
+    __device__ __forceinline__ void load(const uint8_t* data, const uint8_t* scale, uint64_t col,
+                                         const U& u, bool on) {
+        constexpr int kHalf = VEC == 8 ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < 2 * kHalf; ++i) w[i] = 0;
+        s1 = s2 = 127;
+        if constexpr (G == 8) {   // the head's four scale bytes are a word
+            if (on) {
+                const uint32_t all = *reinterpret_cast<const uint32_t*>(scale + (col >> 5));
+                s1 = all >> (u.o1 >> 5) * 8 & 255u;
+                s2 = all >> (u.o2 >> 5) * 8 & 255u;
+            }
+        } else {
+            if (on && u.h1) s1 = scale[(col + u.o1) >> 5];
+            if (on && u.h2) s2 = scale[(col + u.o2) >> 5];
+        }
+        if (on && u.h1) part(data + col + u.o1, w);
+        if (on && u.h2) part(data + col + u.o2, w + kHalf);
+    }
+    // the values before scaling, and the chunks' scales
     template <int KIND>
-    __device__ __forceinline__ void get(uint64_t* v) const {
-        const uint64_t f1 = twice(scale_of(s1)), f2 = twice(scale_of(s2));
-        float b[4];
+    __device__ __forceinline__ void get(uint64_t* v, float& f1, float& f2) const {
+        f1 = scale_of(s1), f2 = scale_of(s2);
+        float b[4], c[4];
         if constexpr (VEC == 1) {
-            float c[4];
             bytes4<KIND>(w[0], b);
             bytes4<KIND>(w[1], c);
-            v[0] = pair(__fmul_rn(b[0], scale_of(s1)), __fmul_rn(c[0], scale_of(s2)));
+            v[0] = pair(b[0], c[0]);
+        } else if constexpr (VEC == 2) {
+            bytes4<KIND>(w[0], b);
+            bytes4<KIND>(w[1], c);
+            v[0] = pair(b[0], b[1]), v[1] = pair(c[0], c[1]);
         } else {
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) {
                 bytes4<KIND>(w[i], b);
-                const uint64_t f = i < VEC / 4 ? f1 : f2;
-                v[2 * i] = mul2(pair(b[0], b[1]), f);
-                v[2 * i + 1] = mul2(pair(b[2], b[3]), f);
+                v[2 * i] = pair(b[0], b[1]), v[2 * i + 1] = pair(b[2], b[3]);
             }
         }
     }
 };
-template <class T, int VEC, int SRC>
+template <class T, int VEC, int G, int SRC>
 struct Source {   // x as T
     Raw<T, VEC> r;
-    __device__ __forceinline__ void get(uint64_t* v) const { r.get(v); }
+    __device__ __forceinline__ void get(uint64_t* v, float& f1, float& f2) const {
+        r.get(v);
+        f1 = f2 = 1.0f;
+    }
 };
-template <class T, int VEC>
-struct Source<T, VEC, 1> {
-    Bytes<VEC> r;
-    __device__ __forceinline__ void get(uint64_t* v) const { r.template get<kE4M3>(v); }
+template <class T, int VEC, int G>
+struct Source<T, VEC, G, 1> {
+    Bytes<VEC, G> r;
+    __device__ __forceinline__ void get(uint64_t* v, float& f1, float& f2) const {
+        r.template get<kE4M3>(v, f1, f2);
+    }
 };
-template <class T, int VEC>
-struct Source<T, VEC, 2> {
-    Bytes<VEC> r;
-    __device__ __forceinline__ void get(uint64_t* v) const { r.template get<kInt8>(v); }
+template <class T, int VEC, int G>
+struct Source<T, VEC, G, 2> {
+    Bytes<VEC, G> r;
+    __device__ __forceinline__ void get(uint64_t* v, float& f1, float& f2) const {
+        r.template get<kInt8>(v, f1, f2);
+    }
 };
 
 // The blocks below a.q_blocks take the queries, the others the keys, so that a
@@ -515,17 +566,18 @@ struct Source<T, VEC, 2> {
 // a.partial; gains_kernel adds them in block order.  The next head's loads are
 // issued before a head is worked on.
 // SRC: 0 x as T, 1 e4m3, 2 int8.
-template <class T, int VEC, int NU, int SRC>
+template <class T, int VEC, int NU, int G, int SRC>
 __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
     backward_kernel(const __grid_constant__ Args a) {
     __shared__ uint64_t turns[kMaxDim / 2];
     __shared__ __align__(16) float gains[kMaxDim];
     extern __shared__ float sums[];   // at the end [groups][dim]
     const Deal& d = a.d;
+    const uint32_t group = G > 0 ? G : d.group, dim = G > 0 ? 2 * VEC * G : d.dim;
     const bool is_q = blockIdx.x < a.q_blocks;
     const void* gain = is_q ? a.gq : a.gk;
     for (uint32_t i = threadIdx.x; i < d.half; i += kThreads) turns[i] = a.plan.turns[i];
-    for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) gains[i] = gain_at(gain, a.gain_type, i);
+    for (uint32_t i = threadIdx.x; i < dim; i += kThreads) gains[i] = gain_at(gain, a.gain_type, i);
     __syncthreads();
     const uint32_t block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
     const uint32_t blocks = is_q ? a.q_blocks : gridDim.x - a.q_blocks;
@@ -533,28 +585,28 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
     const uint32_t heads = (uint32_t)in.heads, splits = is_q ? a.q_splits : a.k_splits;
     const uint64_t pitch = is_q ? a.pq : a.pk;
 
-    const uint32_t lane = threadIdx.x & (d.group - 1);
-    const float inv_dim = __fdiv_rn(1.0f, (float)d.dim);
-    Unit u[NU];
+    const uint32_t lane = threadIdx.x & (group - 1);
+    const float inv_dim = __fdiv_rn(1.0f, (float)dim);
+    Unit<(G > 0)> u[NU];
     uint64_t dg[NU][VEC];
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
-        u[n] = unit_of<VEC>(d, lane + n * d.group);
+        u[n] = unit_of<VEC, G>(d, lane + n * group);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dg[n][i] = 0;
     }
     const uint64_t tasks = warp_tasks(a, splits), stride = (uint64_t)blocks * (kThreads / 32);
     for (uint64_t w = (uint64_t)block * (kThreads / 32) + (threadIdx.x >> 5); w < tasks; w += stride) {
-        const Task k(a, w, heads, splits);
+        const Task k(a, group, w, heads, splits);
         const uint32_t count = k.hi - k.lo, rounds = __reduce_max_sync(0xFFFFFFFFu, count);
         const T* dy = static_cast<const T*>(in.p) + k.t * in.ts + k.lo * in.hs;
         const T* xp = static_cast<const T*>(src.p) + k.t * src.ts + k.lo * src.hs;
         const uint8_t* data = (is_q ? a.q8 : a.k8) + k.t * pitch;
         const uint8_t* scale = (is_q ? a.sq : a.sk) + k.t * (pitch >> 5);
-        uint64_t col = (uint64_t)k.lo * d.dim;
+        uint64_t col = (uint64_t)k.lo * dim;
         T* dx = static_cast<T*>(out.p) + k.t * out.ts + k.lo * out.hs;
         Raw<T, VEC> g0[NU];
-        Source<T, VEC, SRC> x0[NU];
+        Source<T, VEC, G, SRC> x0[NU];
         auto load = [&](uint32_t h) {
             const bool read = k.live && h < count;
 #pragma unroll
@@ -567,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
             }
             dy += in.hs;
             if (SRC == 0) xp += src.hs;
-            col += d.dim;
+            col += dim;
         };
         load(0);
         Turn<VEC> turn[NU];
@@ -577,35 +629,54 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
         for (uint32_t h = 0; h < rounds; ++h) {
             const bool here = h < count, read = here && k.live;
             uint64_t v[NU][VEC], x[NU][VEC];
+            float f1[NU], f2[NU];
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
                 g0[n].get(v[n]);
-                x0[n].get(x[n]);
+                x0[n].get(x[n], f1[n], f2[n]);
             }
             load(h + 1);
-            uint64_t ss = 0;
+            // the squares before scaling, then scaled twice: no scale's square is formed
+            float own = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NU; ++n)
+            for (int n = 0; n < NU; ++n) {
+                if constexpr (VEC == 1) {
+                    float b, c;
+                    unpair(mul2(x[n][0], x[n][0]), b, c);
+                    own = __fadd_rn(own, __fadd_rn(__fmul_rn(__fmul_rn(b, f1[n]), f1[n]),
+                                                   __fmul_rn(__fmul_rn(c, f2[n]), f2[n])));
+                } else {
+                    uint64_t q1 = 0, q2 = 0;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) ss = fma2(x[n][i], x[n][i], ss);
-            const float all = group_sum(sum2(ss), d.group);
+                    for (int i = 0; i < VEC / 2; ++i) {
+                        q1 = fma2(x[n][i], x[n][i], q1);
+                        q2 = fma2(x[n][VEC / 2 + i], x[n][VEC / 2 + i], q2);
+                    }
+                    own = __fadd_rn(own, __fadd_rn(__fmul_rn(__fmul_rn(sum2(q1), f1[n]), f1[n]),
+                                                   __fmul_rn(__fmul_rn(sum2(q2), f2[n]), f2[n])));
+                }
+            }
+            const float all = group_sum<G>(own, group);
             // nothing of a padding token may reach the sums, not even 0 * rsqrt(0)
-            const uint64_t r = twice(read ? rsqrtf(__fmaf_rn(all, inv_dim, a.eps)) : 0.0f);
+            const float r1 = read ? rsqrtf(__fmaf_rn(all, inv_dim, a.eps)) : 0.0f;
+            const uint64_t r = twice(r1);
             uint64_t dot2 = 0;
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
                 if (u[n].turned && read) turn[n](d, v[n]);
                 uint64_t g[VEC];
                 unit_floats<VEC>(gains, u[n], g);
+                const float e1 = __fmul_rn(f1[n], r1), e2 = __fmul_rn(f2[n], r1);
+                const uint64_t h1 = VEC == 1 ? pair(e1, e2) : twice(e1), h2 = twice(e2);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    x[n][i] = mul2(x[n][i], r);
+                    x[n][i] = mul2(x[n][i], i < VEC / 2 || VEC == 1 ? h1 : h2);
                     dg[n][i] = fma2(v[n][i], x[n][i], dg[n][i]);
                     v[n][i] = mul2(v[n][i], g[i]);
                     dot2 = fma2(v[n][i], x[n][i], dot2);
                 }
             }
-            const uint64_t dot = twice(-__fmul_rn(group_sum(sum2(dot2), d.group), inv_dim));
+            const uint64_t dot = twice(-__fmul_rn(group_sum<G>(sum2(dot2), group), inv_dim));
 #pragma unroll
             for (int n = 0; n < NU; ++n) {
 #pragma unroll
@@ -616,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
         }
     }
     // the groups' sums, added in group order
-    const uint32_t mine = threadIdx.x / d.group, groups = kThreads / d.group;
+    const uint32_t mine = threadIdx.x / group, groups = kThreads / group;
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
         float f[2 * VEC];
@@ -624,15 +695,15 @@ __global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
         for (int i = 0; i < VEC; ++i) unpair(dg[n][i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            if (u[n].h1) sums[mine * d.dim + u[n].o1 + i] = f[i];
-            if (u[n].h2) sums[mine * d.dim + u[n].o2 + i] = f[VEC + i];
+            if (u[n].h1) sums[mine * dim + u[n].o1 + i] = f[i];
+            if (u[n].h2) sums[mine * dim + u[n].o2 + i] = f[VEC + i];
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < d.dim; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < dim; i += kThreads) {
         float s = 0.0f;
-        for (uint32_t m = 0; m < groups; ++m) s = __fadd_rn(s, sums[m * d.dim + i]);
-        a.partial[(uint64_t)blockIdx.x * d.dim + i] = s;
+        for (uint32_t m = 0; m < groups; ++m) s = __fadd_rn(s, sums[m * dim + i]);
+        a.partial[(uint64_t)blockIdx.x * dim + i] = s;
     }
 }
 
@@ -649,7 +720,7 @@ __global__ void __launch_bounds__(kThreads) gains_kernel(const float* __restrict
     if (lo == hi) return;
     float s = 0.0f;
     for (uint32_t b = lo + lane; b < hi; b += 32) s = __fadd_rn(s, partial[(uint64_t)b * dim + i]);
-    s = group_sum(s, 32);
+    s = group_sum<32>(s, 32);
     if (lane) return;
     void* out = is_q ? dgq : dgk;
     if (accumulate) s = __fadd_rn(s, gain_at(out, type, i));
@@ -700,7 +771,6 @@ bool multiple(const Heads& h, uint64_t e, uint64_t vec) {
 // The widest chunk that divides the head, its rotated part and every row's start.
 int chunk_of(const ark_rope_plan* p, uint64_t dim, uint64_t e, const Heads* h, int n) {
     for (int vec = 8; vec > 1; vec /= 2) {
-        if (vec == 2) continue;
         const uint64_t rot = p->rotary_dim;
         bool ok = dim % vec == 0 && (p->interleaved ? rot % (2 * vec) == 0 : rot / 2 % vec == 0);
         for (int i = 0; ok && i < n; ++i) ok = multiple(h[i], e, (uint64_t)vec);
@@ -760,32 +830,46 @@ uint32_t blocks_of(uint64_t tokens, uint32_t splits, uint32_t group, uint64_t mo
     return (uint32_t)(need < most ? need : most);
 }
 
-template <class T, int VEC, int NU, bool NORM, int HOLD>
+// the static form of a head, where there is one (16-bit types)
+template <class T>
+int full_of(const Deal& d, int vec) {
+    if (sizeof(T) != 2 || vec != 8 || d.rot != d.dim) return 0;
+    return d.dim == 128 ? 8 : d.dim == 64 ? 4 : 0;
+}
+
+template <class T, int VEC, int NU, int G, bool NORM, int HOLD>
 int forward_t(Args& a, cudaStream_t s) {
     a.splits = splits_of(a.tokens, a.q.heads + a.k.heads, a.d.group);
     const uint32_t grid = blocks_of(a.tokens, a.splits, a.d.group, (uint64_t)sm_count() * 16);
-    forward_kernel<T, VEC, NU, NORM, HOLD><<<grid, kThreads, 0, s>>>(a);
+    forward_kernel<T, VEC, NU, G, NORM, HOLD><<<grid, kThreads, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
 template <class T, bool NORM, int HOLD>
 int forward_v(Args& a, int vec, cudaStream_t s) {
-    if (vec == 8) return forward_t<T, 8, 1, NORM, HOLD>(a, s);
+    if constexpr (sizeof(T) == 2) {
+        const int full = full_of<T>(a.d, vec);
+        if (full == 8) return forward_t<T, 8, 1, 8, NORM, HOLD>(a, s);
+        if (full == 4) return forward_t<T, 8, 1, 4, NORM, HOLD>(a, s);
+    }
+    if (vec == 8) return forward_t<T, 8, 1, 0, NORM, HOLD>(a, s);
     if constexpr (HOLD != 0)
         return ARK_E_UNSUPPORTED;   // not reached: the checkpoint is then a launch of its own
     else
-        return vec == 4 ? forward_t<T, 4, 1, NORM, 0>(a, s) : forward_t<T, 1, 4, NORM, 0>(a, s);
+        return vec == 4   ? forward_t<T, 4, 1, 0, NORM, 0>(a, s)
+               : vec == 2 ? forward_t<T, 2, 2, 0, NORM, 0>(a, s)
+                          : forward_t<T, 1, 4, 0, NORM, 0>(a, s);
 }
 
-template <class T, int VEC, int NU>
+template <class T, int VEC, int NU, int G>
 int backward_t(Args& a, uint32_t blocks, cudaStream_t s) {
     const size_t smem = (size_t)(kThreads / a.d.group) * a.d.dim * sizeof(float);
     if (a.kind < 0)
-        backward_kernel<T, VEC, NU, 0><<<blocks, kThreads, smem, s>>>(a);
+        backward_kernel<T, VEC, NU, G, 0><<<blocks, kThreads, smem, s>>>(a);
     else if (a.kind == kE4M3)
-        backward_kernel<T, VEC, NU, 1 + kE4M3><<<blocks, kThreads, smem, s>>>(a);
+        backward_kernel<T, VEC, NU, G, 1 + kE4M3><<<blocks, kThreads, smem, s>>>(a);
     else
-        backward_kernel<T, VEC, NU, 1 + kInt8><<<blocks, kThreads, smem, s>>>(a);
+        backward_kernel<T, VEC, NU, G, 1 + kInt8><<<blocks, kThreads, smem, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
@@ -1016,9 +1100,15 @@ int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* d
     const uint32_t blocks = back_blocks(a);
     rc = by_type(type, [&](auto t) {
         using T = decltype(t);
-        return vec == 8   ? backward_t<T, 8, 1>(a, blocks, s)
-               : vec == 4 ? backward_t<T, 4, 1>(a, blocks, s)
-                          : backward_t<T, 1, 4>(a, blocks, s);
+        if constexpr (sizeof(T) == 2) {
+            const int full = full_of<T>(a.d, vec);
+            if (full == 8) return backward_t<T, 8, 1, 8>(a, blocks, s);
+            if (full == 4) return backward_t<T, 8, 1, 4>(a, blocks, s);
+        }
+        return vec == 8   ? backward_t<T, 8, 1, 0>(a, blocks, s)
+               : vec == 4 ? backward_t<T, 4, 1, 0>(a, blocks, s)
+               : vec == 2 ? backward_t<T, 2, 2, 0>(a, blocks, s)
+                          : backward_t<T, 1, 4, 0>(a, blocks, s);
     });
     if (rc) return rc;
     gains_kernel<<<(2 * (unsigned)dim * 32 + kThreads - 1) / kThreads, kThreads, 0, s>>>(
