@@ -30,6 +30,9 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kMaxDim = ARK_ROPE_MAX_DIM;
 constexpr int kBlocksPerSm = 6;
+// More blocks spill: 8192 tokens of 40 heads from e4m3 took 64 us with 4, 78 with
+// 5, 101 with 6 (32768: 199, 228, 340).
+constexpr int kBackPerSm = 4;
 
 struct Heads {
     void* p;
@@ -295,7 +298,7 @@ __device__ __forceinline__ float group_sum(float v, uint32_t group) {
 
 // Checkpoint the two chunks of 8 of a lane.  A scale block is 4 lanes' chunks
 // of one half (half layout), or both chunks of 2 lanes (then they adjoin).
-template <int KIND, class T, class U>
+template <int KIND, int G, class T, class U>
 __device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col, const U& u, bool on,
                                      const Raw<T, 8>& x) {
     const bool next = u.o2 == u.o1 + 8;
@@ -319,17 +322,28 @@ __device__ __forceinline__ void hold(uint8_t* data, uint8_t* scale, uint64_t col
         m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
         const uint32_t n = __shfl_xor_sync(0xFFFFFFFFu, m, 2);
         if (!next) m = __vmaxu2(m, n);
-        if (!on || !u.h1) return;
         float f1, f2;
         widen2(m, f1, f2, T());
         b1 = scale_byte<KIND>(__float_as_uint(f1)), b2 = scale_byte<KIND>(__float_as_uint(f2));
+        if constexpr (G > 0) {   // the head's 2 or 4 scale bytes as one store
+            uint32_t all = b1 << (u.o1 >> 5) * 8 | b2 << (u.o2 >> 5) * 8;
+            all |= __shfl_xor_sync(0xFFFFFFFFu, all, 2);
+            if (G == 8) all |= __shfl_xor_sync(0xFFFFFFFFu, all, 4);
+            if (on && u.o1 == 0) {
+                if (G == 8)
+                    *reinterpret_cast<uint32_t*>(scale + (col >> 5)) = all;
+                else
+                    *reinterpret_cast<uint16_t*>(scale + (col >> 5)) = (uint16_t)all;
+            }
+        }
+        if (!on || !u.h1) return;
         quant_words<T, KIND, 4>(x.w, b1, q);
         quant_words<T, KIND, 4>(x.w + 4, b2, q + 2);
     }
     *reinterpret_cast<uint2*>(data + col + u.o1) = make_uint2(q[0], q[1]);
     *reinterpret_cast<uint2*>(data + col + u.o2) = make_uint2(q[2], q[3]);
-    if ((u.o1 & 31u) == 0) scale[(col + u.o1) >> 5] = (uint8_t)b1;
-    if ((u.o2 & 31u) == 0) scale[(col + u.o2) >> 5] = (uint8_t)b2;
+    if (G == 0 && (u.o1 & 31u) == 0) scale[(col + u.o1) >> 5] = (uint8_t)b1;
+    if (G == 0 && (u.o2 & 31u) == 0) scale[(col + u.o2) >> 5] = (uint8_t)b2;
 }
 
 // a row's columns behind the last head, up to the pitch
@@ -431,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_
                 for (int j = 0; j < kHeads; ++j) {
                     const bool here = from + h + j < to;
                     if constexpr (HOLD != 0 && VEC == 8)
-                        hold<HOLD - 1>(data, scale, col, u[0], here, raw[j][0]);
+                        hold<HOLD - 1, G>(data, scale, col, u[0], here, raw[j][0]);
                     uint64_t v[NU][VEC];
 #pragma unroll
                     for (int n = 0; n < NU; ++n) raw[j][n].get(v[n]);
@@ -567,7 +581,7 @@ struct Source<T, VEC, G, 2> {
 // issued before a head is worked on.
 // SRC: 0 x as T, 1 e4m3, 2 int8.
 template <class T, int VEC, int NU, int G, int SRC>
-__global__ void __launch_bounds__(kThreads, NU == 1 && sizeof(T) == 2 ? 5 : 4)
+__global__ void __launch_bounds__(kThreads, kBackPerSm)
     backward_kernel(const __grid_constant__ Args a) {
     __shared__ uint64_t turns[kMaxDim / 2];
     __shared__ __align__(16) float gains[kMaxDim];
@@ -873,9 +887,8 @@ int backward_t(Args& a, uint32_t blocks, cudaStream_t s) {
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
-// Blocks of the backward: kBackPerSm to an SM, shared between queries and keys
+// Blocks of the backward: those that fit, shared between queries and keys
 // by their heads, and none without a task.
-constexpr uint64_t kBackPerSm = 5;
 uint32_t back_blocks(Args& a) {
     const uint64_t hq = a.q.heads, hk = a.k.heads, most = (uint64_t)sm_count() * kBackPerSm;
     const uint64_t tokens = a.tokens ? a.tokens : 1;   // no tokens: a block without work leaves zero sums
