@@ -183,6 +183,46 @@ class Optimizer:
         self._gbuf = self._device_view(p.value, n_full, "<f2")
         return self._gbuf
 
+    def grad_view(self, name: str, *shape):
+        """The range of grad_buffer() that holds tensor `name` of the layout,
+        as [shape] (default: flat): where a backward writes that tensor's
+        gradient, for example qk_norm_rope_backward(out_gains=...)."""
+        if getattr(self, "_gbuf", None) is None:
+            raise RuntimeError("grad_view needs grad_buffer() first")
+        t = next((t for t in self.layout.tensors if t.name == name), None)
+        if t is None:
+            raise KeyError(f"no tensor {name!r} in layout {self.layout.name!r}")
+        numel = 1
+        for d in shape:
+            numel *= d
+        lo = self.layout.offsets[name]
+        if (shape and numel != t.numel) or lo + t.numel > self._gbuf.numel():
+            raise ValueError(f"{name}: {t.numel} elements at {lo}, asked for {list(shape)} of a "
+                             f"buffer of {self._gbuf.numel()}")
+        flat = self._gbuf[lo: lo + t.numel]
+        return flat.view(*shape) if shape else flat
+
+    def weight_grad(self, name: str, x, dy, accumulate: bool = True):
+        """Add (or write) X^T dY, a projection's gradient from its input's
+        8-bit checkpoint (activations.Act8) and the loss-scaled dY [tokens,
+        out], to the range of grad_buffer() of weight `name` [in, out]: the
+        += of the reference's backward (objc/bridge.m:907-949) after
+        zero_grads().  Enqueued on the step's stream, like the step that reads
+        it; x and dy have to be ready there."""
+        import torch
+        from . import activations
+        out = self.grad_view(name, x.cols, dy.shape[1])
+        device = out.device
+        handle = self.stream_handle or 0
+        stream = (torch.cuda.ExternalStream(handle, device) if handle
+                  else torch.cuda.default_stream(device))
+        other = torch.cuda.current_stream(device) != stream
+        with torch.cuda.stream(stream):
+            activations.weight_grad(x, dy, out=out, accumulate=accumulate)
+        if other:   # their memory is not reused before the step's stream has read it
+            for t in (x.data, x.scale, dy):
+                t.record_stream(stream)
+
     def _device_view(self, ptr, n, typestr):
         import torch
 
