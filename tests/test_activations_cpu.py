@@ -8,7 +8,7 @@ import torch
 
 import act_ref as ref
 import ark_b200 as ab
-from ark_b200 import _lib, activations
+from ark_b200 import _lib
 
 INVALID, MISALIGNED, UNSUPPORTED = -1, -2, -8
 P = 0x7F0000001000      # an aligned address that nothing reads
@@ -108,8 +108,14 @@ def heads(p=P, h=4, ts=256, hs=64):
     return by(_lib.Heads(p, h, ts, hs))
 
 
-def plan(rot=64, **kw):
-    return by(ab.RopePlan(rot, **kw).c)
+def plan_struct(rot=64):
+    c = _lib.RopePlan()
+    assert _lib.lib().ark_cuda_rope_plan(by(c), rot, 0, 10000.0, 0, 1.0, 0.0, 32.0, 1.0) == 0
+    return c
+
+
+def plan(rot=64):
+    return by(plan_struct(rot))
 
 
 def rope(pl=None, q=None, k=None, oq=None, ok=None, t=0, tokens=8, dim=64, pos=None, pt=0, seq=8):
@@ -131,7 +137,7 @@ def test_rope_refuses():
     assert rope(oq=heads(hs=63)) == INVALID                   # heads of an output overlap
     assert rope(oq=heads(ts=255)) == INVALID
     assert rope(tokens=0) == 0 and rope(q=heads(h=0), oq=heads(h=0)) == 0
-    broken = ab.RopePlan(64).c
+    broken = plan_struct()
     for field, value in (("rotary_dim", 63), ("rotary_dim", 0), ("interleaved", 2)):
         c = type(broken).from_buffer_copy(broken)
         setattr(c, field, value)
@@ -234,20 +240,6 @@ def test_plan_frequencies(rot, kw):
 def test_plan_refuses(bad):
     with pytest.raises((ValueError, ab.ArkError)):
         ab.RopePlan(**{"rotary_dim": 64, **bad})
-
-
-def test_positions_are_checked():
-    f = activations._positions
-    dev = torch.device("cpu")
-    assert f(None, 8, None, dev) == (None, 0, 8) and f(None, 8, 4, dev) == (None, 0, 4)
-    with pytest.raises(ValueError):
-        f(None, 8, 0, dev)
-    with pytest.raises(ValueError):
-        f(torch.zeros(8, dtype=torch.int32), 8, 4, dev)
-    with pytest.raises(TypeError):
-        f(torch.zeros(8), 8, None, dev)
-    with pytest.raises(ValueError):
-        f(torch.zeros(7, dtype=torch.int64), 8, None, dev)
 
 
 # ----------------------------------------------------------------- formulas against differences

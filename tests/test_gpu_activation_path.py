@@ -212,7 +212,8 @@ def test_tensors_without_the_right_shape_are_refused():
                  lambda: ab.rope(q.transpose(1, 2), None, p), lambda: ab.rope(q, q[:7], p), lambda: ab.rope(q, q.float(), p),
                  lambda: ab.rope(q[..., :32], None, p), lambda: ab.rope(q, None, p, positions=torch.zeros(7, device="cuda", dtype=torch.int32)),
                  lambda: ab.rope(q, None, p, positions=torch.zeros(8, dtype=torch.int32)),
-                 lambda: ab.rope(q, None, p, out=(q, q)),
+                 lambda: ab.rope(q, None, p, out=(q, q)), lambda: ab.rope(q, q, p, out=(q, None)),
+                 lambda: ab.rope(q, None, p, seq_len=0), lambda: ab.rope(q, None, p, torch.zeros(8, device="cuda", dtype=torch.int32), 8),
                  lambda: ab.qk_norm_rope(q, None, g[:32], None, p), lambda: ab.qk_norm_rope(q, q, g, g.float(), p),
                  lambda: ab.qk_norm_rope_backward(q, None, ab.act8_pack(x[:7]), None, g, None, p),
                  lambda: ab.qk_norm_rope_backward(q, q, c, q, g, g, p),
