@@ -134,7 +134,7 @@ SIGNATURES = {
     "ark_cuda_act8_pitch": (c_u64, [c_u64]),
     "ark_cuda_act8_pack": (c_i, [c_p, c_i32, c_u64, _p_act8, c_p]),
     "ark_cuda_act8_unpack": (c_i, [_p_act8, c_p, c_i32, c_u64, c_p]),
-    "ark_cuda_weight_grad_workspace": (c_u64, [_p_act8, c_p, c_u64, c_u64, c_p, c_i32, c_u64]),
+    "ark_cuda_weight_grad_workspace": (c_u64, [_p_act8, c_p, c_u64, c_u64]),
     "ark_cuda_weight_grad": (c_i, [_p_act8, c_p, c_i32, c_u64, c_u64, c_p, c_i32, c_u64, c_i32, c_p,
                                    c_u64, c_p]),
     "ark_cuda_swiglu": (c_i, [c_p, c_u64, c_p, c_u64, c_i32, c_u64, c_u64, c_p, c_u64, _p_act8,

@@ -222,7 +222,7 @@ Tensor weight_grad(const Act8& x, const Tensor& dy, const MaybeTensor& out, bool
     const int type = type_code(w.scalar_type());
     const uint64_t ldw = (uint64_t)w.stride(0);
     const uint64_t need =
-        ark_cuda_weight_grad_workspace(x.c(), dy.data_ptr(), ld, (uint64_t)n, w.data_ptr(), type, ldw);
+        ark_cuda_weight_grad_workspace(x.c(), dy.data_ptr(), ld, (uint64_t)n);
     Tensor ws;
     if (need) ws = fresh({(int64_t)need}, at::kByte, dy.device());
     check("ark_cuda_weight_grad",

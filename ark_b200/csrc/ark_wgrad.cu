@@ -53,7 +53,8 @@ struct Few {      // a CTA alone: 128 x 128
 };
 struct Pair {     // two CTAs: 256 x 256, of which each brings 128 columns of dY
     static constexpr int kBN = 256, kBBytes = kBN / 2 / 64 * kAtom, kStage = kABytes + kBBytes;
-    static constexpr int kStages = 6, kSmem = kStages * kStage + 1024;
+    static constexpr int kStages = 6, kStaged = 16 * 32 * 16 * 4;   // epilogue: 2 KB per warp
+    static constexpr int kSmem = kStages * kStage + kStaged + 1024;
 };
 
 struct Out {
@@ -301,33 +302,90 @@ __device__ __forceinline__ void out_put(const Out& o, uint64_t i, float v) {
     else
         static_cast<__half*>(o.p)[i] = __float2half_rn(v);
 }
-template <int N, class T>
-__device__ __forceinline__ void out_vec(T* p, float* v, bool accumulate) {
-    if (accumulate) {
-        float old[N];
-        load_vec<N>(p, old);
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = __fadd_rn(v[j], old[j]);
-    }
-    store_vec<N>(p, v);
+// four elements of a row of whole vectors
+__device__ __forceinline__ void out_old4(const Out& o, uint64_t i, float* v) {
+    if (o.f32)
+        load_vec<4>(static_cast<const float*>(o.p) + i, v);
+    else if (o.bf16)
+        load_vec<4>(static_cast<const __nv_bfloat16*>(o.p) + i, v);
+    else
+        load_vec<4>(static_cast<const __half*>(o.p) + i, v);
 }
-// N (4 or 8) sums of one row of an m x n output, rounded once to its type
-template <int N>
-__device__ __forceinline__ void out_row(const Out& o, uint32_t m, uint32_t n, uint32_t row,
-                                        uint32_t col, float* v, bool accumulate) {
+__device__ __forceinline__ void out_put4(const Out& o, uint64_t i, const float* v) {
+    if (o.f32)
+        store_vec<4>(static_cast<float*>(o.p) + i, v);
+    else if (o.bf16)
+        store_vec<4>(static_cast<__nv_bfloat16*>(o.p) + i, v);
+    else
+        store_vec<4>(static_cast<__half*>(o.p) + i, v);
+}
+// four sums of one row of an m x n output, rounded once to its type
+__device__ __forceinline__ void out_row4(const Out& o, uint32_t m, uint32_t n, uint32_t row,
+                                         uint32_t col, float* v, bool accumulate) {
     if (row >= m || col >= n) return;
     const uint64_t i = (uint64_t)row * o.ld + col;
-    if (o.vec && col + N <= n) {
-        if (o.f32)
-            out_vec<N>(static_cast<float*>(o.p) + i, v, accumulate);
-        else if (o.bf16)
-            out_vec<N>(static_cast<__nv_bfloat16*>(o.p) + i, v, accumulate);
-        else
-            out_vec<N>(static_cast<__half*>(o.p) + i, v, accumulate);
+    if (o.vec && col + 4 <= n) {
+        float old[4];
+        if (accumulate) {
+            out_old4(o, i, old);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], old[j]);
+        }
+        out_put4(o, i, v);
     } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
+        for (int j = 0; j < 4; ++j)
             if (col + j < n) out_put(o, i + j, accumulate ? __fadd_rn(v[j], out_get(o, i + j)) : v[j]);
+    }
+}
+
+// A warp's 32 x 16 block of sums, staged in shared memory, to rows row0 on and
+// columns col0 on of an m x n output.  Through the staging four lanes come to
+// share a row, so that a store fills whole sectors of 8 rows; element by element
+// (rows on any boundary) 16 lanes share one.
+template <class O>
+__device__ __forceinline__ void out_block(O* p, const Out& o, uint32_t m, uint32_t n, uint32_t row0,
+                                          uint32_t col0, const float4* staged, uint32_t lane,
+                                          bool accumulate) {
+    if (o.vec && col0 + 16 <= n) {
+        const uint32_t r0 = lane / 4;
+        p += (uint64_t)(row0 + r0) * o.ld + col0 + (lane & 3) * 4;
+        float old[4][4];
+        if (accumulate) {   // all reads before the first write
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (row0 + r0 + i * 8 < m) load_vec<4>(p + (uint64_t)(i * 8) * o.ld, old[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t r = r0 + i * 8;
+            const float4 f = staged[r * 4 + ((lane & 3) ^ (r >> 1 & 3))];
+            float v[4] = {f.x, f.y, f.z, f.w};
+            if (accumulate) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], old[i][j]);
+            }
+            if (row0 + r < m) store_vec<4>(p + (uint64_t)(i * 8) * o.ld, v);
+        }
+        return;
+    }
+    const uint32_t e = lane & 15, r0 = lane / 16;
+    const float* one = reinterpret_cast<const float*>(staged);
+    if (col0 + e >= n) return;
+    p += (uint64_t)(row0 + r0) * o.ld + col0 + e;
+#pragma unroll 1
+    for (uint32_t h = 0; h < 32; h += 8, p += 8 * o.ld) {
+        float old[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            old[i] = accumulate && row0 + r0 + h + 2 * i < m ? Elem<O>::to_f(p[(uint64_t)(2 * i) * o.ld]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t r = r0 + h + 2 * i;
+            const float v = one[(r * 4 + (e / 4 ^ (r >> 1 & 3))) * 4 + e % 4];
+            if (row0 + r < m)
+                p[(uint64_t)(2 * i) * o.ld] = Elem<O>::from_f(accumulate ? __fadd_rn(v, old[i]) : v);
+        }
     }
 }
 
@@ -567,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             v[3] = __fadd_rn(v[3], q.w);
         }
         if (lost) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
-        out_row<4>(a.out, a.m, a.n, m0 + row, n0 + col, v, a.accumulate);
+        out_row4(a.out, a.m, a.n, m0 + row, n0 + col, v, a.accumulate);
     }
     cluster_sync();   // nobody leaves while its tile is read
     if (warp == kMmaWarp) {
@@ -712,30 +770,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         // four warps to each quarter of the rows, a quarter of the columns each
         constexpr int kCols = S::kBN * 4 / kPairEpiWarps;
         const uint32_t quarter = warp % 4, c0 = warp / 4 * kCols;
+        float4* staged = reinterpret_cast<float4*>(raw + (stages - smem_u32(raw)) + kStages * S::kStage) +
+                         warp * 128;
         uint32_t buf = 0, bphase = 0;
         for (uint32_t i = blockIdx.x / 2; i < items; i += pairs) {
             uint32_t m, n, it0, it1;
             const uint32_t run = item(i, m, n, it0, it1);
-            const uint32_t row = m * (2 * kBM) + rank * kBM + quarter * 32 + lane;
+            const uint32_t row0 = m * (2 * kBM) + rank * kBM + quarter * 32;
             Out out = a.out;
             bool accumulate = a.accumulate;
             if (a.partial) {
                 out = Out{a.partial + (uint64_t)run * a.m * a.n_pad, a.n_pad, 1, 0, 1};
                 accumulate = false;
             }
-            // 16 columns from c on
-            auto put = [&](uint32_t c, float* v, bool ok) {
+            // 16 columns from c on, of which a lane has one row
+            auto put = [&](uint32_t c, const float* v, bool ok) {
+                const float none = __uint_as_float(0x7FC00000u);
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = ok ? v[j] : __uint_as_float(0x7FC00000u);
-#pragma unroll
-                for (int j = 0; j < 16; j += 8) {
-                    const uint32_t col = n * S::kBN + c + j;
-                    if (RUNS && row < a.m && col + 8 <= a.n && out.vec)
-                        out_vec<8>(static_cast<float*>(out.p) + (uint64_t)row * out.ld + col, v + j,
-                                   accumulate);
-                    else
-                        out_row<8>(out, a.m, a.n, row, col, v + j, accumulate);
-                }
+                for (int j = 0; j < 4; ++j)
+                    staged[lane * 4 + (j ^ (lane >> 1 & 3))] =
+                        ok ? make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3])
+                           : make_float4(none, none, none, none);
+                __syncwarp();
+                const uint32_t col0 = n * S::kBN + c;
+                if (RUNS || out.f32)
+                    out_block(static_cast<float*>(out.p), out, a.m, a.n, row0, col0, staged, lane, accumulate);
+                else if (out.bf16)
+                    out_block(static_cast<__nv_bfloat16*>(out.p), out, a.m, a.n, row0, col0, staged, lane,
+                              accumulate);
+                else
+                    out_block(static_cast<__half*>(out.p), out, a.m, a.n, row0, col0, staged, lane, accumulate);
             };
             auto next = [&] {
                 fence_before();
@@ -747,12 +812,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 const bool ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up);
                 fence_after();
 #pragma unroll 1
-                for (uint32_t c = c0; c < c0 + kCols; c += 32) {
-                    float v[32];
-                    tmem_ld32(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
+                for (uint32_t c = c0; c < c0 + kCols; c += 16) {
+                    float v[16];
+                    tmem_ld16(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
                     put(c, v, ok);
-                    put(c + 16, v + 16, ok);
                 }
                 next();
             } else {
@@ -805,7 +869,7 @@ __global__ void __launch_bounds__(256) runs_kernel(const Args a) {
             v[2] = __fadd_rn(v[2], q.z);
             v[3] = __fadd_rn(v[3], q.w);
         }
-        out_row<4>(a.out, a.m, a.n, row, col, v, a.accumulate);
+        out_row4(a.out, a.m, a.n, row, col, v, a.accumulate);
     }
 }
 
@@ -945,7 +1009,7 @@ struct Way {
     uint32_t splits;   // pairs: runs of tokens
     uint64_t x_bytes, partial_bytes;
 };
-Way way_of(uint64_t tokens, uint64_t m, uint64_t n, bool vec) {
+Way way_of(uint64_t tokens, uint64_t m, uint64_t n) {
     const uint64_t iters = (tokens + kBK - 1) / kBK, sms = (uint64_t)sm_count();
     const uint64_t few = (m + 127) / 128 * ((n + 127) / 128);
     const uint64_t tiles = (m + 255) / 256 * ((n + 255) / 256);
@@ -960,20 +1024,14 @@ Way way_of(uint64_t tokens, uint64_t m, uint64_t n, bool vec) {
     for (uint32_t r = 1; r <= 16 && (r == 1 || r * 8 <= iters); ++r) {
         const uint64_t waves = ceil_div(tiles * r, sms / 2);
         const uint64_t t = 8000 + x_bytes * 3 / 2 / 5000 + waves * (1500 + 330 * ceil_div(iters, r)) +
-                           (r > 1 || !vec ? 3000 + 2 * r * run / 8000 : 0);
+                           (r > 1 ? 3000 + 2 * r * run / 8000 : 0);
         if (t < best) best = t, w.pairs = true, w.splits = r;
     }
     if (w.pairs) {
         w.x_bytes = x_bytes;
-        // rows of an output that vectors cannot write go through the FP32 buffer
-        // too: an accumulator's lane holds one row, and element by element 32 rows
-        // at a time 4096 tokens, 2048 x 5501 took 225 us
-        w.partial_bytes = w.splits > 1 || !vec ? w.splits * run : 0;
+        w.partial_bytes = w.splits > 1 ? w.splits * run : 0;
     }
     return w;
-}
-bool out_vec_rows(const void* dw, int32_t type, uint64_t ld) {
-    return aligned16(dw) && ld * type_size(type) % 16 == 0;
 }
 // the workspace's last part: dY realigned
 uint64_t ws_dy(uint64_t tokens, const void* dy, uint64_t lddy, uint64_t n) {
@@ -988,10 +1046,9 @@ using namespace ark;
 extern "C" {
 
 uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
-                                        uint64_t n_out, const void* dw, int32_t dw_type,
-                                        uint64_t lddw) {
+                                        uint64_t n_out) {
     if (!x || !x->rows || !x->cols || !n_out) return 0;
-    const Way w = way_of(x->rows, x->cols, n_out, out_vec_rows(dw, dw_type, lddw));
+    const Way w = way_of(x->rows, x->cols, n_out);
     return w.x_bytes + w.partial_bytes + ws_dy(x->rows, dy, lddy, n_out);
 }
 
@@ -1022,7 +1079,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     a.n = (uint32_t)n_out;
     a.iters = (a.tokens + kBK - 1) / kBK;
     a.out = Out{dw, lddw, dw_type == ARK_TYPE_F32, dw_type == ARK_TYPE_BF16,
-                out_vec_rows(dw, dw_type, lddw)};
+                aligned16(dw) && lddw * e % 16 == 0};
     a.accumulate = accumulate != 0;
     if (x->rows == 0) {
         if (accumulate) return ARK_OK;
@@ -1031,7 +1088,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
     }
 
-    const Way w = way_of(x->rows, x->cols, n_out, a.out.vec);
+    const Way w = way_of(x->rows, x->cols, n_out);
     const uint64_t need_dy = ws_dy(x->rows, dy, lddy, n_out);
     const uint64_t need = w.x_bytes + w.partial_bytes + need_dy;
     if (need) {

@@ -439,13 +439,11 @@ ARK_API int ark_cuda_act8_unpack(const ark_act8* in, void* y, int32_t type, uint
  * scale; a sum that F16 cannot hold becomes an infinity, which the step
  * takes for an overflow.  The result is the same bits on every call.
  * workspace: 16-byte aligned, ark_cuda_weight_grad_workspace bytes on the
- * current device: x in 16 bits for large gradients, FP32 sums where the tokens
- * are split over them or dw's rows are not 16-byte aligned, dy again where its
- * rows are not; 0, and then it may be NULL, for a small gradient of aligned
- * rows. */
+ * current device: x in 16 bits for large gradients, FP32 sums where their
+ * tokens are split, dy again where its rows are not 16-byte aligned; 0, and
+ * then it may be NULL, for a small gradient of aligned rows. */
 ARK_API uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
-                                                uint64_t n_out, const void* dw, int32_t dw_type,
-                                                uint64_t lddw);
+                                                uint64_t n_out);
 ARK_API int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
                                  uint64_t n_out, void* dw, int32_t dw_type, uint64_t lddw,
                                  int32_t accumulate, void* workspace, uint64_t workspace_bytes,

@@ -76,13 +76,13 @@ def test_weight_grad_refuses():
     assert wg(x=by(act(rows=(1 << 31) - 1))) == INVALID
     assert wg(n=0) == 0 and wg(x=by(act(cols=0))) == 0
     L, a = _lib.lib(), act()
-    need = L.ark_cuda_weight_grad_workspace(by(a), P + 2, 64, 63, P, 0, 64)
+    need = L.ark_cuda_weight_grad_workspace(by(a), P + 2, 64, 63)
     assert need > 0                                           # rows that have to be realigned
     assert wg(dy=P + 2, n=63) == INVALID
     assert wg(dy=P + 2, n=63, ws=P, wsb=need - 1) == INVALID
     assert wg(dy=P + 2, n=63, ws=P + 4, wsb=need) == MISALIGNED
-    assert L.ark_cuda_weight_grad_workspace(by(act(rows=0)), P, 64, 64, P, 0, 64) == 0
-    assert L.ark_cuda_weight_grad_workspace(None, P, 64, 64, P, 0, 64) == 0
+    assert L.ark_cuda_weight_grad_workspace(by(act(rows=0)), P, 64, 64) == 0
+    assert L.ark_cuda_weight_grad_workspace(None, P, 64, 64) == 0
 
 
 def test_swiglu_refuses():
