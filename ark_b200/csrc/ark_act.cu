@@ -381,8 +381,29 @@ __global__ void __launch_bounds__(kThreads) swiglu_kernel(
     }
 }
 
+// One stored element in 64 bits.
+template <int KIND>
+__device__ __forceinline__ double held_one(const uint8_t* data, const uint8_t* scale, uint64_t at) {
+    float v[4];
+    bytes4<KIND>(data[at], v);
+    return (double)__fmul_rn(v[0], scale_of(scale[at >> 5]));
+}
+// How many FP32 steps y is from the middle between two values of a 16-bit type.
+__device__ __forceinline__ uint32_t from_tie(float y, __half) {
+    const int d = (int)(__float_as_uint(y) & 0x1FFFu) - 0x1000;
+    return (uint32_t)abs(d);
+}
+__device__ __forceinline__ uint32_t from_tie(float y, __nv_bfloat16) {
+    const int d = (int)(__float_as_uint(y) & 0xFFFFu) - 0x8000;
+    return (uint32_t)abs(d);
+}
+
 // With y8, the product is remade, rounded to T as the forward's was, and
-// checkpointed for the weight gradient of the projection that read it.
+// checkpointed for the weight gradient of the projection that read it.  The
+// product of two 8-bit values often lies next to a border of T, and once rounded
+// next to one of the 8-bit grid, where the last bit of FP32 would decide by a whole
+// step: values within FP32's error of a border of T, about one in 500, are made
+// again in 64 bits and rounded to FP32.
 template <class T, int KIND, bool REMAKE>
 __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
     const T* dy, uint64_t lddy, const uint8_t* __restrict__ a8, const uint8_t* __restrict__ sa,
@@ -400,6 +421,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
         Chunk<T> g, cy;
         g.load(dy + w.row * lddy, col, n, lie);
         float u[16], v[16], d[16], o[16];
+        uint32_t near = 0;
         held<KIND>(a8, sa, at, u);
         held<KIND>(b8, sb, at, v);
         g.get(d);
@@ -410,6 +432,12 @@ __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
             const float t = __fmul_rn(u[j], s);
             const float slope = __fmul_rn(s, __fmaf_rn(u[j], rest, 1.0f));
             o[j] = __fmul_rn(t, v[j]);
+            if constexpr (REMAKE && !std::is_same<T, float>::value) {
+                // exp(-|a|) is off by 2 + 1.2 |a| ulps, of which `rest` reaches s; the
+                // sum, the reciprocal and three products add 4, the mantissa doubles
+                const float ulps = __fmaf_rn(__fmaf_rn(2.4f, fabsf(u[j]), 4.0f), rest, 8.0f);
+                near |= (float)from_tie(o[j], T()) <= ulps ? 1u << j : 0u;
+            }
             u[j] = __fmul_rn(__fmul_rn(d[j], v[j]), slope);
             v[j] = __fmul_rn(d[j], t);
         }
@@ -418,6 +446,16 @@ __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
         g.set(v);
         g.store(db + w.row * lddb, col, n, lie);
         if (REMAKE) {
+            if constexpr (!std::is_same<T, float>::value) {
+                for (; near; near &= near - 1) {
+                    const int which = __ffs(near) - 1;
+                    const double p = held_one<KIND>(a8, sa, at * 16 + which);
+                    const double q = held_one<KIND>(b8, sb, at * 16 + which);
+                    const float y = (float)(p / (1.0 + exp(-p)) * q);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[j] = j == which ? y : o[j];
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] = j < n ? o[j] : 0.0f;
             cy.set(o);
