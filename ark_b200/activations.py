@@ -16,17 +16,32 @@ through libark_cuda.so, by way of the binding ark_b200/lib/_ark_torch.so
 """
 from __future__ import annotations
 
+import importlib.util
+import os
+
 import torch  # noqa: F401  (its libraries have to be loaded before the binding)
 
 from . import _lib
 
 _lib.lib()     # the binding links it; missing or of another version, this says so
-try:
-    from .lib import _ark_torch
-except ImportError as e:
-    raise RuntimeError("ark_b200/lib/_ark_torch.so is missing or was built for another torch: build it "
-                       "with `make -C ark_b200/csrc` (or __graft_entry__.build()); ark_b200 has no "
-                       "fallback") from e
+
+
+def _binding():
+    # by its file: importing the directory `lib` as a submodule would put a module in the
+    # place of the package's function lib()
+    path = os.path.join(os.path.dirname(_lib.LIB_PATH), "_ark_torch.so")
+    spec = importlib.util.spec_from_file_location("ark_b200._ark_torch", path)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as e:
+        raise RuntimeError("ark_b200/lib/_ark_torch.so is missing or was built for another torch: build it "
+                           "with `make -C ark_b200/csrc` (or __graft_entry__.build()); ark_b200 has no "
+                           "fallback") from e
+    return module
+
+
+_ark_torch = _binding()
 
 Act8, RopePlan = _ark_torch.Act8, _ark_torch.RopePlan
 act8_pack, act8_unpack, weight_grad = _ark_torch.act8_pack, _ark_torch.act8_unpack, _ark_torch.weight_grad

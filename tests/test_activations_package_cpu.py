@@ -1,0 +1,20 @@
+"""The activation operators beside the rest of the package: what was there
+before their first use is there after it."""
+import subprocess
+import sys
+
+from conftest import ROOT
+
+
+def run(code):
+    return subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+
+
+def test_lib_stays_a_function():
+    r = run("import ark_b200 as ab\n"
+            "before = ab.lib\n"
+            "ab.Act8, ab.RopePlan, ab.weight_grad\n"
+            "assert ab.lib is before and ab.lib().ark_cuda_act8_pitch(1) == 128\n"
+            "from ark_b200 import lib\n"
+            "assert lib is before\n")
+    assert r.returncode == 0, r.stderr
