@@ -6,8 +6,10 @@ an exception when it is missing: there is no fallback implementation.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import subprocess
+import sys
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -164,10 +166,13 @@ class ArkError(RuntimeError):
 
 
 def build(quiet=True):
-    """Compile libark_cuda.so/.a for sm_100a (nvcc cross-compiles without a GPU)."""
-    cmd = ["make", "-C", os.path.join(PKG, "csrc")]
+    """Compile libark_cuda.so/.a for sm_100a (nvcc cross-compiles without a GPU),
+    and the torch binding of the activation operators where torch is installed."""
+    cmd = ["make", "-C", os.path.join(PKG, "csrc"), "all"]
     if quiet:
         cmd.insert(1, "-s")
+    if importlib.util.find_spec("torch"):
+        cmd += ["torch", "PYTHON=" + sys.executable]
     subprocess.run(cmd, check=True)
 
 

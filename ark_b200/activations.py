@@ -36,8 +36,8 @@ def _binding():
         spec.loader.exec_module(module)
     except ImportError as e:
         raise RuntimeError("ark_b200/lib/_ark_torch.so is missing or was built for another torch: build it "
-                           "with `make -C ark_b200/csrc` (or __graft_entry__.build()); ark_b200 has no "
-                           "fallback") from e
+                           "with `make -C ark_b200/csrc all torch` (or __graft_entry__.build()); ark_b200 "
+                           "has no fallback") from e
     return module
 
 

@@ -1,5 +1,6 @@
 """The activation operators beside the rest of the package: what was there
 before their first use is there after it."""
+import os
 import subprocess
 import sys
 
@@ -18,3 +19,12 @@ def test_lib_stays_a_function():
             "from ark_b200 import lib\n"
             "assert lib is before\n")
     assert r.returncode == 0, r.stderr
+
+
+def test_the_c_library_builds_without_torch():
+    """`make` in a Python that has no torch: the commands for the library, none for the binding."""
+    r = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "ark_b200", "csrc"),
+                        f"PYTHON={sys.executable} -I -S"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stderr == ""
+    assert "libark_cuda.a" in r.stdout and "libark_cuda.so" in r.stdout
+    assert "_ark_torch" not in r.stdout and "torch/include" not in r.stdout
