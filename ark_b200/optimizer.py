@@ -358,6 +358,8 @@ class Optimizer:
         return {"pass1_blocks": b1.value, "pass2_blocks": b2.value, "threads": t.value}
 
     def close(self):
+        # the buffers are the library's and go with the handle: no view of them is given out after
+        self._gbuf = self._wbuf = None
         if getattr(self, "_h", None):
             _lib.lib().ark_cuda_opt_destroy(self._h)
             self._h = None

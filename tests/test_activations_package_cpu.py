@@ -4,6 +4,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 from conftest import ROOT
 
 
@@ -28,3 +30,18 @@ def test_the_c_library_builds_without_torch():
     assert r.returncode == 0 and r.stderr == ""
     assert "libark_cuda.a" in r.stdout and "libark_cuda.so" in r.stdout
     assert "_ark_torch" not in r.stdout and "torch/include" not in r.stdout
+
+
+def test_no_view_of_a_closed_optimizers_buffer():
+    """close() gives the gradient buffer back: a range of it would be freed memory."""
+    import torch
+
+    import ark_b200 as ab
+    from ark_b200 import layout
+    opt = object.__new__(ab.Optimizer)
+    opt.layout, opt._h = layout.decoder_layout("tiny", 1, 8, 16, 32), None
+    opt._gbuf = torch.zeros(opt.layout.n)
+    assert opt.grad_view("l0.w1").numel() == 128
+    opt.close()
+    with pytest.raises(RuntimeError, match="grad_buffer"):
+        opt.grad_view("l0.w1")
