@@ -1,0 +1,33 @@
+// ark_ring.h -- a reader's place among barriers that complete in turn.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define ARK_HD __host__ __device__ __forceinline__
+#else
+#define ARK_HD inline
+#endif
+
+namespace ark {
+
+// N barriers, waited for by their phase's parity.  A wait that ran out is final:
+// the barrier is then stuck in the phase that was waited for, and a later wait
+// for the other parity would be answered at once by the phase before it, whose
+// results are long gone.  So nothing is waited for after that.
+template <uint32_t N>
+struct Ring {
+    uint32_t at = 0, parity = 0;
+    bool ok = true;
+    // waited(barrier, parity): whether the phase has completed
+    template <class F>
+    ARK_HD bool wait(F waited) {
+        ok = ok && waited(at, parity);
+        return ok;
+    }
+    ARK_HD void next() {
+        if (++at == N) at = 0, parity ^= 1u;
+    }
+};
+
+}  // namespace ark

@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "ark_act8.cuh"
+#include "ark_ring.h"
 
 namespace ark {
 namespace {
@@ -772,7 +773,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t quarter = warp % 4, c0 = warp / 4 * kCols;
         float4* staged = reinterpret_cast<float4*>(raw + (stages - smem_u32(raw)) + kStages * S::kStage) +
                          warp * 128;
-        uint32_t buf = 0, bphase = 0;
+        Ring<2> acc;   // a wait that ran out makes every tile from there on NaN
+        auto wait = [&] {
+            return acc.wait([&](uint32_t b, uint32_t parity) {
+                return warp_wait<kSleep>(smem_u32(acc_full + b), parity, gave_up);
+            });
+        };
         for (uint32_t i = blockIdx.x / 2; i < items; i += pairs) {
             uint32_t m, n, it0, it1;
             const uint32_t run = item(i, m, n, it0, it1);
@@ -805,16 +811,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             auto next = [&] {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive_at(bar_of(smem_u32(acc_empty + buf), 0));
-                if (++buf == 2) buf = 0, bphase ^= 1u;
+                if (lane == 0) bar_arrive_at(bar_of(smem_u32(acc_empty + acc.at), 0));
+                acc.next();
             };
             if constexpr (!RUNS) {
-                const bool ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up);
+                const bool ok = wait();
                 fence_after();
 #pragma unroll 1
                 for (uint32_t c = c0; c < c0 + kCols; c += 16) {
                     float v[16];
-                    tmem_ld16(tmem + buf * S::kBN + (quarter * 32 << 16) + c,
+                    tmem_ld16(tmem + acc.at * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
                     put(c, v, ok);
                 }
@@ -822,14 +828,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             } else {
                 // the runs' sums are added in registers
                 float sum[kCols / 16][16];
-                bool ok = true;
                 for (uint32_t k = 0; k < a.chunks; ++k) {
-                    ok = warp_wait<kSleep>(smem_u32(acc_full + buf), bphase, gave_up) && ok;
+                    wait();
                     fence_after();
 #pragma unroll
                     for (int c = 0; c < kCols / 16; ++c) {
                         float v[16];
-                        tmem_ld16(tmem + buf * S::kBN + (quarter * 32 << 16) + c0 + c * 16,
+                        tmem_ld16(tmem + acc.at * S::kBN + (quarter * 32 << 16) + c0 + c * 16,
                                   reinterpret_cast<uint32_t*>(v));
 #pragma unroll
                         for (int j = 0; j < 16; ++j) sum[c][j] = k ? __fadd_rn(sum[c][j], v[j]) : v[j];
@@ -837,7 +842,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     next();
                 }
 #pragma unroll
-                for (int c = 0; c < kCols / 16; ++c) put(c0 + c * 16, sum[c], ok);
+                for (int c = 0; c < kCols / 16; ++c) put(c0 + c * 16, sum[c], acc.ok);
             }
         }
     }
