@@ -71,7 +71,7 @@ class OptStatus(ctypes.Structure):
 class Act8(ctypes.Structure):
     """ark_act8."""
     _fields_ = [("data", c_p), ("scale", c_p), ("rows", c_u64), ("cols", c_u64), ("kind", c_i32),
-                ("reserved", c_u32)]
+                ("wide", c_u32)]
 
 
 ARK_ROPE_MAX_DIM = 256

@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const T* __restrict__ x,
     }
 }
 
-template <class T, int KIND>
+// OPERAND: as operand16 says
+template <class T, int KIND, bool OPERAND = false>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restrict__ data,
                                                           const uint8_t* __restrict__ scale,
                                                           uint64_t rows, uint32_t cols,
@@ -311,7 +312,8 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const uint8_t* __restr
             for (int j = 0; j < 16; ++j) c.f[j] = saturate<float>(c.f[j]);
         } else {
             uint4 lo, hi;
-            operand16<T, KIND>(*reinterpret_cast<const uint4*>(data + at * 16), scale[at >> 1], lo, hi);
+            operand16<T, KIND, OPERAND>(*reinterpret_cast<const uint4*>(data + at * 16), scale[at >> 1],
+                                        lo, hi);
             c.w[0] = lo.x, c.w[1] = lo.y, c.w[2] = lo.z, c.w[3] = lo.w;
             c.w[4] = hi.x, c.w[5] = hi.y, c.w[6] = hi.z, c.w[7] = hi.w;
         }
@@ -492,10 +494,10 @@ int pack_t(const T* x, uint64_t ldx, const ark_act8* o, cudaStream_t s) {
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
 }
 
-template <class T, int KIND>
+template <class T, int KIND, bool OPERAND = false>
 int unpack_t(const ark_act8* c, T* y, uint64_t ldy, cudaStream_t s) {
     const uint32_t per = (uint32_t)(act8_pitch(c->cols) / 16);
-    auto k = unpack_kernel<T, KIND>;
+    auto k = unpack_kernel<T, KIND, OPERAND>;
     k<<<grid_of(c->rows * per), kThreads, 0, s>>>(c->data, c->scale, c->rows, (uint32_t)c->cols,
                                                      per, lie_of(y, ldy), y, ldy);
     return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
@@ -530,6 +532,18 @@ bool same_shape(const ark_act8* a, const ark_act8* b) {
 }
 
 }  // namespace
+
+int act8_operands(const ark_act8* c, void* y, int32_t type, uint64_t ldy, cudaStream_t s) {
+    if (type == ARK_TYPE_F16) {
+        __half* p = static_cast<__half*>(y);
+        return c->kind == kE4M3 ? unpack_t<__half, kE4M3, true>(c, p, ldy, s)
+                                : unpack_t<__half, kInt8, true>(c, p, ldy, s);
+    }
+    // BF16 operands are what unpacking makes
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(y);
+    return c->kind == kE4M3 ? unpack_t<__nv_bfloat16, kE4M3>(c, p, ldy, s)
+                            : unpack_t<__nv_bfloat16, kInt8>(c, p, ldy, s);
+}
 
 int realign_rows(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, void* dst, uint64_t ldd,
                  cudaStream_t s) {

@@ -9,8 +9,9 @@
 // byte is k + 127.  A power of two makes x * 2^-k and q * 2^k exact in FP32,
 // so the only rounding of the format is the one to 8 bits (nearest even), the
 // bytes do not depend on who computes them, and the matrix kernel can turn a
-// byte back into an FP16 / BF16 operand without a second rounding.  Against a
-// scale max|x| / top it costs int8 half a bit on average and e4m3 nothing.
+// byte back into a 16-bit operand without a second rounding, within that type's
+// range (operand16).  Against a scale max|x| / top it costs int8 half a bit on
+// average and e4m3 nothing.
 // A block that holds an infinity or a NaN gets scale byte 255 and bytes 0 and
 // reads back as NaN: an overflowed forward still makes the step a skipped one.
 #pragma once
@@ -311,21 +312,37 @@ struct Fast<__nv_bfloat16, kInt8> {
         return *reinterpret_cast<const uint32_t*>(&r);
     }
 };
-// Sixteen bytes of one block to 16-bit values in order.
-template <class T, int KIND>
+// The same for an operand of the matrix kernels: a magnitude above 65536 becomes an
+// infinity in FP16, so that the gradient shows it.  65536 itself is what the 8-bit
+// rounding makes of the largest FP16 numbers; 65504 is as near to them.  BF16 has the
+// FP32 range, and saturates only what 8 bits rounded up to 2^128.
+__device__ __forceinline__ uint32_t operand_pair(float a, float b, __half) {
+    a = fabsf(a) == 65536.0f ? copysignf(65504.0f, a) : a;
+    b = fabsf(b) == 65536.0f ? copysignf(65504.0f, b) : b;
+    return narrow2(a, b, __half());
+}
+__device__ __forceinline__ uint32_t operand_pair(float a, float b, __nv_bfloat16) {
+    return pair_of(a, b, __nv_bfloat16());
+}
+// Sixteen bytes of one block to 16-bit values in order.  OPERAND: out of range as
+// operand_pair, else saturating.  Every value of a checkpoint of FP16 numbers is an
+// FP16 number (but for 65536), down to 2^-24: the 8-bit rounding takes low bits off and
+// puts none on.  Values of a checkpoint of a wider type are rounded once.
+template <class T, int KIND, bool OPERAND>
 __device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uint4& hi) {
     if (byte >= Fast<T, KIND>::kLo && byte <= Fast<T, KIND>::kHi) {
         const Fast<T, KIND> f(byte);
         lo = make_uint4(f.pair(w.x, 0), f.pair(w.x, 2), f.pair(w.y, 0), f.pair(w.y, 2));
         hi = make_uint4(f.pair(w.z, 0), f.pair(w.z, 2), f.pair(w.w, 0), f.pair(w.w, 2));
     } else {
+        auto two = [](float x, float y) {
+            return OPERAND ? operand_pair(x, y, T()) : pair_of(x, y, T());
+        };
         float v[8];
         dequant8<KIND>(make_uint2(w.x, w.y), byte, v);
-        lo = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
-                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+        lo = make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
         dequant8<KIND>(make_uint2(w.z, w.w), byte, v);
-        hi = make_uint4(pair_of(v[0], v[1], T()), pair_of(v[2], v[3], T()),
-                        pair_of(v[4], v[5], T()), pair_of(v[6], v[7], T()));
+        hi = make_uint4(two(v[0], v[1]), two(v[2], v[3]), two(v[4], v[5]), two(v[6], v[7]));
     }
 }
 
@@ -454,6 +471,8 @@ int by_type(int32_t type, F f) {
 
 // null data is fine for an empty checkpoint
 int act8_check(const ark_act8* c);
+// act8_unpack to 16-bit operands of the matrix kernels (operand16), rows of whole vectors
+int act8_operands(const ark_act8* c, void* y, int32_t type, uint64_t ldy, cudaStream_t s);
 // 16-bit rows that start on any element, copied to rows of whole 16-byte vectors
 int realign_rows(const void* src, uint64_t ld, uint64_t rows, uint32_t cols, void* dst, uint64_t ldd,
                  cudaStream_t s);

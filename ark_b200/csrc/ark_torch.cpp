@@ -105,7 +105,7 @@ int kind_code(const std::string& kind) {
 class Act8 {
 public:
     // tensors that a caller holds
-    Act8(const py::object& data, const py::object& scale, int64_t cols, const std::string& kind)
+    Act8(const py::object& data, const py::object& scale, int64_t cols, const std::string& kind, bool wide)
         : cols_(cols), kind_(kind_code(kind)) {
         if (cols < 0) bad_value("cols: expected a length");
         const int64_t pitch = (int64_t)ark_cuda_act8_pitch((uint64_t)cols);
@@ -116,17 +116,21 @@ public:
         shaped(scale_, "scale", pitch / 32);
         need_device(data_.device(), scale_.device());
         c_ = ark_act8{data_.data_ptr<uint8_t>(), scale_.data_ptr<uint8_t>(), (uint64_t)rows_,
-                      (uint64_t)cols_, kind_, 0};
+                      (uint64_t)cols_, kind_, wide};
     }
     // room for one, in one allocation
-    Act8(int64_t rows, int64_t cols, int kind, at::Device d) : rows_(rows), cols_(cols), kind_(kind) {
+    Act8(int64_t rows, int64_t cols, int kind, at::Device d, at::ScalarType from) : rows_(rows), cols_(cols), kind_(kind) {
         if (rows < 0 || cols < 0) bad_value("rows, cols: expected lengths");
         if (!d.is_cuda()) bad_value("buffers must be CUDA tensors (device memory)");
         const int64_t pitch = (int64_t)ark_cuda_act8_pitch((uint64_t)cols);
         whole_ = fresh({rows * (pitch + pitch / 32)}, at::kByte, d);
         uint8_t* p = whole_.data_ptr<uint8_t>();
         c_ = ark_act8{p, p + rows * pitch, (uint64_t)rows, (uint64_t)cols, kind, 0};
+        hold(from);
     }
+    // what it is packed from
+    void hold(at::ScalarType from) { c_.wide = from != at::kHalf; }
+    bool wide() const { return c_.wide != 0; }
     const ark_act8* c() const { return &c_; }
     at::Device device() const { return whole_.defined() ? whole_.device() : data_.device(); }
     int64_t rows() const { return rows_; }
@@ -171,17 +175,19 @@ private:
 };
 
 // ------------------------------------------------------------ checkpoints
-Act8 act8_pack(const Tensor& x, const std::string& kind, const std::optional<Act8>& out) {
+Act8 act8_pack(const Tensor& x, const std::string& kind, Act8* out) {
     const uint64_t ld = rows_of(x, "x");
     const On on(x.device());
     if (out) {
         out->need("out", x.size(0), x.size(1));
         need_device(x.device(), out->device());
     }
-    const Act8 c = out ? *out : Act8(x.size(0), x.size(1), kind_code(kind), x.device());
+    const Act8 c = out ? *out : Act8(x.size(0), x.size(1), kind_code(kind), x.device(), x.scalar_type());
     check("ark_cuda_act8_pack",
           ark_cuda_act8_pack(x.data_ptr(), type_code(x.scalar_type()), ld, c.c(), on.stream));
-    return c;
+    if (!out) return c;
+    out->hold(x.scalar_type());
+    return *out;
 }
 
 Tensor act8_unpack(const Act8& c, at::ScalarType dtype, const MaybeTensor& out) {
@@ -221,12 +227,13 @@ Tensor weight_grad(const Act8& x, const Tensor& dy, const MaybeTensor& out, bool
     }
     const int type = type_code(w.scalar_type());
     const uint64_t ldw = (uint64_t)w.stride(0);
-    const uint64_t need =
-        ark_cuda_weight_grad_workspace(x.c(), dy.data_ptr(), ld, (uint64_t)n);
+    ark_act8 c = *x.c();
+    if (dy.scalar_type() != at::kHalf) c.wide = 0;   // BF16 has the range
+    const uint64_t need = ark_cuda_weight_grad_workspace(&c, dy.data_ptr(), ld, (uint64_t)n);
     Tensor ws;
     if (need) ws = fresh({(int64_t)need}, at::kByte, dy.device());
     check("ark_cuda_weight_grad",
-          ark_cuda_weight_grad(x.c(), dy.data_ptr(), type_code(dy.scalar_type()), ld, (uint64_t)n,
+          ark_cuda_weight_grad(&c, dy.data_ptr(), type_code(dy.scalar_type()), ld, (uint64_t)n,
                                w.data_ptr(), type, ldw, accumulate, need ? ws.data_ptr() : nullptr, need,
                                on.stream));
     return w;
@@ -248,8 +255,8 @@ py::object swiglu(const Tensor& a, const Tensor& b, const std::optional<std::str
     std::optional<Act8> ca, cb;
     if (checkpoint) {
         const int kind = kind_code(*checkpoint);
-        ca.emplace(rows, cols, kind, a.device());
-        cb.emplace(rows, cols, kind, a.device());
+        ca.emplace(rows, cols, kind, a.device(), a.scalar_type());
+        cb.emplace(rows, cols, kind, a.device(), a.scalar_type());
     }
     check("ark_cuda_swiglu",
           ark_cuda_swiglu(a.data_ptr(), la, b.data_ptr(), lb, type_code(a.scalar_type()), (uint64_t)rows,
@@ -281,7 +288,7 @@ py::tuple swiglu_backward(const Tensor& dy, const Act8& ca, const Act8& cb,
         db = fresh({rows, cols}, dy.scalar_type(), dy.device());
     }
     std::optional<Act8> cy;
-    if (checkpoint) cy.emplace(rows, cols, ca.kind(), dy.device());
+    if (checkpoint) cy.emplace(rows, cols, ca.kind(), dy.device(), dy.scalar_type());
     check("ark_cuda_swiglu_backward",
           ark_cuda_swiglu_backward(dy.data_ptr(), lg, type_code(dy.scalar_type()), ca.c(), cb.c(),
                                    da.data_ptr(), (uint64_t)da.stride(0), db.data_ptr(),
@@ -445,8 +452,8 @@ py::tuple qk_norm_rope(const Tensor& q, const MaybeTensor& k, const Tensor& gain
     std::optional<Act8> cq, ck;
     if (checkpoint) {
         const int kind = kind_code(*checkpoint);
-        cq.emplace(q.size(0), q.size(1) * q.size(2), kind, q.device());
-        if (k) ck.emplace(k->size(0), k->size(1) * k->size(2), kind, q.device());
+        cq.emplace(q.size(0), q.size(1) * q.size(2), kind, q.device(), q.scalar_type());
+        if (k) ck.emplace(k->size(0), k->size(1) * k->size(2), kind, q.device(), q.scalar_type());
     }
     check("ark_cuda_qk_norm_rope",
           ark_cuda_qk_norm_rope(&plan.c, &p.q, p.pk(), &p.out_q, p.pok(), type_code(q.scalar_type()),
@@ -535,16 +542,18 @@ scale: uint8 [rows, data.shape[1] / 32], the power-of-two scale of 32 columns as
        its exponent + 127 (255: the block held an infinity or a NaN and reads
        back as NaN).
 kind:  "e4m3" (4 significant bits at every size) or "int8" (a fixed step of 1/127
-       to 1/64 of the block's largest).)")
-        .def(py::init<const py::object&, const py::object&, int64_t, const std::string&>(), arg("data"),
-             arg("scale"), arg("cols"), arg("kind") = "e4m3")
+       to 1/64 of the block's largest).
+wide:  whether it may hold values that FP16 cannot: true of one packed from BF16 or
+       FP32 here; of bytes that a caller holds, the caller says so.)")
+        .def(py::init<const py::object&, const py::object&, int64_t, const std::string&, bool>(), arg("data"),
+             arg("scale"), arg("cols"), arg("kind") = "e4m3", arg("wide") = false)
         .def_static(
             "empty",
             [](int64_t rows, int64_t cols, const std::string& kind, const std::optional<at::Device>& device) {
                 const int code = kind_code(kind);
                 at::Device d = device ? *device : at::Device(at::kCUDA);
                 if (d.is_cuda() && !d.has_index()) d = at::Device(at::kCUDA, c10::cuda::current_device());
-                return Act8(rows, cols, code, d);
+                return Act8(rows, cols, code, d, at::kHalf);
             },
             arg("rows"), arg("cols"), arg("kind") = "e4m3", arg("device") = none,
             "Room for a checkpoint (its contents are whatever was there), in one allocation; data and\n"
@@ -556,6 +565,7 @@ kind:  "e4m3" (4 significant bits at every size) or "int8" (a fixed step of 1/12
         .def_property_readonly("cols", &Act8::cols)
         .def_property_readonly("pitch", &Act8::pitch)
         .def_property_readonly("kind", &Act8::kind_name)
+        .def_property_readonly("wide", &Act8::wide)
         .def_property_readonly("nbytes", &Act8::nbytes);
 
     py::class_<RopePlan>(m, "RopePlan", R"(The rotation of the first rotary_dim elements of each head.
@@ -586,7 +596,10 @@ Host memory only: made once, usable on every device and in graphs.)")
           "hold saturates at its largest.");
     m.def("weight_grad", &weight_grad, arg("x"), arg("dy"), arg("out") = none, arg("accumulate") = false,
           arg("dtype") = none, R"(dW [in, out_features] = X^T dY of y = x W, X [tokens, in] read from its
-checkpoint, dY [tokens, out_features] FP16 or BF16.
+checkpoint, dY [tokens, out_features] FP16 or BF16.  The products are of dY's type;
+FP16 dY with a checkpoint that is `wide` takes two products of BF16 (dY as the sum of
+two) and so keeps the checkpoint's range.  With FP16 dY and one that is not, a value
+above FP16's range becomes an infinity in dW.
 
 out: where to write (FP16, BF16 or FP32; for example a range of the gradient
      buffer viewed as [in, out_features]); default: a new tensor of `dtype`

@@ -4,8 +4,10 @@
 // Both operands have the summed dimension (tokens) as their slow one, so both
 // go to the tensor cores MN-major: a stage holds 64 tokens as rows of 128
 // bytes (64 columns), 8 rows to a 1024-byte swizzle atom; accumulators are FP32
-// in TMEM.  A byte of X becomes an FP16 / BF16 operand exactly (at most 8
-// significant bits times a power of two).
+// in TMEM.  A byte of X, at most 8 significant bits times a power of two, becomes a
+// BF16 operand exactly, and an FP16 one if X was FP16 (operand16).  FP16 dY with a
+// checkpoint of a wider type is brought to BF16 operands, whose range holds X: dY as
+// the sum of two of them, which holds its 11 bits, and so in two products (wide).
 //
 // Many tiles (pair_kernel): X is unpacked once into a 16-bit workspace, then
 // both operands come by TMA to pairs of CTAs with 256 x 256 tiles.  The grid is
@@ -446,7 +448,7 @@ __device__ __forceinline__ void fill_stages(const Args& a, uint32_t it0, uint32_
             // only while it is written
             uint4 lo[4], hi[4];
 #pragma unroll
-            for (int h = 0; h < 4; ++h) operand16<T, KIND>(q[p][h], sc[p][h], lo[h], hi[h]);
+            for (int h = 0; h < 4; ++h) operand16<T, KIND, true>(q[p][h], sc[p][h], lo[h], hi[h]);
             load(p);
             if (!(ok = warp_wait(smem_u32(empty + s), phase ^ 1u, gave_up))) break;
             const uint32_t at = stages + s * STAGE + atom * kAtom;
@@ -1043,37 +1045,25 @@ uint64_t ws_dy(uint64_t tokens, const void* dy, uint64_t lddy, uint64_t n) {
     return tma_rows(dy, lddy, n) ? 0 : tokens * realigned(n) * 2;
 }
 
-}  // namespace
-}  // namespace ark
-
-using namespace ark;
-
-extern "C" {
-
-uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
-                                        uint64_t n_out) {
-    if (!x || !x->rows || !x->cols || !n_out) return 0;
-    const Way w = way_of(x->rows, x->cols, n_out);
-    return w.x_bytes + w.partial_bytes + ws_dy(x->rows, dy, lddy, n_out);
+Out out_of(void* dw, int32_t type, uint64_t ld) {
+    return Out{dw, ld, type == ARK_TYPE_F32, type == ARK_TYPE_BF16,
+               aligned16(dw) && ld * type_size(type) % 16 == 0};
+}
+// a.partial's runs into a.out
+int add_runs(const Args& a, cudaStream_t s) {
+    static std::atomic<uint64_t> ready{0};
+    const uint64_t blocks = ((uint64_t)a.m * a.n_pad / 4 + 255) / 256, most = (uint64_t)sm_count() * 8;
+    return launch(runs_kernel, (uint32_t)(blocks < most ? blocks : most), 256, 0, 1, ready, s, a);
 }
 
-int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
-                         uint64_t n_out, void* dw, int32_t dw_type, uint64_t lddw,
-                         int32_t accumulate, void* workspace, uint64_t workspace_bytes,
-                         void* cuda_stream) {
-    const int rc = act8_check(x);
-    if (rc) return rc;
-    if (dy_type != ARK_TYPE_F16 && dy_type != ARK_TYPE_BF16) return ARK_E_UNSUPPORTED;
-    if (!type_size(dw_type)) return ARK_E_INVALID_ARG;
-    if (x->rows >= (1ull << 31) - kBK || n_out >= (1ull << 31) - 256) return ARK_E_INVALID_ARG;
-    if (x->cols > 1 && lddw < n_out) return ARK_E_INVALID_ARG;
-    if (x->cols == 0 || n_out == 0) return ARK_OK;
-    if (!dw || (x->rows && !dy)) return ARK_E_INVALID_ARG;
-    if (x->rows > 1 && lddy < n_out && lddy != 0) return ARK_E_INVALID_ARG;
-    const uint64_t e = type_size(dw_type);
-    if (!aligned_to(dw, e) || !aligned_to(dy, 2)) return ARK_E_MISALIGNED;
-    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+uint64_t need_of(const Way& w, const ark_act8* x, const void* dy, uint64_t lddy, uint64_t n) {
+    return w.x_bytes + w.partial_bytes + ws_dy(x->rows, dy, lddy, n);
+}
 
+// The gradient with operands of dY's type; arguments are checked.
+int product(const Way& w, const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
+            uint64_t n_out, void* dw, int32_t dw_type, uint64_t lddw, int32_t accumulate, uint8_t* ws,
+            cudaStream_t s) {
     Args a = {};
     a.x = x->data;
     a.scale = x->scale;
@@ -1083,8 +1073,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
     a.m = (uint32_t)x->cols;
     a.n = (uint32_t)n_out;
     a.iters = (a.tokens + kBK - 1) / kBK;
-    a.out = Out{dw, lddw, dw_type == ARK_TYPE_F32, dw_type == ARK_TYPE_BF16,
-                aligned16(dw) && lddw * e % 16 == 0};
+    a.out = out_of(dw, dw_type, lddw);
     a.accumulate = accumulate != 0;
     if (x->rows == 0) {
         if (accumulate) return ARK_OK;
@@ -1093,16 +1082,8 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
     }
 
-    const Way w = way_of(x->rows, x->cols, n_out);
-    const uint64_t need_dy = ws_dy(x->rows, dy, lddy, n_out);
-    const uint64_t need = w.x_bytes + w.partial_bytes + need_dy;
-    if (need) {
-        if (!workspace || workspace_bytes < need) return ARK_E_INVALID_ARG;
-        if (!aligned16(workspace)) return ARK_E_MISALIGNED;
-    }
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint64_t ld = lddy;
-    if (need_dy) {
+    if (ws_dy(x->rows, dy, lddy, n_out)) {
         ld = realigned(n_out);
         void* to = ws + w.x_bytes + w.partial_bytes;
         if (const int rc2 = realign_rows(dy, lddy, x->rows, a.n, to, ld, s)) return rc2;
@@ -1123,7 +1104,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         // more than 2048 tokens are summed in runs that the epilogue adds
         const uint32_t run = (a.iters + a.splits - 1) / a.splits;
         a.chunks = a.out.f32 ? (run + 31) / 32 : 1;
-        failed = ark_cuda_act8_unpack(x, ws, dy_type, a.pitch, cuda_stream);
+        failed = act8_operands(x, ws, dy_type, a.pitch, s);
         if (failed) return failed;
         CUtensorMap map_x;
         failed = encode(&map_x, dy_type, ws, x->rows, x->cols, a.pitch);
@@ -1131,9 +1112,7 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
         failed = dy_type == ARK_TYPE_F16 ? launch_pair<__half>(map_x, map, a, s)
                                      : launch_pair<__nv_bfloat16>(map_x, map, a, s);
         if (failed || !a.partial) return failed;
-        const uint64_t blocks = ((uint64_t)a.m * a.n_pad / 4 + 255) / 256, most = (uint64_t)sm_count() * 8;
-        static std::atomic<uint64_t> ready{0};
-        return launch(runs_kernel, (uint32_t)(blocks < most ? blocks : most), 256, 0, 1, ready, s, a);
+        return add_runs(a, s);
     }
     a.tiles_m = (a.m + kBM - 1) / kBM;
     a.tiles_n = (a.n + Few::kBN - 1) / Few::kBN;
@@ -1146,6 +1125,119 @@ int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uin
                                 : launch_few<__half, kInt8>(map, a, parts, s);
     return x->kind == kE4M3 ? launch_few<__nv_bfloat16, kE4M3>(map, a, parts, s)
                             : launch_few<__nv_bfloat16, kInt8>(map, a, parts, s);
+}
+
+// dY of FP16 as the sum of two BF16 numbers (8 bits and the 3 that are left; an infinity
+// or a NaN stays in the first): 8 columns per thread.
+__global__ void __launch_bounds__(256) halves_kernel(const __half* __restrict__ dy, uint64_t lddy,
+                                                     uint64_t rows, uint32_t cols, uint32_t per_row,
+                                                     __nv_bfloat16* __restrict__ hi,
+                                                     __nv_bfloat16* __restrict__ lo, uint64_t ld) {
+    const uint64_t total = rows * per_row;
+    const bool vec = aligned16(dy) && lddy % 8 == 0;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = i / per_row;
+        const uint32_t col = (uint32_t)(i - row * per_row) * 8;
+        float v[8], h[8];
+        load8(dy + row * lddy + col, (int)(cols - col), vec, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            h[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
+            v[j] = isfinite(h[j]) ? __fsub_rn(v[j], h[j]) : 0.0f;
+        }
+        store_vec<8>(hi + row * ld + col, h);
+        store_vec<8>(lo + row * ld + col, v);
+    }
+}
+
+// Workspace of wide(): both halves of dY, the FP32 gradient, then that of a product.
+struct Wide {
+    uint64_t ld, ldw, half, sums, inner;   // elements, elements, bytes
+    uint64_t bytes() const { return 2 * half + sums + inner; }
+};
+Wide wide_of(const Way& way, const ark_act8* x, uint64_t n) {
+    Wide w;
+    w.ld = realigned(n);
+    w.ldw = (n + 3) / 4 * 4;
+    w.half = x->rows * w.ld * 2;
+    w.sums = x->cols * w.ldw * 4;
+    w.inner = need_of(way, x, nullptr, w.ld, n);
+    return w;
+}
+// FP16 dY with a checkpoint that FP16 may not hold
+int wide(const Way& way, const ark_act8* x, const void* dy, uint64_t lddy, uint64_t n, void* dw,
+         int32_t dw_type, uint64_t lddw, int32_t accumulate, uint8_t* ws, cudaStream_t s) {
+    const Wide w = wide_of(way, x, n);
+    __nv_bfloat16* hi = reinterpret_cast<__nv_bfloat16*>(ws);
+    __nv_bfloat16* lo = reinterpret_cast<__nv_bfloat16*>(ws + w.half);
+    float* sums = reinterpret_cast<float*>(ws + 2 * w.half);
+    uint8_t* inner = ws + 2 * w.half + w.sums;
+    const uint32_t per = (uint32_t)(w.ld / 8);
+    const uint64_t blocks = (x->rows * per + 255) / 256, most = (uint64_t)sm_count() * 8;
+    halves_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
+        static_cast<const __half*>(dy), lddy, x->rows, (uint32_t)n, per, hi, lo, w.ld);
+    if (cudaGetLastError() != cudaSuccess) return ARK_E_CUDA;
+    int rc = product(way, x, lo, ARK_TYPE_BF16, w.ld, n, sums, ARK_TYPE_F32, w.ldw, 0, inner, s);
+    if (!rc) rc = product(way, x, hi, ARK_TYPE_BF16, w.ld, n, sums, ARK_TYPE_F32, w.ldw, 1, inner, s);
+    if (rc) return rc;
+    Args a = {};
+    a.m = (uint32_t)x->cols;
+    a.n = (uint32_t)n;
+    a.n_pad = (uint32_t)w.ldw;
+    a.splits = 1;
+    a.partial = sums;
+    a.out = out_of(dw, dw_type, lddw);
+    a.accumulate = accumulate != 0;
+    return add_runs(a, s);
+}
+
+}  // namespace
+}  // namespace ark
+
+using namespace ark;
+
+extern "C" {
+
+uint64_t ark_cuda_weight_grad_workspace(const ark_act8* x, const void* dy, uint64_t lddy,
+                                        uint64_t n_out) {
+    if (!x || !x->rows || !x->cols || !n_out) return 0;
+    const Way w = way_of(x->rows, x->cols, n_out);
+    const uint64_t need = need_of(w, x, dy, lddy, n_out);
+    if (!x->wide) return need;
+    const uint64_t more = wide_of(w, x, n_out).bytes();   // dY may be FP16
+    return need > more ? need : more;
+}
+
+int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_type, uint64_t lddy,
+                         uint64_t n_out, void* dw, int32_t dw_type, uint64_t lddw,
+                         int32_t accumulate, void* workspace, uint64_t workspace_bytes,
+                         void* cuda_stream) {
+    const int rc = act8_check(x);
+    if (rc) return rc;
+    if (dy_type != ARK_TYPE_F16 && dy_type != ARK_TYPE_BF16) return ARK_E_UNSUPPORTED;
+    if (!type_size(dw_type)) return ARK_E_INVALID_ARG;
+    if (x->rows >= (1ull << 31) - kBK || n_out >= (1ull << 31) - 256) return ARK_E_INVALID_ARG;
+    if (x->cols > 1 && lddw < n_out) return ARK_E_INVALID_ARG;
+    if (x->cols == 0 || n_out == 0) return ARK_OK;
+    if (!dw || (x->rows && !dy)) return ARK_E_INVALID_ARG;
+    if (x->rows > 1 && lddy < n_out && lddy != 0) return ARK_E_INVALID_ARG;
+    const uint64_t e = type_size(dw_type);
+    if (!aligned_to(dw, e) || !aligned_to(dy, 2)) return ARK_E_MISALIGNED;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+
+    const Way w = x->rows ? way_of(x->rows, x->cols, n_out) : Way{};
+    const bool in_halves = x->rows && x->wide && dy_type == ARK_TYPE_F16;
+    const uint64_t need = in_halves ? wide_of(w, x, n_out).bytes()
+                          : x->rows ? need_of(w, x, dy, lddy, n_out)
+                                    : 0;
+    if (need) {
+        if (!workspace || workspace_bytes < need) return ARK_E_INVALID_ARG;
+        if (!aligned16(workspace)) return ARK_E_MISALIGNED;
+    }
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (in_halves) return wide(w, x, dy, lddy, n_out, dw, dw_type, lddw, accumulate, ws, s);
+    return product(w, x, dy, dy_type, lddy, n_out, dw, dw_type, lddw, accumulate, ws, s);
 }
 
 }  // extern "C"

@@ -418,7 +418,8 @@ typedef struct ark_act8 {
     uint8_t* scale;
     uint64_t rows, cols;
     int32_t  kind;      /* ARK_ACT8_* */
-    uint32_t reserved;
+    uint32_t wide;      /* not 0: may hold values that F16 cannot, as packed from
+                           BF16 or F32 (ark_cuda_weight_grad); the caller's to set */
 } ark_act8;
 
 ARK_API uint64_t ark_cuda_act8_pitch(uint64_t cols);
@@ -438,6 +439,13 @@ ARK_API int ark_cuda_act8_unpack(const ark_act8* in, void* y, int32_t type, uint
  * tensor's range of ark_cuda_opt_grad_buffer with dy carrying the loss
  * scale; a sum that F16 cannot hold becomes an infinity, which the step
  * takes for an overflow.  The result is the same bits on every call.
+ * The operands are of dy's type.  BF16 holds every x (up to 2^128, which
+ * saturates).  With F16 and x->wide == 0, x is rounded to F16: exact for a
+ * checkpoint of F16 numbers; a magnitude above 65536 becomes an infinity and
+ * shows in dw, one below 2^-25 becomes 0.  With F16 and x->wide != 0, x
+ * keeps its range: dy is taken apart into two BF16 operands whose sum it is,
+ * at the price of two products and a larger workspace (needed with F16 alone:
+ * with a BF16 dy, clear `wide` before asking for the size).
  * workspace: 16-byte aligned, ark_cuda_weight_grad_workspace bytes on the
  * current device: x in 16 bits for large gradients, FP32 sums where their
  * tokens are split, dy again where its rows are not 16-byte aligned; 0, and

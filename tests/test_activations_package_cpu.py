@@ -45,3 +45,23 @@ def test_no_view_of_a_closed_optimizers_buffer():
     opt.close()
     with pytest.raises(RuntimeError, match="grad_buffer"):
         opt.grad_view("l0.w1")
+
+
+def test_wide_checkpoints_need_room_for_both_halves():
+    """FP16 dY with a checkpoint of a wider type: the workspace holds dY twice, and the call says
+    so when it does not; a BF16 dY needs none of it."""
+    import ctypes
+
+    from ark_b200 import _lib
+    L, p = _lib.lib(), 0x7F0000001000      # an aligned address that nothing reads
+    narrow, wide = (_lib.Act8(p, p, 64, 100, 0, w) for w in (0, 1))
+    need = [L.ark_cuda_weight_grad_workspace(ctypes.byref(x), p, 64, 64) for x in (narrow, wide)]
+    assert need[1] >= need[0] + 2 * 64 * 64 * 2 + 100 * 64 * 4
+
+    def call(x, ws, nbytes, dy_type=0):
+        return L.ark_cuda_weight_grad(ctypes.byref(x), p, dy_type, 64, 64, p, 0, 64, 0, ws, nbytes, None)
+
+    assert call(wide, None, 0) == -1 and call(wide, p, need[1] - 1) == -1
+    assert call(wide, p + 8, need[1]) == -2
+    if need[0]:
+        assert call(wide, p, need[0] - 1, dy_type=1) == -1
