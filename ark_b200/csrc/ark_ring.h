@@ -18,12 +18,11 @@ namespace ark {
 template <uint32_t N>
 struct Ring {
     uint32_t at = 0, parity = 0;
-    bool ok = true;
-    // waited(barrier, parity): whether the phase has completed
-    template <class F>
-    ARK_HD bool wait(F waited) {
-        ok = ok && waited(at, parity);
-        return ok;
+    // lost(): whether a wait has run out; waited(barrier, parity): whether the phase has
+    // completed, and if not, lost() from then on
+    template <class L, class F>
+    ARK_HD bool wait(L lost, F waited) const {
+        return !lost() && waited(at, parity);
     }
     ARK_HD void next() {
         if (++at == N) at = 0, parity ^= 1u;

@@ -45,6 +45,14 @@ constexpr int kPairEpiWarps = 16, kPairThreads = (kPairEpiWarps + 2) * 32;
 constexpr int kAtom = kBK * 128;              // 64 tokens x 64 columns of 16 bits
 constexpr int kABytes = kBM / 64 * kAtom;
 constexpr int kAhead = 2;                     // steps of a team in flight
+// The tensor cores add 16 tokens at a time to a sum that is cut off to FP32, not
+// rounded: each addition may lose a unit of the last place, 2^-23 of the sum, and
+// always towards zero.  So one accumulator takes a bounded run of 64-token steps, and
+// runs are added by FP32 additions that round.  FP32 gradients: 32 steps, 128
+// additions.  16-bit ones: 128 steps, whose 512 additions lose at most 2^-14, an
+// eighth of FP16's half step.
+constexpr uint32_t kRun32 = 32, kRun16 = 128;
+constexpr uint32_t kFewRuns = 4;              // accumulators of few_kernel
 constexpr uint32_t kSleepNs = 1000000;
 constexpr long long kWaitClocks = 4000000000ll;   // 2 s
 
@@ -345,30 +353,35 @@ __device__ __forceinline__ void out_row4(const Out& o, uint32_t m, uint32_t n, u
 // A warp's 32 x 16 block of sums, staged in shared memory, to rows row0 on and
 // columns col0 on of an m x n output.  Through the staging four lanes come to
 // share a row, so that a store fills whole sectors of 8 rows; element by element
-// (rows on any boundary) 16 lanes share one.
-template <class O>
+// (rows on any boundary) 16 lanes share one.  AHEAD: of a lane's 4 rows, how many are
+// read before the first is written.
+template <int AHEAD, class O>
 __device__ __forceinline__ void out_block(O* p, const Out& o, uint32_t m, uint32_t n, uint32_t row0,
                                           uint32_t col0, const float4* staged, uint32_t lane,
                                           bool accumulate) {
     if (o.vec && col0 + 16 <= n) {
         const uint32_t r0 = lane / 4;
         p += (uint64_t)(row0 + r0) * o.ld + col0 + (lane & 3) * 4;
-        float old[4][4];
-        if (accumulate) {   // all reads before the first write
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (row0 + r0 + i * 8 < m) load_vec<4>(p + (uint64_t)(i * 8) * o.ld, old[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t r = r0 + i * 8;
-            const float4 f = staged[r * 4 + ((lane & 3) ^ (r >> 1 & 3))];
-            float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll 1
+        for (int h = 0; h < 4; h += AHEAD) {
+            float old[AHEAD][4];
             if (accumulate) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], old[i][j]);
+                for (int i = 0; i < AHEAD; ++i)
+                    if (row0 + r0 + (h + i) * 8 < m) load_vec<4>(p + (uint64_t)(i * 8) * o.ld, old[i]);
             }
-            if (row0 + r < m) store_vec<4>(p + (uint64_t)(i * 8) * o.ld, v);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t r = r0 + (h + i) * 8;
+                const float4 f = staged[r * 4 + ((lane & 3) ^ (r >> 1 & 3))];
+                float v[4] = {f.x, f.y, f.z, f.w};
+                if (accumulate) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], old[i][j]);
+                }
+                if (row0 + r < m) store_vec<4>(p + (uint64_t)(i * 8) * o.ld, v);
+            }
+            p += (uint64_t)(AHEAD * 8) * o.ld;
         }
         return;
     }
@@ -377,13 +390,13 @@ __device__ __forceinline__ void out_block(O* p, const Out& o, uint32_t m, uint32
     if (col0 + e >= n) return;
     p += (uint64_t)(row0 + r0) * o.ld + col0 + e;
 #pragma unroll 1
-    for (uint32_t h = 0; h < 32; h += 8, p += 8 * o.ld) {
-        float old[4];
+    for (uint32_t h = 0; h < 32; h += 2 * AHEAD, p += 2 * AHEAD * o.ld) {
+        float old[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < AHEAD; ++i)
             old[i] = accumulate && row0 + r0 + h + 2 * i < m ? Elem<O>::to_f(p[(uint64_t)(2 * i) * o.ld]) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
             const uint32_t r = r0 + h + 2 * i;
             const float v = one[(r * 4 + (e / 4 ^ (r >> 1 & 3))) * 4 + e % 4];
             if (row0 + r < m)
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&tmem_at)),
-                     "r"(4 * S::kBN)
+                     "r"(kFewRuns * S::kBN)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -634,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                     "r"(4 * S::kBN));
+                     "r"(kFewRuns * S::kBN));
     }
 }
 
@@ -653,8 +666,11 @@ __device__ __forceinline__ void pair_tile(const Args& a, uint32_t t, uint32_t& m
     m = band * 8 + (at - n * high);
 }
 
-// RUNS: FP32 sums of several runs of an item's tokens, added by the epilogue.
-template <class T, bool RUNS>
+// RUNS: several runs of an item's tokens, whose FP32 sums the epilogue adds, and writes
+// as FP32 (the partial sums too) or as the output's 16-bit type: two kernels, since all
+// three types in one spilled twice as many registers.
+enum Runs { kOneRun, kRunsTo32, kRunsTo16 };
+template <class T, Runs RUNS>
 __global__ void __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
                 const Args a) {
@@ -777,9 +793,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                          warp * 128;
         Ring<2> acc;   // a wait that ran out makes every tile from there on NaN
         auto wait = [&] {
-            return acc.wait([&](uint32_t b, uint32_t parity) {
-                return warp_wait<kSleep>(smem_u32(acc_full + b), parity, gave_up);
-            });
+            return acc.wait([&] { return __any_sync(0xFFFFFFFFu, *gave_up); },
+                            [&](uint32_t b, uint32_t parity) {
+                                return warp_wait<kSleep>(smem_u32(acc_full + b), parity, gave_up);
+                            });
         };
         for (uint32_t i = blockIdx.x / 2; i < items; i += pairs) {
             uint32_t m, n, it0, it1;
@@ -791,24 +808,28 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 out = Out{a.partial + (uint64_t)run * a.m * a.n_pad, a.n_pad, 1, 0, 1};
                 accumulate = false;
             }
-            // 16 columns from c on, of which a lane has one row
-            auto put = [&](uint32_t c, const float* v, bool ok) {
+            // a lane's 16 columns of one row, among the warp's 32 rows
+            auto stage = [&](const float* v, bool ok) {
                 const float none = __uint_as_float(0x7FC00000u);
-                __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     staged[lane * 4 + (j ^ (lane >> 1 & 3))] =
                         ok ? make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3])
                            : make_float4(none, none, none, none);
-                __syncwarp();
+            };
+            // what is staged, as the columns from c on
+            auto put = [&](uint32_t c) {
+                constexpr int kAhead = RUNS == kOneRun ? 4 : 2;
                 const uint32_t col0 = n * S::kBN + c;
-                if (RUNS || out.f32)
-                    out_block(static_cast<float*>(out.p), out, a.m, a.n, row0, col0, staged, lane, accumulate);
+                if (RUNS == kRunsTo32 || (RUNS == kOneRun && out.f32))
+                    out_block<kAhead>(static_cast<float*>(out.p), out, a.m, a.n, row0, col0, staged, lane,
+                                      accumulate);
                 else if (out.bf16)
-                    out_block(static_cast<__nv_bfloat16*>(out.p), out, a.m, a.n, row0, col0, staged, lane,
-                              accumulate);
+                    out_block<kAhead>(static_cast<__nv_bfloat16*>(out.p), out, a.m, a.n, row0, col0, staged,
+                                      lane, accumulate);
                 else
-                    out_block(static_cast<__half*>(out.p), out, a.m, a.n, row0, col0, staged, lane, accumulate);
+                    out_block<kAhead>(static_cast<__half*>(out.p), out, a.m, a.n, row0, col0, staged, lane,
+                                      accumulate);
             };
             auto next = [&] {
                 fence_before();
@@ -816,7 +837,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if (lane == 0) bar_arrive_at(bar_of(smem_u32(acc_empty + acc.at), 0));
                 acc.next();
             };
-            if constexpr (!RUNS) {
+            if constexpr (RUNS == kOneRun) {
                 const bool ok = wait();
                 fence_after();
 #pragma unroll 1
@@ -824,14 +845,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     float v[16];
                     tmem_ld16(tmem + acc.at * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
-                    put(c, v, ok);
+                    __syncwarp();
+                    stage(v, ok);
+                    __syncwarp();
+                    put(c);
                 }
                 next();
             } else {
                 // the runs' sums are added in registers
-                float sum[kCols / 16][16];
+                float sum[kCols / 16][16] = {};
+                bool ok;   // the last wait's: it is false after a lost one
+#pragma unroll 1
                 for (uint32_t k = 0; k < a.chunks; ++k) {
-                    wait();
+                    ok = wait();
                     fence_after();
 #pragma unroll
                     for (int c = 0; c < kCols / 16; ++c) {
@@ -839,12 +865,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         tmem_ld16(tmem + acc.at * S::kBN + (quarter * 32 << 16) + c0 + c * 16,
                                   reinterpret_cast<uint32_t*>(v));
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) sum[c][j] = k ? __fadd_rn(sum[c][j], v[j]) : v[j];
+                        for (int j = 0; j < 16; ++j) sum[c][j] = __fadd_rn(sum[c][j], v[j]);
                     }
                     next();
                 }
+                // unrolled, four copies of the output's code spilled the sums
+#pragma unroll 1
+                for (int k = 0; k < kCols / 16; ++k) {
+                    __syncwarp();
 #pragma unroll
-                for (int c = 0; c < kCols / 16; ++c) put(c0 + c * 16, sum[c], acc.ok);
+                    for (int c = 0; c < kCols / 16; ++c)
+                        if (c == k) stage(sum[c], ok);
+                    __syncwarp();
+                    put(c0 + k * 16);
+                }
             }
         }
     }
@@ -949,12 +983,15 @@ int launch_few(const CUtensorMap& map, const Args& a, uint32_t parts, cudaStream
 }
 template <class T>
 int launch_pair(const CUtensorMap& x, const CUtensorMap& dy, const Args& a, cudaStream_t s) {
-    static std::atomic<uint64_t> ready{0}, runs{0};
+    static std::atomic<uint64_t> ready[3];
     const uint32_t most = (uint32_t)sm_count() / 2, items = a.tiles * a.splits;
     const uint32_t pairs = items < most ? items : most;
-    if (a.chunks > 1)
-        return launch(pair_kernel<T, true>, pairs * 2, kPairThreads, Pair::kSmem, 2, runs, s, x, dy, a);
-    return launch(pair_kernel<T, false>, pairs * 2, kPairThreads, Pair::kSmem, 2, ready, s, x, dy, a);
+    auto run = [&](auto kernel, Runs r) {
+        return launch(kernel, pairs * 2, kPairThreads, Pair::kSmem, 2, ready[r], s, x, dy, a);
+    };
+    if (a.chunks == 1) return run(pair_kernel<T, kOneRun>, kOneRun);
+    if (a.partial || a.out.f32) return run(pair_kernel<T, kRunsTo32>, kRunsTo32);
+    return run(pair_kernel<T, kRunsTo16>, kRunsTo16);
 }
 
 // [rows, cols] of 16-bit elements, ld apart, in boxes of 64 columns by 64 rows
@@ -1024,6 +1061,7 @@ Way way_of(uint64_t tokens, uint64_t m, uint64_t n) {
     Way w = {false, 1, 1, 0, 0};
     uint64_t best = ~0ull;
     for (uint32_t p = 1; p <= 8 && p <= iters; p *= 2) {
+        if (ceil_div(iters, p) > kFewRuns * kRun32) continue;   // its accumulators take no more
         const uint64_t t = ceil_div(few, few_fit(p)) * (6500 + 370 * ceil_div(iters, p));
         if (t < best) best = t, w.parts = p;
     }
@@ -1100,10 +1138,8 @@ int product(const Way& w, const ark_act8* x, const void* dy, int32_t dy_type, ui
         a.splits = w.splits;
         a.partial = w.partial_bytes ? reinterpret_cast<float*>(ws + w.x_bytes) : nullptr;
         a.n_pad = (a.n + 3) / 4 * 4;
-        // the tensor cores' FP32 sums are cut off, not rounded: FP32 gradients of
-        // more than 2048 tokens are summed in runs that the epilogue adds
-        const uint32_t run = (a.iters + a.splits - 1) / a.splits;
-        a.chunks = a.out.f32 ? (run + 31) / 32 : 1;
+        const uint32_t run = (a.iters + a.splits - 1) / a.splits, most = a.out.f32 ? kRun32 : kRun16;
+        a.chunks = (run + most - 1) / most;
         failed = act8_operands(x, ws, dy_type, a.pitch, s);
         if (failed) return failed;
         CUtensorMap map_x;
@@ -1119,7 +1155,7 @@ int product(const Way& w, const ark_act8* x, const void* dy, int32_t dy_type, ui
     a.tiles = a.tiles_m * a.tiles_n;
     const uint32_t parts = w.parts;
     a.chunks = a.iters / parts / 16;
-    a.chunks = a.chunks < 1 ? 1 : a.chunks > 4 ? 4 : a.chunks;
+    a.chunks = a.chunks < 1 ? 1 : a.chunks > kFewRuns ? kFewRuns : a.chunks;   // of at most kRun32 steps
     if (dy_type == ARK_TYPE_F16)
         return x->kind == kE4M3 ? launch_few<__half, kE4M3>(map, a, parts, s)
                                 : launch_few<__half, kInt8>(map, a, parts, s);

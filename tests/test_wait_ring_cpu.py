@@ -25,13 +25,14 @@ int main(int, char** argv) {
     Barrier b[2];
     b[0].last = atoi(argv[2]), b[1].last = atoi(argv[3]);
     ark::Ring<2> r;
+    bool lost = false;
     for (unsigned i = 0; i < items; ++i) {
-        const bool ok = r.wait([&](unsigned at, unsigned parity) {
+        const bool ok = r.wait([&] { return lost; }, [&](unsigned at, unsigned parity) {
             // the writer completes the next phase as soon as the reader waits, until it stops
             if (!b[at].passed(parity) && b[at].done < b[at].last) ++b[at].done;
-            return b[at].passed(parity);
+            lost = !b[at].passed(parity);
+            return !lost;
         });
-        if (ok != r.ok) return 1;
         putchar(ok ? '1' : '0');
         r.next();
     }
