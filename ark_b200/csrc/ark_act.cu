@@ -391,8 +391,12 @@ __device__ __forceinline__ double held_one(const uint8_t* data, const uint8_t* s
     return (double)__fmul_rn(v[0], scale_of(scale[at >> 5]));
 }
 // How many FP32 steps y is from the middle between two values of a 16-bit type.
+// FP16 drops 13 of the 24 bits, and below 2^-14, among its subnormals, one more for each
+// power of two; at 26 nothing is left that could round to its smallest.
 __device__ __forceinline__ uint32_t from_tie(float y, __half) {
-    const int d = (int)(__float_as_uint(y) & 0x1FFFu) - 0x1000;
+    const uint32_t bits = __float_as_uint(y), e = bits >> 23 & 255u;
+    const uint32_t half = 1u << (min(max(126u, e + 13u) - e, 26u) - 1u);   // e: 2^-14 has 113
+    const int d = (int)((bits & 0x7FFFFFu | 0x800000u) & (2 * half - 1u)) - (int)half;
     return (uint32_t)abs(d);
 }
 __device__ __forceinline__ uint32_t from_tie(float y, __nv_bfloat16) {
