@@ -390,18 +390,11 @@ __device__ __forceinline__ double held_one(const uint8_t* data, const uint8_t* s
     bytes4<KIND>(data[at], v);
     return (double)__fmul_rn(v[0], scale_of(scale[at >> 5]));
 }
-// How many FP32 steps y is from the middle between two values of a 16-bit type.
-// FP16 drops 13 of the 24 bits, and below 2^-14, among its subnormals, one more for each
-// power of two; at 26 nothing is left that could round to its smallest.
-__device__ __forceinline__ uint32_t from_tie(float y, __half) {
-    const uint32_t bits = __float_as_uint(y), e = bits >> 23 & 255u;
-    const uint32_t half = 1u << (min(max(126u, e + 13u) - e, 26u) - 1u);   // e: 2^-14 has 113
-    const int d = (int)((bits & 0x7FFFFFu | 0x800000u) & (2 * half - 1u)) - (int)half;
-    return (uint32_t)abs(d);
-}
-__device__ __forceinline__ uint32_t from_tie(float y, __nv_bfloat16) {
-    const int d = (int)(__float_as_uint(y) & 0xFFFFu) - 0x8000;
-    return (uint32_t)abs(d);
+// Whether y rounds to two values of T when it is off by a factor of up to `most`.
+template <class T>
+__device__ __forceinline__ bool splits(float y, float most) {
+    const uint32_t w = narrow2(__fmul_rn(y, most), __fmul_rn(y, __fsub_rn(2.0f, most)), T());
+    return __byte_perm(w, w, 0x1032) != w;
 }
 
 // With y8, the product is remade, rounded to T as the forward's was, and
@@ -409,7 +402,8 @@ __device__ __forceinline__ uint32_t from_tie(float y, __nv_bfloat16) {
 // product of two 8-bit values often lies next to a border of T, and once rounded
 // next to one of the 8-bit grid, where the last bit of FP32 would decide by a whole
 // step: values within FP32's error of a border of T, about one in 500, are made
-// again in 64 bits and rounded to FP32.
+// again in 64 bits and rounded to FP32.  Rounding both ends of the error finds the
+// borders of every size, those of FP16's subnormals too.
 template <class T, int KIND, bool REMAKE>
 __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
     const T* dy, uint64_t lddy, const uint8_t* __restrict__ a8, const uint8_t* __restrict__ sa,
@@ -439,10 +433,12 @@ __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
             const float slope = __fmul_rn(s, __fmaf_rn(u[j], rest, 1.0f));
             o[j] = __fmul_rn(t, v[j]);
             if constexpr (REMAKE && !std::is_same<T, float>::value) {
-                // exp(-|a|) is off by 2 + 1.2 |a| ulps, of which `rest` reaches s; the
-                // sum, the reciprocal and three products add 4, the mantissa doubles
-                const float ulps = __fmaf_rn(__fmaf_rn(2.4f, fabsf(u[j]), 4.0f), rest, 8.0f);
-                near |= (float)from_tie(o[j], T()) <= ulps ? 1u << j : 0u;
+                // exp(-|a|) is off by 2 + 1.2 |a| ulps of 2^-23, of which `rest` reaches s;
+                // the sum, the reciprocal and three products add 4, the test itself 1
+                constexpr float kUlp = 1.0f / 8388608.0f;
+                const float most = __fmaf_rn(__fmaf_rn(1.2f * kUlp, fabsf(u[j]), 2 * kUlp), rest,
+                                             1.0f + 5 * kUlp);
+                near |= splits<T>(o[j], most) ? 1u << j : 0u;
             }
             u[j] = __fmul_rn(__fmul_rn(d[j], v[j]), slope);
             v[j] = __fmul_rn(d[j], t);
