@@ -341,8 +341,12 @@ __global__ void __launch_bounds__(kThreads) realign_kernel(const __half* __restr
 // silu(a) = a * s with s = 1 / (1 + exp(-a)); its slope is s * (1 + a * (1 - s)).
 // From e = exp(-|a|) <= 1, which can underflow but not overflow, both s and
 // 1 - s come without cancellation and keep their small end.
+// T: what the result is rounded to.  For a 16-bit type the fast exponential, off by
+// 2 + 1.2 |a| ulps of FP32, is far below its half step; FP32 results take the full one
+// (1 ulp).  The reciprocal is off by 1.
+template <class T>
 __device__ __forceinline__ void sigmoid(float a, float& s, float& rest) {
-    const float e = __expf(-fabsf(a));
+    const float e = std::is_same<T, float>::value ? expf(-fabsf(a)) : __expf(-fabsf(a));
     float r;   // of 1 to 2
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
     const float t = __fmul_rn(e, r);
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_kernel(
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             float s, rest;
-            sigmoid(u[j], s, rest);
+            sigmoid<T>(u[j], s, rest);
             u[j] = __fmul_rn(__fmul_rn(u[j], s), v[j]);
         }
         cy.set(u);
@@ -404,8 +408,9 @@ __device__ __forceinline__ bool splits(float y, float most) {
 // step: values within FP32's error of a border of T, about one in 500, are made
 // again in 64 bits and rounded to FP32.  Rounding both ends of the error finds the
 // borders of every size, those of FP16's subnormals too.
+// Blocks an SM: what 80 and 64 registers allow, without spills.
 template <class T, int KIND, bool REMAKE>
-__global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
+__global__ void __launch_bounds__(kThreads, REMAKE ? 3 : 4) swiglu_back_kernel(
     const T* dy, uint64_t lddy, const uint8_t* __restrict__ a8, const uint8_t* __restrict__ sa,
     const uint8_t* __restrict__ b8, const uint8_t* __restrict__ sb, uint64_t rows, uint32_t cols,
     uint32_t per_row, int lie, T* da, uint64_t ldda, T* db, uint64_t lddb,
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(kThreads) swiglu_back_kernel(
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             float s, rest;
-            sigmoid(u[j], s, rest);
+            sigmoid<T>(u[j], s, rest);
             const float t = __fmul_rn(u[j], s);
             const float slope = __fmul_rn(s, __fmaf_rn(u[j], rest, 1.0f));
             o[j] = __fmul_rn(t, v[j]);

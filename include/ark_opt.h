@@ -461,7 +461,8 @@ ARK_API int ark_cuda_weight_grad(const ark_act8* x, const void* dy, int32_t dy_t
                                  int32_t accumulate, void* workspace, uint64_t workspace_bytes,
                                  void* cuda_stream);
 
-/* y = silu(a) * b, [rows, cols].  With a8 and b8 (both or neither), a and b
+/* y = silu(a) * b, [rows, cols], made in FP32 and rounded once to `type` (an
+ * F32 y is off by at most 2^-21 of itself).  With a8 and b8 (both or neither), a and b
  * are checkpointed in the same pass.  y may be a or b. */
 ARK_API int ark_cuda_swiglu(const void* a, uint64_t lda, const void* b, uint64_t ldb, int32_t type,
                             uint64_t rows, uint64_t cols, void* y, uint64_t ldy,
