@@ -249,15 +249,27 @@ __device__ __forceinline__ void unit_floats(const float* p, const U& u, uint64_t
 }
 
 // cos and sin (times the plan's gain) of a unit's VEC rotated pairs
-template <int VEC>
+// T: what the result is rounded to.  FP32 holds 24 of the turn's 32 bits, 2^-25 of a
+// half turn, which is nothing beside a 16-bit result's half step; for an FP32 result
+// the 8 bits below turn it on by an angle too small for more than its first power.
+template <class T, int VEC>
 struct Turn {
     float c[VEC], s[VEC];
     __device__ __forceinline__ void set(const Args& a, const uint64_t* turns, int64_t p) {
+        constexpr float kHalfTurn = 4.656612873077392578125e-10f;   // 2^-31
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             // the top 32 bits of the turn, signed: [-1/2, 1/2) of a turn
             const int32_t top = (int32_t)(((uint64_t)p * turns[i]) >> 32);
-            sincospif(__fmul_rn((float)top, 4.656612873077392578125e-10f), &s[i], &c[i]);
+            if constexpr (std::is_same<T, float>::value) {
+                sincospif(__fmul_rn((float)(top & ~255), kHalfTurn), &s[i], &c[i]);
+                const float on = __fmul_rn((float)(top & 255), 3.14159265f * kHalfTurn);
+                const float turned = __fmaf_rn(c[i], on, s[i]);
+                c[i] = __fmaf_rn(-s[i], on, c[i]);
+                s[i] = turned;
+            } else {
+                sincospif(__fmul_rn((float)top, kHalfTurn), &s[i], &c[i]);
+            }
             c[i] = __fmul_rn(c[i], a.plan.gain);
             s[i] = __fmul_rn(a.inverse ? -s[i] : s[i], a.plan.gain);
         }
@@ -414,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, NU == 1 ? kBlocksPerSm : 4) forward_
     const uint64_t tasks = warp_tasks(a, a.splits), stride = (uint64_t)gridDim.x * (kThreads / 32);
     for (uint64_t w = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < tasks; w += stride) {
         const Task k(a, group, w, heads, a.splits);
-        Turn<VEC> turn[NU];
+        Turn<T, VEC> turn[NU];
 #pragma unroll
         for (int n = 0; n < NU; ++n)
             if (u[n].turned && u[n].h1) turn[n].set(a, turns + u[n].at, k.p);
@@ -636,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, kBackPerSm)
             col += dim;
         };
         load(0);
-        Turn<VEC> turn[NU];
+        Turn<T, VEC> turn[NU];
 #pragma unroll
         for (int n = 0; n < NU; ++n)
             if (u[n].turned && u[n].h1) turn[n].set(a, turns + u[n].at, k.p);

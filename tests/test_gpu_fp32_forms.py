@@ -31,3 +31,23 @@ def test_swiglu(kind):
     # a (1 - s) by 3 of its own size
     size = (G * B).abs() * s * (5 * (1 + A * (1 - s)).abs() + 3 * (A * (1 - s)).abs())
     assert ((da.cpu().double() - G * B * slope).abs() <= ULP * size + tiny(A, G * B)).all()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_angles_near_quarter_turns(layout):
+    """Pairs (1, 0) rotate into (cos, sin).  sincospi is off by 2 ulps, a turn by its 2^-32 (its
+    lower bits are cut) and by a position's 2^-64 of a turn; small cosines and sines show it."""
+    rot = 64
+    plan = ab.RopePlan(rot, layout=layout, base=10000.0)
+    freq, _ = ref.frequencies(rot)
+    pos = torch.arange(0, 1 << 22, 37)
+    q = torch.zeros(pos.numel(), 1, rot)
+    i1, i2 = (slice(0, 32), slice(32, 64)) if layout == "half" else (slice(0, 64, 2), slice(1, 64, 2))
+    q[..., i1] = 1
+    y = ab.rope(q.cuda(), None, plan, pos.cuda())[0].cpu().double()[:, 0]
+    angle = pos.double().view(-1, 1) * freq
+    # in 64 bits the angle is off by 2^-53 of itself, and the plan by 3.41e-19 a position
+    slack = 2 * 3.1416 * 2.0 ** -32 + angle * 2.0 ** -52 + pos.double().view(-1, 1) * 3.42e-19
+    for got, want in ((y[:, i1], torch.cos(angle)), (y[:, i2], torch.sin(angle))):
+        # two roundings after sincospi's: the turn on, and the product with 1
+        assert ((got - want).abs() <= (2 * ULP + 2 * 2.0 ** -24) * want.abs() + slack).all()
