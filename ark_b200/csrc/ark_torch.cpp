@@ -348,6 +348,7 @@ struct Positions {
             bad_value("positions: expected contiguous [" + std::to_string(tokens) + "], got " + shape_of(t));
         p = t.data_ptr();
         type = type_code(t.scalar_type());
+        if (!p) seq = 1;   // no tokens: torch gives no memory, and the call takes no positions for a length
     }
 };
 
