@@ -743,12 +743,12 @@ __global__ void __launch_bounds__(kThreads) gains_kernel(const float* __restrict
     const uint32_t i = is_q ? at : at - dim;
     if (i >= dim) return;
     const uint32_t lo = is_q ? 0 : q_blocks, hi = is_q ? q_blocks : blocks;
-    if (lo == hi) return;
+    void* out = is_q ? dgq : dgk;
+    if (!out) return;   // no such gain; one of no heads gets zero
     float s = 0.0f;
     for (uint32_t b = lo + lane; b < hi; b += 32) s = __fadd_rn(s, partial[(uint64_t)b * dim + i]);
     s = group_sum<32>(s, 32);
     if (lane) return;
-    void* out = is_q ? dgq : dgk;
     if (accumulate) s = __fadd_rn(s, gain_at(out, type, i));
     if (type == ARK_TYPE_F32)
         static_cast<float*>(out)[i] = s;
@@ -1114,11 +1114,17 @@ int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* d
     if (!aligned_to(gain_q, type_size(gain_type)) || !aligned_to(gain_k, type_size(gain_type)) ||
         !aligned_to(dgain_q, type_size(dgain_type)) || !aligned_to(dgain_k, type_size(dgain_type)))
         return ARK_E_MISALIGNED;
-    if (a.q.heads + a.k.heads == 0) return ARK_OK;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    if (!dk) dgain_k = nullptr;
+    auto sum_gains = [&](uint32_t blocks) {
+        gains_kernel<<<(2 * (unsigned)dim * 32 + kThreads - 1) / kThreads, kThreads, 0, s>>>(
+            a.partial, a.q_blocks, blocks, (uint32_t)dim, dgain_q, dgain_k, dgain_type, accumulate != 0);
+        return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+    };
+    if (a.q.heads + a.k.heads == 0) return accumulate || (!dgain_q && !dgain_k) ? ARK_OK : sum_gains(0);
     if (!workspace || workspace_bytes < ark_cuda_qk_norm_rope_workspace(dim)) return ARK_E_INVALID_ARG;
     if (!aligned_to(workspace, 4)) return ARK_E_MISALIGNED;
     a.partial = static_cast<float*>(workspace);
-    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     const Heads all[6] = {a.q, a.k, a.oq, a.ok, a.xq, a.xk};
     const int vec = chunk_of(plan, dim, e, all, 6);
     a.d = deal_of(plan, dim, vec);
@@ -1135,10 +1141,7 @@ int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* d
                : vec == 2 ? backward_t<T, 2, 2, 0>(a, blocks, s)
                           : backward_t<T, 1, 4, 0>(a, blocks, s);
     });
-    if (rc) return rc;
-    gains_kernel<<<(2 * (unsigned)dim * 32 + kThreads - 1) / kThreads, kThreads, 0, s>>>(
-        a.partial, a.q_blocks, blocks, (uint32_t)dim, dgain_q, dgain_k, dgain_type, accumulate != 0);
-    return cudaGetLastError() == cudaSuccess ? ARK_OK : ARK_E_CUDA;
+    return rc ? rc : sum_gains(blocks);
 }
 
 }  // extern "C"

@@ -18,3 +18,20 @@ def test_positions_of_no_tokens(itype):
     assert y[0].shape == q.shape and y[2].rows == 0
     back = ab.qk_norm_rope_backward(q, q[:, :2], y[2], y[3], g, g, plan, pos)
     assert (back[2] == 0).all() and (back[3] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hk", [(0, 2), (3, 0), (0, 0)])
+def test_gains_of_no_heads_have_no_gradient(hq, hk):
+    """A sum over no heads is zero, and stays what was there when it is added to."""
+    plan, tokens, dim = ab.RopePlan(32), 5, 32
+    q, k = (torch.randn(tokens, h, dim, device="cuda").half() for h in (hq, hk))
+    g = torch.ones(dim, device="cuda")
+    junk = [torch.full((dim,), 7.0, device="cuda") for _ in range(2)]
+    kept = [t.clone() for t in junk]
+    out = ab.qk_norm_rope_backward(q, k, q, k, g, g, plan, out_gains=tuple(junk))
+    ab.qk_norm_rope_backward(q, k, q, k, g, g, plan, out_gains=tuple(kept), accumulate=True)
+    for h, got, more in ((hq, out[2], kept[0]), (hk, out[3], kept[1])):
+        if h:
+            assert torch.equal(more, got + 7) and got.any()
+        else:
+            assert (got == 0).all() and (more == 7).all()
