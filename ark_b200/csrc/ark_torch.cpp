@@ -175,14 +175,16 @@ private:
 };
 
 // ------------------------------------------------------------ checkpoints
-Act8 act8_pack(const Tensor& x, const std::string& kind, Act8* out) {
+Act8 act8_pack(const Tensor& x, const std::optional<std::string>& kind, Act8* out) {
     const uint64_t ld = rows_of(x, "x");
+    const int code = kind ? kind_code(*kind) : out ? out->kind() : ARK_ACT8_E4M3;
+    if (out && code != out->kind()) bad_value("out: expected a checkpoint of " + *kind + ", got " + out->kind_name());
     const On on(x.device());
     if (out) {
         out->need("out", x.size(0), x.size(1));
         need_device(x.device(), out->device());
     }
-    const Act8 c = out ? *out : Act8(x.size(0), x.size(1), kind_code(kind), x.device(), x.scalar_type());
+    const Act8 c = out ? *out : Act8(x.size(0), x.size(1), code, x.device(), x.scalar_type());
     check("ark_cuda_act8_pack",
           ark_cuda_act8_pack(x.data_ptr(), type_code(x.scalar_type()), ld, c.c(), on.stream));
     if (!out) return c;
@@ -590,8 +592,8 @@ Host memory only: made once, usable on every device and in graphs.)")
         .def_property_readonly("gain", [](const RopePlan& p) { return p.c.gain; })
         .def("frequencies", &RopePlan::frequencies, "Radians per position of each pair.");
 
-    m.def("act8_pack", &act8_pack, arg("x"), arg("kind") = "e4m3", arg("out") = none,
-          "Checkpoint x [rows, cols] (FP16, BF16 or FP32) in 8 bits.");
+    m.def("act8_pack", &act8_pack, arg("x"), arg("kind") = none, arg("out") = none,
+          "Checkpoint x [rows, cols] (FP16, BF16 or FP32) in 8 bits.  kind: that of out, or \"e4m3\".");
     m.def("act8_unpack", &act8_unpack, arg("checkpoint"), arg("dtype") = at::kHalf, arg("out") = none,
           "The activation that a checkpoint stands for; a finite value that the type cannot\n"
           "hold saturates at its largest.");

@@ -35,3 +35,14 @@ def test_gains_of_no_heads_have_no_gradient(hq, hk):
             assert torch.equal(more, got + 7) and got.any()
         else:
             assert (got == 0).all() and (more == 7).all()
+
+
+def test_pack_is_of_the_kind_that_was_asked_for():
+    x = torch.randn(4, 64, device="cuda").half()
+    room = ab.Act8.empty(4, 64, "int8")
+    assert ab.act8_pack(x).kind == "e4m3" and ab.act8_pack(x, "int8").kind == "int8"
+    assert ab.act8_pack(x, out=room).kind == "int8" and ab.act8_pack(x, "int8", room).kind == "int8"
+    with pytest.raises(ValueError, match="int8"):
+        ab.act8_pack(x, "e4m3", out=room)
+    with pytest.raises(ValueError, match="kind"):
+        ab.act8_pack(x, "int4", out=room)
