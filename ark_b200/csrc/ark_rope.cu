@@ -274,9 +274,10 @@ struct Turn {
             s[i] = __fmul_rn(a.inverse ? -s[i] : s[i], a.plan.gain);
         }
     }
-    // rotate a unit's pairs in place
+    // Rotate a unit's pairs in place.  A layout's products are rounded in one order, whatever
+    // the width of a chunk: results do not depend on how rows are aligned.
     __device__ __forceinline__ void operator()(const Deal& d, uint64_t* v) const {
-        if (VEC == 1 || d.interleaved) {   // both of a rotated pair in one register pair
+        if (d.interleaved) {   // both of a rotated pair in one register pair
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 float x, y;
@@ -284,6 +285,10 @@ struct Turn {
                 v[i] = pair(__fmaf_rn(x, c[i], -__fmul_rn(y, s[i])),
                             __fmaf_rn(y, c[i], __fmul_rn(x, s[i])));
             }
+        } else if constexpr (VEC == 1) {
+            float x, y;
+            unpair(v[0], x, y);
+            v[0] = pair(__fmaf_rn(y, -s[0], __fmul_rn(x, c[0])), __fmaf_rn(y, c[0], __fmul_rn(x, s[0])));
         } else {
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) {

@@ -46,3 +46,19 @@ def test_pack_is_of_the_kind_that_was_asked_for():
         ab.act8_pack(x, "e4m3", out=room)
     with pytest.raises(ValueError, match="kind"):
         ab.act8_pack(x, "int4", out=room)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [F32, F16, torch.bfloat16])
+def test_rotation_does_not_depend_on_the_rows_alignment(layout, dtype):
+    """Chunks of 1, 2, 4 and 8 elements: the same products, rounded in the same order."""
+    plan, g = ab.RopePlan(48, layout=layout), torch.Generator().manual_seed(9)
+    x = torch.randn(300, 6, 48, generator=g).to(dtype).cuda()
+    pos = torch.randint(0, 100000, (300,), generator=g).cuda()
+    for inverse in (False, True):
+        want = ab.rope(x, None, plan, pos, inverse=inverse)[0]
+        for off in (1, 2, 4):
+            odd = torch.empty(300, 6 * 48 + off, dtype=dtype, device="cuda")[:, off:].view(300, 6, 48).copy_(x)
+            assert odd.data_ptr() % (16 if dtype == F32 else 8) or off == 4
+            assert torch.equal(ab.rope(odd, None, plan, pos, inverse=inverse)[0], want)
+            assert torch.equal(ab.rope(odd, None, plan, pos, inverse=inverse, out=(odd, None))[0], want)
