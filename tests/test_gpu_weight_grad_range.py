@@ -101,3 +101,36 @@ def test_who_is_wide():
         assert [c.wide for c in (a, b, cy, cq, ck)] == [wide] * 5
     ab.act8_pack(x.half(), out=room)
     assert not room.wide and ab.Act8(room.data, room.scale, 64, "e4m3", wide=True).wide
+
+
+def test_captured_replayed_and_on_two_streams():
+    sets = [[t.cuda() for t in inputs(500, 300, 200, s)] for s in (11, 12)]
+    want = [x.double().T @ dy.double() for x, dy in sets]
+
+    def call(x, dy):
+        return ab.weight_grad(ab.act8_pack(x, "int8"), dy, dtype=F32)
+
+    x, dy = (t.clone() for t in sets[0])
+    call(x, dy)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(x, dy)
+        graphs.append((graph, out))
+    for (a, b), w in ((sets[1], want[1]), (sets[0], want[0])):
+        x.copy_(a), dy.copy_(b)
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out.double(), w) for _, out in graphs)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(4):
+        got = []
+        for st, s in zip(streams, sets):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(call(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g.double(), w) for g, w in zip(got, want))
