@@ -241,14 +241,16 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) {
 }
 
 // Scale bytes between which q * 2^k needs neither saturation nor a scale
-// outside of T; every block of ordinary activations lies between them.  The
-// others (and NaN blocks) go through FP32.
+// outside of T; every block of ordinary activations lies between them.  Up to
+// kNone, as in a block of zeros (scale byte 1), every value rounds to zero, and so
+// do scale and products: no branch of its own for a row's padding.  The others (and
+// NaN blocks) go through FP32.
 template <class T, int KIND>
 struct Fast;
 template <>
 struct Fast<__half, kE4M3> {
     // 2^-24 is the smallest FP16; 448 * 2^7 is below 65504
-    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 7;
+    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 7, kNone = 127 - 37;
     __half2 s;
     __device__ __forceinline__ explicit Fast(uint32_t byte) {
         s = __float2half2_rn(__uint_as_float(byte << 23));
@@ -262,7 +264,7 @@ struct Fast<__half, kE4M3> {
 };
 template <>
 struct Fast<__half, kInt8> {
-    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 5;
+    static constexpr uint32_t kLo = 127 - 24, kHi = 127 + 5, kNone = 127 - 37;
     __half2 s, t;   // 2^k and -1152 * 2^k
     __device__ __forceinline__ explicit Fast(uint32_t byte) {
         const float f = __uint_as_float(byte << 23);
@@ -281,7 +283,7 @@ template <>
 struct Fast<__nv_bfloat16, kE4M3> {
     // exponent and mantissa of e4m3 moved to BF16's, whose bias is 120 larger:
     // the value times 2^-120, subnormals included
-    static constexpr uint32_t kLo = 1, kHi = 127 + 7;
+    static constexpr uint32_t kLo = 1, kHi = 127 + 7, kNone = 0;
     __nv_bfloat162 s;
     __device__ __forceinline__ explicit Fast(uint32_t byte) {
         s = __float2bfloat162_rn(__uint_as_float((byte + 120u) << 23));
@@ -295,7 +297,7 @@ struct Fast<__nv_bfloat16, kE4M3> {
 };
 template <>
 struct Fast<__nv_bfloat16, kInt8> {
-    static constexpr uint32_t kLo = 1, kHi = 127 + 120;
+    static constexpr uint32_t kLo = 1, kHi = 127 + 120, kNone = 0;
     __nv_bfloat162 s;
     __device__ __forceinline__ explicit Fast(uint32_t byte) {
         s = __float2bfloat162_rn(__uint_as_float(byte << 23));
@@ -330,8 +332,9 @@ __device__ __forceinline__ uint32_t operand_pair(float a, float b, __nv_bfloat16
 // puts none on.  Values of a checkpoint of a wider type are rounded once.
 template <class T, int KIND, bool OPERAND>
 __device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uint4& hi) {
-    if (byte >= Fast<T, KIND>::kLo && byte <= Fast<T, KIND>::kHi) {
-        const Fast<T, KIND> f(byte);
+    using F = Fast<T, KIND>;
+    if (byte <= F::kHi && (byte >= F::kLo || byte <= F::kNone)) {
+        const F f(byte);
         lo = make_uint4(f.pair(w.x, 0), f.pair(w.x, 2), f.pair(w.y, 0), f.pair(w.y, 2));
         hi = make_uint4(f.pair(w.z, 0), f.pair(w.z, 2), f.pair(w.w, 0), f.pair(w.w, 2));
     } else {

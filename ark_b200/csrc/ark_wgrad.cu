@@ -49,9 +49,9 @@ constexpr int kAhead = 2;                     // steps of a team in flight
 // rounded: each addition may lose a unit of the last place, 2^-23 of the sum, and
 // always towards zero.  So one accumulator takes a bounded run of 64-token steps, and
 // runs are added by FP32 additions that round.  FP32 gradients: 32 steps, 128
-// additions.  16-bit ones: 128 steps, whose 512 additions lose at most 2^-14, an
-// eighth of FP16's half step.
-constexpr uint32_t kRun32 = 32, kRun16 = 128;
+// additions.  16-bit ones: as many as lose an eighth of the type's half step, 2^-14 for
+// FP16 (512 additions) and 2^-11 for BF16 (4096).
+constexpr uint32_t kRun32 = 32, kRunF16 = 128, kRunBF16 = 1024;
 constexpr uint32_t kFewRuns = 4;              // accumulators of few_kernel
 constexpr uint32_t kSleepNs = 1000000;
 constexpr long long kWaitClocks = 4000000000ll;   // 2 s
@@ -359,16 +359,18 @@ template <int AHEAD, class O>
 __device__ __forceinline__ void out_block(O* p, const Out& o, uint32_t m, uint32_t n, uint32_t row0,
                                           uint32_t col0, const float4* staged, uint32_t lane,
                                           bool accumulate) {
+    using Raw4 = typename std::conditional<sizeof(O) == 4, uint4, uint2>::type;   // four elements
     if (o.vec && col0 + 16 <= n) {
         const uint32_t r0 = lane / 4;
         p += (uint64_t)(row0 + r0) * o.ld + col0 + (lane & 3) * 4;
 #pragma unroll 1
         for (int h = 0; h < 4; h += AHEAD) {
-            float old[AHEAD][4];
+            Raw4 old[AHEAD];   // as they lie there: widening one would wait for it
             if (accumulate) {
 #pragma unroll
                 for (int i = 0; i < AHEAD; ++i)
-                    if (row0 + r0 + (h + i) * 8 < m) load_vec<4>(p + (uint64_t)(i * 8) * o.ld, old[i]);
+                    if (row0 + r0 + (h + i) * 8 < m)
+                        old[i] = *reinterpret_cast<const Raw4*>(p + (uint64_t)(i * 8) * o.ld);
             }
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
@@ -376,8 +378,10 @@ __device__ __forceinline__ void out_block(O* p, const Out& o, uint32_t m, uint32
                 const float4 f = staged[r * 4 + ((lane & 3) ^ (r >> 1 & 3))];
                 float v[4] = {f.x, f.y, f.z, f.w};
                 if (accumulate) {
+                    float w[4];
+                    load_vec<4>(reinterpret_cast<const O*>(&old[i]), w);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], old[i][j]);
+                    for (int j = 0; j < 4; ++j) v[j] = __fadd_rn(v[j], w[j]);
                 }
                 if (row0 + r < m) store_vec<4>(p + (uint64_t)(i * 8) * o.ld, v);
             }
@@ -390,17 +394,19 @@ __device__ __forceinline__ void out_block(O* p, const Out& o, uint32_t m, uint32
     if (col0 + e >= n) return;
     p += (uint64_t)(row0 + r0) * o.ld + col0 + e;
 #pragma unroll 1
-    for (uint32_t h = 0; h < 32; h += 2 * AHEAD, p += 2 * AHEAD * o.ld) {
-        float old[AHEAD];
+    for (uint32_t h = 0; h < 32; h += 8, p += 8 * o.ld) {
+        O old[4];
+        if (accumulate) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            old[i] = accumulate && row0 + r0 + h + 2 * i < m ? Elem<O>::to_f(p[(uint64_t)(2 * i) * o.ld]) : 0.0f;
+            for (int i = 0; i < 4; ++i)
+                if (row0 + r0 + h + 2 * i < m) old[i] = p[(uint64_t)(2 * i) * o.ld];
+        }
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const uint32_t r = r0 + h + 2 * i;
-            const float v = one[(r * 4 + (e / 4 ^ (r >> 1 & 3))) * 4 + e % 4];
-            if (row0 + r < m)
-                p[(uint64_t)(2 * i) * o.ld] = Elem<O>::from_f(accumulate ? __fadd_rn(v, old[i]) : v);
+            float v = one[(r * 4 + (e / 4 ^ (r >> 1 & 3))) * 4 + e % 4];
+            if (accumulate) v = __fadd_rn(v, Elem<O>::to_f(old[i]));
+            if (row0 + r < m) p[(uint64_t)(2 * i) * o.ld] = Elem<O>::from_f(v);
         }
     }
 }
@@ -791,35 +797,32 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t quarter = warp % 4, c0 = warp / 4 * kCols;
         float4* staged = reinterpret_cast<float4*>(raw + (stages - smem_u32(raw)) + kStages * S::kStage) +
                          warp * 128;
-        Ring<2> acc;   // a wait that ran out makes every tile from there on NaN
-        auto wait = [&] {
-            return acc.wait([&] { return __any_sync(0xFFFFFFFFu, *gave_up); },
-                            [&](uint32_t b, uint32_t parity) {
-                                return warp_wait<kSleep>(smem_u32(acc_full + b), parity, gave_up);
-                            });
+        Ring<2> acc;
+        auto wait = [&] { return warp_wait<kSleep>(smem_u32(acc_full + acc.at), acc.parity, gave_up); };
+        // where an item's sums go: its run of tokens, or the output
+        auto where = [&](uint32_t run) {
+            return a.partial ? Out{a.partial + (uint64_t)run * a.m * a.n_pad, a.n_pad, 1, 0, 1} : a.out;
         };
-        for (uint32_t i = blockIdx.x / 2; i < items; i += pairs) {
+        const bool accumulate = a.accumulate && !a.partial;
+        auto tile = [&](uint32_t i) {
             uint32_t m, n, it0, it1;
             const uint32_t run = item(i, m, n, it0, it1);
             const uint32_t row0 = m * (2 * kBM) + rank * kBM + quarter * 32;
-            Out out = a.out;
-            bool accumulate = a.accumulate;
-            if (a.partial) {
-                out = Out{a.partial + (uint64_t)run * a.m * a.n_pad, a.n_pad, 1, 0, 1};
-                accumulate = false;
-            }
+            const Out out = where(run);
             // a lane's 16 columns of one row, among the warp's 32 rows
             auto stage = [&](const float* v, bool ok) {
                 const float none = __uint_as_float(0x7FC00000u);
+                __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     staged[lane * 4 + (j ^ (lane >> 1 & 3))] =
                         ok ? make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3])
                            : make_float4(none, none, none, none);
+                __syncwarp();
             };
             // what is staged, as the columns from c on
             auto put = [&](uint32_t c) {
-                constexpr int kAhead = RUNS == kOneRun ? 4 : 2;
+                constexpr int kAhead = 2;
                 const uint32_t col0 = n * S::kBN + c;
                 if (RUNS == kRunsTo32 || (RUNS == kOneRun && out.f32))
                     out_block<kAhead>(static_cast<float*>(out.p), out, a.m, a.n, row0, col0, staged, lane,
@@ -838,26 +841,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 acc.next();
             };
             if constexpr (RUNS == kOneRun) {
-                const bool ok = wait();
+                if (!wait()) return false;
                 fence_after();
 #pragma unroll 1
                 for (uint32_t c = c0; c < c0 + kCols; c += 16) {
                     float v[16];
                     tmem_ld16(tmem + acc.at * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
-                    __syncwarp();
-                    stage(v, ok);
-                    __syncwarp();
+                    stage(v, true);
                     put(c);
                 }
                 next();
+                return true;
             } else {
                 // the runs' sums are added in registers
                 float sum[kCols / 16][16] = {};
-                bool ok;   // the last wait's: it is false after a lost one
 #pragma unroll 1
                 for (uint32_t k = 0; k < a.chunks; ++k) {
-                    ok = wait();
+                    if (!wait()) return false;
                     fence_after();
 #pragma unroll
                     for (int c = 0; c < kCols / 16; ++c) {
@@ -872,15 +873,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 // unrolled, four copies of the output's code spilled the sums
 #pragma unroll 1
                 for (int k = 0; k < kCols / 16; ++k) {
-                    __syncwarp();
 #pragma unroll
                     for (int c = 0; c < kCols / 16; ++c)
-                        if (c == k) stage(sum[c], ok);
-                    __syncwarp();
+                        if (c == k) stage(sum[c], true);
                     put(c0 + k * 16);
                 }
+                return true;
             }
-        }
+        };
+        // NaN for the warp's part of a tile
+        auto lost = [&](uint32_t i) {
+            uint32_t m, n, it0, it1;
+            const uint32_t run = item(i, m, n, it0, it1);
+            const Out out = where(run);
+            const uint32_t row = m * (2 * kBM) + rank * kBM + quarter * 32 + lane, col = n * S::kBN + c0;
+            for (uint32_t c = col; row < a.m && c < min(col + kCols, a.n); ++c)
+                out_put(out, (uint64_t)row * out.ld + c, __uint_as_float(0x7FC00000u));
+        };
+        until_lost(blockIdx.x / 2, items, pairs, tile, lost);
     }
     __syncwarp();
     fence_before();
@@ -1138,7 +1148,8 @@ int product(const Way& w, const ark_act8* x, const void* dy, int32_t dy_type, ui
         a.splits = w.splits;
         a.partial = w.partial_bytes ? reinterpret_cast<float*>(ws + w.x_bytes) : nullptr;
         a.n_pad = (a.n + 3) / 4 * 4;
-        const uint32_t run = (a.iters + a.splits - 1) / a.splits, most = a.out.f32 ? kRun32 : kRun16;
+        const uint32_t run = (a.iters + a.splits - 1) / a.splits;
+        const uint32_t most = a.out.f32 ? kRun32 : a.out.bf16 ? kRunBF16 : kRunF16;
         a.chunks = (run + most - 1) / most;
         failed = act8_operands(x, ws, dy_type, a.pitch, s);
         if (failed) return failed;

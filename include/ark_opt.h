@@ -435,10 +435,10 @@ ARK_API int ark_cuda_act8_unpack(const ark_act8* in, void* y, int32_t type, uint
  * layout, objc/bridge.m:229-411) from the checkpoint of x [tokens, in]:
  *   dw[i, o] = (accumulate ? dw[i, o] : 0) + sum over t of x[t, i] dy[t, o],
  * products and sums in FP32, rounded once to dw's type.  The matrix units cut
- * their FP32 sums off where others round; runs of at most 2048 tokens (8192
- * where dw is of 16 bits) are summed by them and added with rounding, so that
- * this loses at most 2^-16 (2^-14) of the sum of magnitudes, however many
- * tokens there are.  dy: F16 or BF16
+ * their FP32 sums off where others round; runs of at most 2048 tokens (dw
+ * F32; F16: 8192, BF16: 65536) are summed by them and added with rounding, so
+ * that this loses at most 2^-16 (2^-14, 2^-11) of the sum of magnitudes,
+ * however many tokens there are.  dy: F16 or BF16
  * [tokens, n_out]; dw: F16, BF16 or F32 [x->cols, n_out], for example a
  * tensor's range of ark_cuda_opt_grad_buffer with dy carrying the loss
  * scale; a sum that F16 cannot hold becomes an infinity, which the step

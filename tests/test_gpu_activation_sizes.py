@@ -50,7 +50,8 @@ def whole(tokens, nin, nout, dtype, seed):
     ("pairs, one run where FP32 has three", 4200, 2048, 5504, True, False),
     ("pairs, rows of any boundary", 4096, 2048, 5501, True, False),
     ("pairs, dY realigned, an odd height", 2100, 2049, 5503, True, False),
-    ("pairs, 16-bit runs", 8200, 2048, 2301, True, False),
+    ("pairs, runs of FP16", 8200, 2048, 2301, True, False),
+    ("pairs, runs of BF16", 66000, 2048, 2301, True, False),
     ("split tokens", 8192, 768, 2048, True, True),
     ("split tokens, columns not in fours", 8192, 770, 2046, True, True),
     ("split tokens, runs in each", 130000, 500, 510, True, True),

@@ -24,8 +24,8 @@ def sums(x, dy):
 
 
 # an addition of 16 tokens loses at most 2^-23 of the sum of magnitudes: 128 of them in an FP32
-# gradient, 512 in a 16-bit one; the FP32 additions of the runs 2^-24 each
-LOSS = {F32: 128 * 2.0 ** -23, F16: 512 * 2.0 ** -23, BF16: 512 * 2.0 ** -23}
+# gradient, 512 in an FP16 and 4096 in a BF16 one; the FP32 additions of the runs 2^-24 each
+LOSS = {F32: 128 * 2.0 ** -23, F16: 512 * 2.0 ** -23, BF16: 4096 * 2.0 ** -23}
 
 
 @pytest.mark.parametrize("tokens,nin,nout,dtype,out", [
@@ -34,6 +34,7 @@ LOSS = {F32: 128 * 2.0 ** -23, F16: 512 * 2.0 ** -23, BF16: 512 * 2.0 ** -23}
     (128000, 4096, 256, BF16, F32),      # 16 tiles
     (128000, 4096, 256, BF16, BF16),
     (40001, 2048, 2301, BF16, BF16),     # odd
+    (140000, 2048, 2304, BF16, BF16),
     (300000, 256, 256, F16, F32),        # one tile
 ])
 def test_long_sums_keep_their_size(tokens, nin, nout, dtype, out):

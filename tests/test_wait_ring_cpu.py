@@ -25,17 +25,15 @@ int main(int, char** argv) {
     Barrier b[2];
     b[0].last = atoi(argv[2]), b[1].last = atoi(argv[3]);
     ark::Ring<2> r;
-    bool lost = false;
-    for (unsigned i = 0; i < items; ++i) {
-        const bool ok = r.wait([&] { return lost; }, [&](unsigned at, unsigned parity) {
-            // the writer completes the next phase as soon as the reader waits, until it stops
-            if (!b[at].passed(parity) && b[at].done < b[at].last) ++b[at].done;
-            lost = !b[at].passed(parity);
-            return !lost;
-        });
-        putchar(ok ? '1' : '0');
+    ark::until_lost(0, items, 1, [&](unsigned) {
+        // the writer completes the next phase as soon as the reader waits, until it stops
+        Barrier& x = b[r.at];
+        if (!x.passed(r.parity) && x.done < x.last) ++x.done;
+        if (!x.passed(r.parity)) return false;
+        putchar('1');
         r.next();
-    }
+        return true;
+    }, [&](unsigned) { putchar('0'); });
     return 0;
 }
 """
