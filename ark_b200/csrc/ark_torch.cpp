@@ -592,8 +592,11 @@ Host memory only: made once, usable on every device and in graphs.)")
         .def_property_readonly("gain", [](const RopePlan& p) { return p.c.gain; })
         .def("frequencies", &RopePlan::frequencies, "Radians per position of each pair.");
 
+    m.doc() = "The activation operators.  None of them makes an autograd node: what they return\n"
+              "requires no gradient, whatever their inputs do.";
     m.def("act8_pack", &act8_pack, arg("x"), arg("kind") = none, arg("out") = none,
-          "Checkpoint x [rows, cols] (FP16, BF16 or FP32) in 8 bits.  kind: that of out, or \"e4m3\".");
+          "Checkpoint x [rows, cols] (FP16, BF16 or FP32) in 8 bits.  kind: that of out, or \"e4m3\".\n"
+          "No autograd node is made.");
     m.def("act8_unpack", &act8_unpack, arg("checkpoint"), arg("dtype") = at::kHalf, arg("out") = none,
           "The activation that a checkpoint stands for; a finite value that the type cannot\n"
           "hold saturates at its largest.");
@@ -610,7 +613,9 @@ out: where to write (FP16, BF16 or FP32; for example a range of the gradient
 accumulate: add to what is in `out`.)");
     m.def("swiglu", &swiglu, arg("a"), arg("b"), arg("checkpoint") = none, arg("out") = none,
           R"(y = silu(a) * b for a, b [rows, cols].  With checkpoint ("e4m3" or "int8")
-returns (y, Act8 of a, Act8 of b), made in the same pass.  out may be a or b.)");
+returns (y, Act8 of a, Act8 of b), made in the same pass.  out may be a or b.
+
+No autograd node is made: the backward is swiglu_backward, by the caller.)");
     m.def("swiglu_backward", &swiglu_backward, arg("dy"), arg("ca"), arg("cb"), arg("checkpoint") = none,
           arg("out") = none, R"((da, db) of swiglu from the checkpoints of a and b.  With checkpoint, returns
 (da, db, Act8 of the remade product) for the weight gradient of the projection
@@ -623,13 +628,17 @@ positions: int32 / int64 [tokens], any non-negative value; a negative one marks 
            seq_len (default: one sequence).
 inverse:   the opposite rotation, which is the backward.
 out:       (q, k) to write to, for example q and k themselves.
-Any strides with contiguous heads' elements.  Returns (q, k).)");
+Any strides with contiguous heads' elements.  Returns (q, k).
+
+No autograd node is made: the backward is the inverse rotation, by the caller.)");
     m.def("qk_norm_rope", &qk_norm_rope, arg("q"), arg("k"), arg("gain_q"), arg("gain_k"), arg("plan"),
           arg("positions") = none, arg("seq_len") = none, arg("eps") = 1e-6, arg("checkpoint") = none,
           arg("out") = none, R"(RMS norm of each head of q and k (k may be None) with its gain [dim], then the
 rotation, in one pass.  With checkpoint ("e4m3" or "int8") q and k as they come
 in are checkpointed too: returns (q, k, Act8 of q, Act8 of k), each of
-[tokens, heads * dim], else (q, k).)");
+[tokens, heads * dim], else (q, k).
+
+No autograd node is made: the backward is qk_norm_rope_backward, by the caller.)");
     m.def("qk_norm_rope_backward", &qk_norm_rope_backward, arg("dq"), arg("dk"), arg("q"), arg("k"),
           arg("gain_q"), arg("gain_k"), arg("plan"), arg("positions") = none, arg("seq_len") = none,
           arg("eps") = 1e-6, arg("out") = none, arg("out_gains") = none, arg("accumulate") = false,

@@ -24,8 +24,8 @@
 // a cluster of up to 8 CTAs whose FP32 partial tiles are added over distributed
 // shared memory in rank order: no workspace, the same bits every time.
 //
-// Every wait is bounded.  One that runs out makes its CTA leave with NaN as
-// its tile, which the step's finite check turns into a skipped step.
+// Every wait is bounded.  One that runs out makes its CTA leave NaN in its tiles
+// from there on, which the step's finite check turns into a skipped step.
 #include <cuda.h>
 
 #include <atomic>
@@ -810,14 +810,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t row0 = m * (2 * kBM) + rank * kBM + quarter * 32;
             const Out out = where(run);
             // a lane's 16 columns of one row, among the warp's 32 rows
-            auto stage = [&](const float* v, bool ok) {
-                const float none = __uint_as_float(0x7FC00000u);
+            auto stage = [&](const float* v) {
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     staged[lane * 4 + (j ^ (lane >> 1 & 3))] =
-                        ok ? make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3])
-                           : make_float4(none, none, none, none);
+                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 __syncwarp();
             };
             // what is staged, as the columns from c on
@@ -848,7 +846,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     float v[16];
                     tmem_ld16(tmem + acc.at * S::kBN + (quarter * 32 << 16) + c,
                               reinterpret_cast<uint32_t*>(v));
-                    stage(v, true);
+                    stage(v);
                     put(c);
                 }
                 next();
@@ -875,7 +873,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 for (int k = 0; k < kCols / 16; ++k) {
 #pragma unroll
                     for (int c = 0; c < kCols / 16; ++c)
-                        if (c == k) stage(sum[c], true);
+                        if (c == k) stage(sum[c]);
                     put(c0 + k * 16);
                 }
                 return true;

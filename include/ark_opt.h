@@ -530,7 +530,10 @@ ARK_API int ark_cuda_rope(const ark_rope_plan* plan, const ark_heads* q, const a
  * rotation, in one pass; nothing is rounded between.  With q8 (and k8), q and
  * k as they come in are checkpointed too, as [tokens, heads * dim] (padding
  * tokens' rows are unspecified); where dim or the rotated part is not made of
- * whole scale blocks that needs head_stride == dim (else ARK_E_UNSUPPORTED). */
+ * whole scale blocks that needs head_stride == dim (else ARK_E_UNSUPPORTED).
+ * The same tensors give the same bits on every call; the sum of squares is
+ * taken in chunks as wide as the rows' alignment allows, so rows on another
+ * boundary may differ in the last place (the rotation alone does not). */
 ARK_API int ark_cuda_qk_norm_rope(const ark_rope_plan* plan, const ark_heads* q,
                                   const ark_heads* k, const ark_heads* out_q,
                                   const ark_heads* out_k, int32_t type, uint64_t tokens,
