@@ -408,7 +408,8 @@ __device__ __forceinline__ bool splits(float y, float most) {
 // next to one of the 8-bit grid, where the last bit of FP32 would decide by a whole
 // step: values within FP32's error of a border of T, about one in 500, are made
 // again in 64 bits and rounded to FP32.  Rounding both ends of the error finds the
-// borders of every size, those of FP16's subnormals too.
+// borders of every size, those of FP16's subnormals too.  An FP32 product is packed as
+// FP32 made it: next to a border of the 8-bit grid it may go either way.
 // Blocks an SM: what 80 and 64 registers allow, without spills.
 template <class T, int KIND, bool REMAKE>
 __global__ void __launch_bounds__(kThreads, REMAKE ? 3 : 4) swiglu_back_kernel(

@@ -470,7 +470,8 @@ ARK_API int ark_cuda_swiglu(const void* a, uint64_t lda, const void* b, uint64_t
 /* Its backward from the checkpoints: da = dy b silu'(a), db = dy silu(a).
  * With y8, silu(a) * b is remade from the checkpoints, rounded to `type` and
  * checkpointed, for the weight gradient of the projection that reads it: the
- * forward then keeps no y.  da or db may be dy. */
+ * forward then keeps no y.  da or db may be dy.  An element that 8 bits
+ * rounded up to 2^128 (BF16 and F32 above 3.2e38) is an infinity here. */
 ARK_API int ark_cuda_swiglu_backward(const void* dy, uint64_t lddy, int32_t type,
                                      const ark_act8* a8, const ark_act8* b8, void* da,
                                      uint64_t ldda, void* db, uint64_t lddb, const ark_act8* y8,
