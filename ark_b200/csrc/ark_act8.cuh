@@ -241,10 +241,9 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) {
 }
 
 // Scale bytes between which q * 2^k needs neither saturation nor a scale
-// outside of T; every block of ordinary activations lies between them.  Up to
-// kNone, as in a block of zeros (scale byte 1), every value rounds to zero, and so
-// do scale and products: no branch of its own for a row's padding.  The others (and
-// NaN blocks) go through FP32.
+// outside of T; every block of ordinary activations lies between them.  The
+// others (and NaN blocks) go through FP32, but for operands up to kNone, where every
+// value rounds to zero: a row's padding makes such blocks (scale byte 1).
 template <class T, int KIND>
 struct Fast;
 template <>
@@ -333,10 +332,12 @@ __device__ __forceinline__ uint32_t operand_pair(float a, float b, __nv_bfloat16
 template <class T, int KIND, bool OPERAND>
 __device__ __forceinline__ void operand16(uint4 w, uint32_t byte, uint4& lo, uint4& hi) {
     using F = Fast<T, KIND>;
-    if (byte <= F::kHi && (byte >= F::kLo || byte <= F::kNone)) {
+    if (byte >= F::kLo && byte <= F::kHi) {
         const F f(byte);
         lo = make_uint4(f.pair(w.x, 0), f.pair(w.x, 2), f.pair(w.y, 0), f.pair(w.y, 2));
         hi = make_uint4(f.pair(w.z, 0), f.pair(w.z, 2), f.pair(w.w, 0), f.pair(w.w, 2));
+    } else if (OPERAND && byte <= F::kNone) {
+        lo = hi = make_uint4(0u, 0u, 0u, 0u);
     } else {
         auto two = [](float x, float y) {
             return OPERAND ? operand_pair(x, y, T()) : pair_of(x, y, T());
