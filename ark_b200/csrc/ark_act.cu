@@ -646,7 +646,7 @@ int ark_cuda_swiglu_backward(const void* dy, uint64_t lddy, int32_t type, const 
         (rows > 1 && (ldda < cols || lddb < cols)))
         return ARK_E_INVALID_ARG;
     if (rows == 0 || cols == 0) return ARK_OK;
-    if (!dy || !da || !db) return ARK_E_INVALID_ARG;
+    if (!dy || !da || !db || da == db) return ARK_E_INVALID_ARG;
     const uint64_t e = type_size(type);
     if (!aligned_to(dy, e) || !aligned_to(da, e) || !aligned_to(db, e)) return ARK_E_MISALIGNED;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);

@@ -834,6 +834,10 @@ int plan_ok(const ark_rope_plan* p, uint64_t dim) {
 }
 
 int common_ok(const Args& a, uint64_t e, uint64_t dim, int pos_type) {
+    // an output is its own input's memory or nobody's: q's is read and written apart from k's
+    if (a.tokens && a.q.heads && a.k.heads &&
+        (a.oq.p == a.ok.p || a.oq.p == a.k.p || a.ok.p == a.q.p))
+        return ARK_E_INVALID_ARG;
     if (!a.pos && a.seq == 0) return ARK_E_INVALID_ARG;
     if (a.pos && pos_type != ARK_TYPE_I32 && pos_type != ARK_TYPE_I64) return ARK_E_INVALID_ARG;
     if (a.pos && !aligned_to(a.pos, a.pos64 ? 8 : 4)) return ARK_E_MISALIGNED;
@@ -1120,6 +1124,7 @@ int ark_cuda_qk_norm_rope_backward(const ark_rope_plan* plan, const ark_heads* d
     }
     if ((a.q.heads && (!gain_q || !dgain_q)) || (a.k.heads && (!gain_k || !dgain_k)))
         return ARK_E_INVALID_ARG;
+    if (dk && dgain_q && dgain_q == dgain_k) return ARK_E_INVALID_ARG;
     if (!aligned_to(gain_q, type_size(gain_type)) || !aligned_to(gain_k, type_size(gain_type)) ||
         !aligned_to(dgain_q, type_size(dgain_type)) || !aligned_to(dgain_k, type_size(dgain_type)))
         return ARK_E_MISALIGNED;

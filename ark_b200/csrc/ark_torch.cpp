@@ -619,7 +619,7 @@ No autograd node is made: the backward is swiglu_backward, by the caller.)");
     m.def("swiglu_backward", &swiglu_backward, arg("dy"), arg("ca"), arg("cb"), arg("checkpoint") = none,
           arg("out") = none, R"((da, db) of swiglu from the checkpoints of a and b.  With checkpoint, returns
 (da, db, Act8 of the remade product) for the weight gradient of the projection
-that reads it; its kind is that of ca.  out: (da, db), either of which may be dy.)");
+that reads it; its kind is that of ca.  out: (da, db), one of which may be dy.)");
     m.def("rope", &rope, arg("q"), arg("k"), arg("plan"), arg("positions") = none, arg("seq_len") = none,
           arg("inverse") = false, arg("out") = none, R"(Rotate q [tokens, heads, dim] and k [tokens, kv heads, dim] (or None).
 

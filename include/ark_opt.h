@@ -470,7 +470,7 @@ ARK_API int ark_cuda_swiglu(const void* a, uint64_t lda, const void* b, uint64_t
 /* Its backward from the checkpoints: da = dy b silu'(a), db = dy silu(a).
  * With y8, silu(a) * b is remade from the checkpoints, rounded to `type` and
  * checkpointed, for the weight gradient of the projection that reads it: the
- * forward then keeps no y.  da or db may be dy.  An element that 8 bits
+ * forward then keeps no y.  da or db may be dy (not both).  An element that 8 bits
  * rounded up to 2^128 (BF16 and F32 above 3.2e38) is an infinity here. */
 ARK_API int ark_cuda_swiglu_backward(const void* dy, uint64_t lddy, int32_t type,
                                      const ark_act8* a8, const ark_act8* b8, void* da,
@@ -520,7 +520,8 @@ typedef struct ark_heads {
 /* The rotation (inverse: its backward) of q and k (k, out_k: NULL for q
  * alone).  positions: I32 or I64 [tokens], or NULL for token index modulo
  * seq_len.  A negative position marks a padding token: its inputs are not
- * read and its outputs are zero.  out_q / out_k may be q / k.  dim up to
+ * read and its outputs are zero.  out_q may be q and out_k k, but neither the
+ * other's, nor both the same.  dim up to
  * ARK_ROPE_MAX_DIM. */
 ARK_API int ark_cuda_rope(const ark_rope_plan* plan, const ark_heads* q, const ark_heads* k,
                           const ark_heads* out_q, const ark_heads* out_k, int32_t type,
@@ -543,8 +544,8 @@ ARK_API int ark_cuda_qk_norm_rope(const ark_rope_plan* plan, const ark_heads* q,
                                   int32_t pos_type, uint64_t seq_len, const ark_act8* q8,
                                   const ark_act8* k8, void* cuda_stream);
 /* Its backward.  dq, dk: gradients of the outputs; x from the checkpoints q8 /
- * k8, or else from q / k themselves (exactly one of the two).  out_dq / out_dk
- * may be dq / dk.  dgain_q, dgain_k [dim]: the gains' gradients, summed in
+ * k8, or else from q / k themselves (exactly one of the two).  out_dq may be
+ * dq and out_dk dk.  dgain_q, dgain_k [dim], apart from each other: the gains' gradients, summed in
  * FP32 over tokens and heads in a fixed order and rounded once, or added to
  * what is there.  workspace: ark_cuda_qk_norm_rope_workspace(dim) bytes of
  * the current device, 4-byte aligned. */

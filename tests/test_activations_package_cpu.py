@@ -65,3 +65,37 @@ def test_wide_checkpoints_need_room_for_both_halves():
     assert call(wide, p + 8, need[1]) == -2
     if need[0]:
         assert call(wide, p, need[0] - 1, dy_type=1) == -1
+
+
+def test_two_outputs_in_one_place_are_refused():
+    """da and db, the two outputs of a rotation or norm, and the two gains' gradients are written
+    at once: in one place they would be a mixture."""
+    import ctypes
+
+    from ark_b200 import _lib
+    L, by = _lib.lib(), ctypes.byref
+    p = [0x7F0000000000 + (i << 24) for i in range(8)]      # aligned addresses that nothing reads
+    plan = _lib.RopePlan()
+    assert L.ark_cuda_rope_plan(by(plan), 64, 0, 10000.0, 0, 1.0, 0.0, 32.0, 1.0) == 0
+
+    def heads(x):
+        return by(_lib.Heads(x, 4, 256, 64))
+
+    def rope(q, k, oq, ok, tokens=8, pos=p[6] + 4):         # a call that passes ends at the positions
+        return L.ark_cuda_rope(by(plan), heads(q), heads(k), heads(oq), heads(ok), 0, tokens, 64, pos, 4, 0, 0, None)
+
+    def back(oq, ok, gq, gk, ws=p[7] + 2):                  # or at the workspace
+        return L.ark_cuda_qk_norm_rope_backward(
+            by(plan), heads(p[0]), heads(p[1]), heads(oq), heads(ok), 0, 8, 64, None, None, heads(p[2]), heads(p[3]),
+            p[4], p[4], 0, 1e-6, None, 0, 8, gq, gk, 0, 0, ws, L.ark_cuda_qk_norm_rope_workspace(64), None)
+
+    assert back(p[0], p[1], p[4], p[5]) == -2 and back(p[0], p[1], p[4], p[4]) == -1
+    assert back(p[6], p[6], p[4], p[5]) == -1 and back(p[1], p[0], p[4], p[5]) == -1
+    assert back(p[1], p[6], p[4], p[5]) == -1
+    for bad in ((p[0], p[1], p[2], p[2]), (p[0], p[1], p[1], p[2]), (p[0], p[1], p[2], p[0]), (p[0], p[0], p[0], p[2])):
+        assert rope(*bad) == -1
+    assert rope(p[0], p[1], p[0], p[1]) == rope(p[0], p[0], p[1], p[2]) == -2
+    a = _lib.Act8(p[0], p[1], 8, 128, 0, 0)
+    sw = lambda da, db: L.ark_cuda_swiglu_backward(p[2], 128, 0, by(a), by(a), da, 128, db, 128, None, None)  # noqa: E731
+    assert sw(p[3], p[3]) == -1 and sw(p[3], p[4] + 1) == -2
+    assert rope(p[0], p[1], p[2], p[2], tokens=0, pos=p[6]) == 0
