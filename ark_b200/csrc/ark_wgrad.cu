@@ -48,11 +48,13 @@ constexpr int kAhead = 2;                     // steps of a team in flight
 // The tensor cores add 16 tokens at a time to a sum that is cut off to FP32, not
 // rounded: each addition may lose a unit of the last place, 2^-23 of the sum, and
 // always towards zero.  So one accumulator takes a bounded run of 64-token steps, and
-// runs are added by FP32 additions that round.  FP32 gradients: 32 steps, 128
-// additions.  16-bit ones: as many as lose an eighth of the type's half step, 2^-14 for
-// FP16 (512 additions) and 2^-11 for BF16 (4096).
-constexpr uint32_t kRun32 = 32, kRunF16 = 128, kRunBF16 = 1024;
-constexpr uint32_t kFewRuns = 4;              // accumulators of few_kernel
+// runs are added by FP32 additions that round.  FP32 gradients of the pairs: 16 steps,
+// 64 additions (4001 tokens of both signs, 2048 x 5504: off by 2.0e-7 in 77.0 us; 32
+// steps 4.4e-7 in 76.4, 8 steps 1.1e-7 in 81.5).  16-bit ones: as many as lose an
+// eighth of the type's half step, 2^-14 for FP16 (512 additions) and 2^-11 for BF16
+// (4096).  Few tiles: up to 32 steps in each of four accumulators.
+constexpr uint32_t kRun32 = 16, kRunF16 = 128, kRunBF16 = 1024;
+constexpr uint32_t kFewRuns = 4, kFewRun = 32;
 constexpr uint32_t kSleepNs = 1000000;
 constexpr long long kWaitClocks = 4000000000ll;   // 2 s
 
@@ -1069,7 +1071,7 @@ Way way_of(uint64_t tokens, uint64_t m, uint64_t n) {
     Way w = {false, 1, 1, 0, 0};
     uint64_t best = ~0ull;
     for (uint32_t p = 1; p <= 8 && p <= iters; p *= 2) {
-        if (ceil_div(iters, p) > kFewRuns * kRun32) continue;   // its accumulators take no more
+        if (ceil_div(iters, p) > kFewRuns * kFewRun) continue;   // its accumulators take no more
         const uint64_t t = ceil_div(few, few_fit(p)) * (6500 + 370 * ceil_div(iters, p));
         if (t < best) best = t, w.parts = p;
     }
@@ -1164,7 +1166,7 @@ int product(const Way& w, const ark_act8* x, const void* dy, int32_t dy_type, ui
     a.tiles = a.tiles_m * a.tiles_n;
     const uint32_t parts = w.parts;
     a.chunks = a.iters / parts / 16;
-    a.chunks = a.chunks < 1 ? 1 : a.chunks > kFewRuns ? kFewRuns : a.chunks;   // of at most kRun32 steps
+    a.chunks = a.chunks < 1 ? 1 : a.chunks > kFewRuns ? kFewRuns : a.chunks;   // of at most kFewRun steps
     if (dy_type == ARK_TYPE_F16)
         return x->kind == kE4M3 ? launch_few<__half, kE4M3>(map, a, parts, s)
                                 : launch_few<__half, kInt8>(map, a, parts, s);
