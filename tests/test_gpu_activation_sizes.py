@@ -47,7 +47,7 @@ def whole(tokens, nin, nout, dtype, seed):
     ("few tiles, one accumulator", 500, 700, 700, False, False),
     ("few tiles, two accumulators", 2048, 768, 2048, False, False),
     ("few tiles, several accumulators of clusters", 8000, 1000, 1001, False, False),
-    ("pairs, one run where FP32 has three", 4200, 2048, 5504, True, False),
+    ("pairs, one run where FP32 has several", 4200, 2048, 5504, True, False),
     ("pairs, rows of any boundary", 4096, 2048, 5501, True, False),
     ("pairs, dY realigned, an odd height", 2100, 2049, 5503, True, False),
     ("pairs, runs of FP16", 8200, 2048, 2301, True, False),
